@@ -182,6 +182,144 @@ int knhip_kernel_run(const knhip_kernel *kernel, void *stream, void *const *ptrs
 int knhip_kernel_info(const knhip_kernel *kernel, char *strategy, size_t cap, size_t *needed, unsigned *grid, unsigned *block);
 void knhip_kernel_free(knhip_kernel *kernel);
 
+/* ---- serving a decoder token by token, on caller-owned device memory ----------------------------------------------
+ * No counterpart in the reference. Four operators that make one step of a decoder outside any executor: new keys and
+ * values go into a cache (and come back out of it), queries attend over that cache, whole prompts attend over
+ * themselves under caps, distance bias and masks, and a token is drawn from the logits. Like knhip_batched_mat_mul the
+ * calls return once their work is queued on `stream`, allocate nothing, and take scratch memory from `workspace` (256
+ * byte aligned, as many bytes as the operator's _workspace_bytes says, untouched until the work has run; calls whose
+ * work may overlap need one each, and so do two captured graphs that may). They can be captured into a HIP graph.
+ * Addresses are device addresses with the alignment of their element; strides are in elements, may be zero or negative
+ * in operands that are only read, and the axis along a row's `width` is contiguous. Sizes, codes and addresses are checked
+ * on the host before anything is launched. Lengths, slots and page numbers are device data and cannot be: entries out of
+ * range are skipped, as the operators say, and never reach outside the buffers. */
+
+/* Keys and values of past tokens in pages of `page_tokens` tokens: key (page, head, token, i) is element
+ * page * page_stride + head * head_stride + token * token_stride + i of `k`, and the values lie in `v` the same way
+ * (innermost first, an unpadded cache is [pages, heads, page_tokens, width]; a cache without pages is one of a single
+ * page per sequence). KNHIP_F16 keeps the rows as they are. KNHIP_I8 keeps a row x as whole numbers q and one f32 scale:
+ * scale = max |x| / 127, q = x / scale rounded to the nearest, ties to even (all zeros where the scale is zero), standing
+ * for q * scale; the scales are dense arrays [pages, heads, page_tokens]. `width` is a multiple of 16 up to 256, `k` and `v`
+ * are 16 byte aligned and so are the strides in bytes. pages * page_tokens stays below 2^31. */
+typedef struct {
+    int dtype; /* KNHIP_I8 or KNHIP_F16 */
+    int pages, heads, page_tokens, width;
+    void *k;
+    void *v;
+    int64_t page_stride, head_stride, token_stride;
+    float *k_scales; /* KNHIP_I8 only */
+    float *v_scales;
+} knhip_kv_cache;
+/* Rows of keys and values outside the cache, [tokens, heads, width] with the cache's heads and width, and the slot
+ * (page * page_tokens + token inside the page) of each token. */
+typedef struct {
+    int dtype; /* KNHIP_F16 or KNHIP_F32 */
+    int tokens;
+    void *k;
+    int64_t k_token_stride, k_head_stride;
+    void *v;
+    int64_t v_token_stride, v_head_stride;
+    const int32_t *slots;
+} knhip_cache_rows;
+/* Writes the rows into their slots. A token with a slot outside 0 .. pages * page_tokens - 1 is left out (the padding of
+ * a batch: -1); the slots that are written must differ from each other. Finite values beyond +-65504, the range of f16,
+ * and infinities are kept as +-65504, a NaN as 0 in KNHIP_I8 and as itself in KNHIP_F16. */
+int knhip_cache_write(int device, void *stream, const knhip_kv_cache *cache, const knhip_cache_rows *rows);
+/* Reads the rows back: rows->k / rows->v are written with what the slots stand for, rounded once to rows->dtype; zeros
+ * for a slot outside the cache. A slot may occur any number of times; the strides may not let two rows share memory. */
+int knhip_cache_read(int device, void *stream, const knhip_kv_cache *cache, const knhip_cache_rows *rows);
+
+/* Attention of the newest tokens of `batch` sequences over a cache. Sequence b is the `prefix_tokens` tokens that all
+ * sequences share, in the pages prefix_table[0 .. ceil(prefix_tokens / page_tokens) - 1], followed by lengths[b] tokens
+ * of its own, in the pages tables[b * table_stride + 0 .. table_pages - 1]; its last `queries` tokens are the queries (their
+ * keys and values already in the cache). Query t of sequence b stands at place p = prefix_tokens + lengths[b] - queries
+ * + t and sees the places j <= p, with a window only j > p - window. Head h reads head h / (heads / cache.heads) of
+ * the cache. With s = scale * (q . k_j):
+ *     z_j = cap > 0 ? cap * tanh(s / cap) : s, less slopes[h] * (p - j) where slopes are given
+ *     out = sum_j softmax(z)_j v_j, or zeros where nothing is seen
+ * A query that would stand before the sequence's own first token (lengths[b] < queries: a padded batch) gives zeros.
+ * Lengths beyond table_pages * page_tokens count as that, negative ones as 0; the keys of a page number outside the cache
+ * are not seen. q and out are f16; the shared tokens are read once for all sequences. Sums and statistics are f32, the
+ * weights enter the second product as f16. width: a multiple of 16 up to 128. */
+typedef struct {
+    int batch, queries, heads;
+    knhip_kv_cache cache;
+    const void *q; /* [batch, queries, heads, width] */
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    void *out; /* the same shape */
+    int64_t out_batch_stride, out_token_stride, out_head_stride;
+    const int32_t *lengths; /* [batch] */
+    const int32_t *tables;  /* [batch, table_pages] */
+    int64_t table_stride;
+    int table_pages;
+    int prefix_tokens;           /* 0: nothing shared */
+    const int32_t *prefix_table; /* may be NULL when prefix_tokens is 0 */
+    float scale;
+    float cap;           /* 0: none */
+    const float *slopes; /* [heads], NULL: none */
+    int window;          /* 0: none */
+} knhip_cached_attention_args;
+int knhip_cached_attention_workspace_bytes(const knhip_cached_attention_args *args, size_t *bytes);
+int knhip_cached_attention(int device, void *stream, const knhip_cached_attention_args *args, void *workspace, size_t workspace_bytes);
+
+/* Attention of whole prompts, f16: q [batch, queries, heads, width], k and v [batch, keys, kv_heads, width], out like q.
+ * Head h reads head h / (heads / kv_heads) of k and v. Query i stands at place p = i + keys - queries (the queries are
+ * the last ones of the keys). It sees key j when all of these hold:
+ *     causal is 0, or j <= p, or j < prefix[b]                (a prefix mask: the first prefix[b] keys are seen by all)
+ *     window is 0, or j > p - window
+ *     spans is NULL, or spans[b, i, 0] <= j < spans[b, i, 1]  (a document mask: first and one past the last key of the
+ *                                                             query's document; an empty span is a query of padding)
+ * z, out and the precision are those of knhip_cached_attention, with slopes[h] * |p - j|. What nobody sees may hold anything,
+ * NaN too. width: a multiple of 8 up to 128. */
+typedef struct {
+    int batch, queries, keys, heads, kv_heads, width;
+    const void *q;
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    const void *k;
+    int64_t k_batch_stride, k_token_stride, k_head_stride;
+    const void *v;
+    int64_t v_batch_stride, v_token_stride, v_head_stride;
+    void *out;
+    int64_t out_batch_stride, out_token_stride, out_head_stride;
+    float scale;
+    float cap;           /* 0: none */
+    const float *slopes; /* [heads], NULL: none */
+    int causal;
+    int window;            /* 0: none */
+    const int32_t *spans;  /* [batch, queries, 2] dense, NULL: none */
+    const int32_t *prefix; /* [batch], NULL: none */
+} knhip_attention_args;
+int knhip_attention_workspace_bytes(const knhip_attention_args *args, size_t *bytes);
+int knhip_attention(int device, void *stream, const knhip_attention_args *args, void *workspace, size_t workspace_bytes);
+
+/* Draws one token per row of logits [rows, vocab] from given random numbers. Of a row x with maximum m:
+ *     w_i = exp((x_i - m) / temperature); a temperature of 0 or less takes the most probable token, the first of several
+ *     top_k > 0: only the top_k most probable tokens stay
+ *     top_p < 1: of those, in falling order, only the tokens before which less than top_p of their sum lies
+ *     min_p > 0: of those, only the tokens with w_i >= min_p
+ * The most probable token always stays; of equal logits the lower index counts as the more probable. The token is the
+ * first index at which the sum of the kept w, taken in the order of the indices, exceeds uniform[r] times the whole sum;
+ * its probability is its share of that sum. -inf and NaN are never drawn, +inf counts as infinitely more probable than any
+ * finite logit; a row without anything to draw gives token -1 and probability 0. uniform lies in [0, 1) (other values
+ * count as the nearest one in it). The w are f64, held in 64 bit fixed point: rounded to multiples of 2^-(62 - l) for a vocab
+ * of up to 2^l, so that their sums are exact and the same in any order (a w below half a step, 2^-43 or less, is never
+ * drawn). Parameters with a NULL address are off for every row (temperature: 1). vocab: up to 2^20. */
+typedef struct {
+    int dtype; /* KNHIP_F16 or KNHIP_F32 */
+    int rows, vocab;
+    const void *logits;
+    int64_t row_stride;
+    const float *temperature; /* [rows], NULL: 1 */
+    const int32_t *top_k;     /* [rows], NULL or <= 0: off */
+    const float *top_p;       /* [rows], NULL or >= 1: off */
+    const float *min_p;       /* [rows], NULL or <= 0: off */
+    const float *uniform;     /* [rows] */
+    int32_t *tokens;          /* [rows] */
+    float *probabilities;     /* [rows], may be NULL */
+} knhip_sample_args;
+int knhip_sample_workspace_bytes(const knhip_sample_args *args, size_t *bytes);
+int knhip_sample(int device, void *stream, const knhip_sample_args *args, void *workspace, size_t workspace_bytes);
+
 /* ---- graph (kn-graph/src/graph.rs) ------------------------------------------------------------------------- */
 typedef struct knhip_graph knhip_graph;
 typedef uint32_t knhip_value; /* index of a value inside its graph; values are append-only (graph.rs:86-91) */

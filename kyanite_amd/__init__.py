@@ -9,6 +9,9 @@ from .runtime import (STATIC_SCRATCH_BYTES, DeviceBuffer, HipEvent, HipStream, P
                       batched_mat_mul_static, batched_mat_mul_workspace_bytes, matmul_args)
 from .device_tensor import DeviceTensor, StridedShape
 from .autokernel import GatherKernel, LayernormKernel, ReduceKernel, ScalarKernel, SoftmaxKernel
+from .serving import (attention, attention_args, attention_workspace_bytes, cache_read, cache_rows, cache_write, cached_attention,
+                      cached_attention_args, cached_attention_workspace_bytes, kv_cache, sample, sample_args,
+                      sample_workspace_bytes)
 from .graph import (BATCH, BINARY_ALL, REDUCE_ALL, UNARY_ALL, BinaryOp, DType, Graph, OpKind, OptimizerSettings,
                     ReduceOp, Size, UnaryOp, Value, optimize_graph, shape)
 
@@ -19,4 +22,6 @@ __all__ = [
     "DeviceBuffer", "HipEvent", "HipStream", "PinnedMem", "batched_mat_mul", "batched_mat_mul_workspace_bytes", "matmul_args",
     "STATIC_SCRATCH_BYTES", "batched_mat_mul_static",
     "DeviceTensor", "StridedShape", "ScalarKernel", "ReduceKernel", "SoftmaxKernel", "LayernormKernel", "GatherKernel",
+    "attention", "attention_args", "attention_workspace_bytes", "cache_read", "cache_rows", "cache_write", "cached_attention",
+    "cached_attention_args", "cached_attention_workspace_bytes", "kv_cache", "sample", "sample_args", "sample_workspace_bytes",
 ]

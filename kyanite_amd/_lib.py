@@ -43,6 +43,44 @@ class MatmulArgsT(Structure):
                 ("c", c_void_p), ("c_batch_stride", c_int64), ("c_row_stride", c_int64), ("c_col_stride", c_int64)]
 
 
+class KvCacheT(Structure):
+    _fields_ = [("dtype", c_int), ("pages", c_int), ("heads", c_int), ("page_tokens", c_int), ("width", c_int),
+                ("k", c_void_p), ("v", c_void_p), ("page_stride", c_int64), ("head_stride", c_int64),
+                ("token_stride", c_int64), ("k_scales", c_void_p), ("v_scales", c_void_p)]
+
+
+class CacheRowsT(Structure):
+    _fields_ = [("dtype", c_int), ("tokens", c_int), ("k", c_void_p), ("k_token_stride", c_int64),
+                ("k_head_stride", c_int64), ("v", c_void_p), ("v_token_stride", c_int64), ("v_head_stride", c_int64),
+                ("slots", c_void_p)]
+
+
+class CachedAttentionArgsT(Structure):
+    _fields_ = [("batch", c_int), ("queries", c_int), ("heads", c_int), ("cache", KvCacheT), ("q", c_void_p),
+                ("q_batch_stride", c_int64), ("q_token_stride", c_int64), ("q_head_stride", c_int64),
+                ("out", c_void_p), ("out_batch_stride", c_int64), ("out_token_stride", c_int64),
+                ("out_head_stride", c_int64), ("lengths", c_void_p), ("tables", c_void_p), ("table_stride", c_int64),
+                ("table_pages", c_int), ("prefix_tokens", c_int), ("prefix_table", c_void_p), ("scale", c_float),
+                ("cap", c_float), ("slopes", c_void_p), ("window", c_int)]
+
+
+class AttentionArgsT(Structure):
+    _fields_ = [("batch", c_int), ("queries", c_int), ("keys", c_int), ("heads", c_int), ("kv_heads", c_int),
+                ("width", c_int), ("q", c_void_p), ("q_batch_stride", c_int64), ("q_token_stride", c_int64),
+                ("q_head_stride", c_int64), ("k", c_void_p), ("k_batch_stride", c_int64),
+                ("k_token_stride", c_int64), ("k_head_stride", c_int64), ("v", c_void_p),
+                ("v_batch_stride", c_int64), ("v_token_stride", c_int64), ("v_head_stride", c_int64),
+                ("out", c_void_p), ("out_batch_stride", c_int64), ("out_token_stride", c_int64),
+                ("out_head_stride", c_int64), ("scale", c_float), ("cap", c_float), ("slopes", c_void_p),
+                ("causal", c_int), ("window", c_int), ("spans", c_void_p), ("prefix", c_void_p)]
+
+
+class SampleArgsT(Structure):
+    _fields_ = [("dtype", c_int), ("rows", c_int), ("vocab", c_int), ("logits", c_void_p), ("row_stride", c_int64),
+                ("temperature", c_void_p), ("top_k", c_void_p), ("top_p", c_void_p), ("min_p", c_void_p),
+                ("uniform", c_void_p), ("tokens", c_void_p), ("probabilities", c_void_p)]
+
+
 class ExecutorOptionsT(Structure):
     _fields_ = ([("struct_bytes", c_size_t)] +
                 [(name, c_int) for name in (
@@ -105,6 +143,14 @@ SIGNATURES = {
     "knhip_gather_kernel_new": [c_int, POINTER(TensorT), POINTER(TensorT), POINTER(TensorT), c_size_t, POINTER(c_void_p)],
     "knhip_kernel_run": [c_void_p, c_void_p, POINTER(c_void_p), c_size_t],
     "knhip_kernel_info": [c_void_p, c_char_p, c_size_t, PZ, POINTER(ctypes.c_uint), POINTER(ctypes.c_uint)],
+    "knhip_cache_write": [c_int, c_void_p, POINTER(KvCacheT), POINTER(CacheRowsT)],
+    "knhip_cache_read": [c_int, c_void_p, POINTER(KvCacheT), POINTER(CacheRowsT)],
+    "knhip_cached_attention_workspace_bytes": [POINTER(CachedAttentionArgsT), PZ],
+    "knhip_cached_attention": [c_int, c_void_p, POINTER(CachedAttentionArgsT), c_void_p, c_size_t],
+    "knhip_attention_workspace_bytes": [POINTER(AttentionArgsT), PZ],
+    "knhip_attention": [c_int, c_void_p, POINTER(AttentionArgsT), c_void_p, c_size_t],
+    "knhip_sample_workspace_bytes": [POINTER(SampleArgsT), PZ],
+    "knhip_sample": [c_int, c_void_p, POINTER(SampleArgsT), c_void_p, c_size_t],
     "knhip_graph_new": [POINTER(G)],
     "knhip_graph_clone": [G, POINTER(G)],
     "knhip_graph_deserialize": [POINTER(c_uint8), c_size_t, POINTER(G)],

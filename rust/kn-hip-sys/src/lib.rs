@@ -58,6 +58,120 @@ pub struct knhip_matmul_args {
     pub c_col_stride: i64,
 }
 
+/// Keys and values of past tokens, in pages.
+#[repr(C)]
+#[derive(Debug, Copy, Clone)]
+pub struct knhip_kv_cache {
+    pub dtype: c_int,
+    pub pages: c_int,
+    pub heads: c_int,
+    pub page_tokens: c_int,
+    pub width: c_int,
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub page_stride: i64,
+    pub head_stride: i64,
+    pub token_stride: i64,
+    pub k_scales: *mut f32,
+    pub v_scales: *mut f32,
+}
+
+/// Rows that go into a cache or come out of it.
+#[repr(C)]
+#[derive(Debug, Copy, Clone)]
+pub struct knhip_cache_rows {
+    pub dtype: c_int,
+    pub tokens: c_int,
+    pub k: *mut c_void,
+    pub k_token_stride: i64,
+    pub k_head_stride: i64,
+    pub v: *mut c_void,
+    pub v_token_stride: i64,
+    pub v_head_stride: i64,
+    pub slots: *const i32,
+}
+
+/// Attention of the newest tokens of a batch over a cache.
+#[repr(C)]
+#[derive(Debug, Copy, Clone)]
+pub struct knhip_cached_attention_args {
+    pub batch: c_int,
+    pub queries: c_int,
+    pub heads: c_int,
+    pub cache: knhip_kv_cache,
+    pub q: *const c_void,
+    pub q_batch_stride: i64,
+    pub q_token_stride: i64,
+    pub q_head_stride: i64,
+    pub out: *mut c_void,
+    pub out_batch_stride: i64,
+    pub out_token_stride: i64,
+    pub out_head_stride: i64,
+    pub lengths: *const i32,
+    pub tables: *const i32,
+    pub table_stride: i64,
+    pub table_pages: c_int,
+    pub prefix_tokens: c_int,
+    pub prefix_table: *const i32,
+    pub scale: f32,
+    pub cap: f32,
+    pub slopes: *const f32,
+    pub window: c_int,
+}
+
+/// Attention of whole prompts.
+#[repr(C)]
+#[derive(Debug, Copy, Clone)]
+pub struct knhip_attention_args {
+    pub batch: c_int,
+    pub queries: c_int,
+    pub keys: c_int,
+    pub heads: c_int,
+    pub kv_heads: c_int,
+    pub width: c_int,
+    pub q: *const c_void,
+    pub q_batch_stride: i64,
+    pub q_token_stride: i64,
+    pub q_head_stride: i64,
+    pub k: *const c_void,
+    pub k_batch_stride: i64,
+    pub k_token_stride: i64,
+    pub k_head_stride: i64,
+    pub v: *const c_void,
+    pub v_batch_stride: i64,
+    pub v_token_stride: i64,
+    pub v_head_stride: i64,
+    pub out: *mut c_void,
+    pub out_batch_stride: i64,
+    pub out_token_stride: i64,
+    pub out_head_stride: i64,
+    pub scale: f32,
+    pub cap: f32,
+    pub slopes: *const f32,
+    pub causal: c_int,
+    pub window: c_int,
+    pub spans: *const i32,
+    pub prefix: *const i32,
+}
+
+/// One drawn token per row of logits.
+#[repr(C)]
+#[derive(Debug, Copy, Clone)]
+pub struct knhip_sample_args {
+    pub dtype: c_int,
+    pub rows: c_int,
+    pub vocab: c_int,
+    pub logits: *const c_void,
+    pub row_stride: i64,
+    pub temperature: *const f32,
+    pub top_k: *const i32,
+    pub top_p: *const f32,
+    pub min_p: *const f32,
+    pub uniform: *const f32,
+    pub tokens: *mut i32,
+    pub probabilities: *mut f32,
+}
+
 /// What an executor is built with beyond (device, graph, batch size); fill it with `knhip_executor_options_default`.
 #[repr(C)]
 #[derive(Debug, Copy, Clone)]
@@ -178,6 +292,19 @@ extern "C" {
     pub fn knhip_kernel_info(kernel: *const knhip_kernel, strategy: *mut c_char, cap: usize, needed: *mut usize, grid: *mut u32,
                              block: *mut u32) -> c_int;
     pub fn knhip_kernel_free(kernel: *mut knhip_kernel);
+
+    // serving a decoder token by token
+    pub fn knhip_cache_write(device: c_int, stream: *mut c_void, cache: *const knhip_kv_cache, rows: *const knhip_cache_rows) -> c_int;
+    pub fn knhip_cache_read(device: c_int, stream: *mut c_void, cache: *const knhip_kv_cache, rows: *const knhip_cache_rows) -> c_int;
+    pub fn knhip_cached_attention_workspace_bytes(args: *const knhip_cached_attention_args, bytes: *mut usize) -> c_int;
+    pub fn knhip_cached_attention(device: c_int, stream: *mut c_void, args: *const knhip_cached_attention_args, workspace: *mut c_void,
+                                  workspace_bytes: usize) -> c_int;
+    pub fn knhip_attention_workspace_bytes(args: *const knhip_attention_args, bytes: *mut usize) -> c_int;
+    pub fn knhip_attention(device: c_int, stream: *mut c_void, args: *const knhip_attention_args, workspace: *mut c_void,
+                           workspace_bytes: usize) -> c_int;
+    pub fn knhip_sample_workspace_bytes(args: *const knhip_sample_args, bytes: *mut usize) -> c_int;
+    pub fn knhip_sample(device: c_int, stream: *mut c_void, args: *const knhip_sample_args, workspace: *mut c_void,
+                        workspace_bytes: usize) -> c_int;
 
     // layout algebra (kn-cuda-eval/src/shape.rs:25-285), computed by the library
     pub fn knhip_strided_flags(shape: *const usize, strides: *const i64, rank: usize, simple: *mut c_int, dense: *mut c_int) -> c_int;
