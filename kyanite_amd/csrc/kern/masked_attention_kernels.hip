@@ -1,9 +1,24 @@
 // Attention over a paged cache and of whole prompts under caps, distance bias and masks (knhip_cached_attention,
-// knhip_attention).
+// knhip_attention), f16 or quantised keys and values, on the CDNA4 matrix cores.
 //
-// Every mask of either operator is an interval of places per query, [lo, hi): causal and prefix mask end it, window and
-// document begin it (serving_kernels.h). The softmax runs with a running maximum and sum in f32.
+// Every mask of either operator is an interval [lo, hi) of keys per query: causal and prefix mask end it, window and document
+// begin it. Blocks of keys that no query of a workgroup sees are not fetched, blocks that all of them see whole run
+// without a comparison.
+//
+// The rows of a product are the queries that read the same head of keys: all heads of its group times all tokens, so
+// that a block of keys is fetched once for them. Three kernels:
+//   tile_attention_kernel   128 rows per workgroup: prompts, prompts over a cache, and the shared prefix of a batch, whose
+//                           rows are the queries of ALL sequences
+//   row_attention_kernel    up to 16 or 32 rows per workgroup: the few queries of one sequence over its own keys
+//   join_attention_kernel   the softmax of parts: keys are split between workgroups where rows are few, and a sequence with
+//                           a prefix has its own part and the prefix's
+// Scores are computed transposed, S^T = K Q^T, so that a lane owns a query and the accumulators of S^T are the operands of
+// O^T += V^T P^T. The softmax runs in f32 in units of log2, with a running reference that follows the maximum lazily:
+// it moves when a score exceeds it by more than 2^8, weights are at most 256 until then.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
 
 #include "../serving_kernels.h"
 
@@ -11,129 +26,1089 @@ namespace kn {
 
 namespace {
 
+typedef _Float16 half_t;
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+// rows of prompts may start at any element: the hardware takes under-aligned 128 bit accesses
 typedef _Float16 halfx8_any __attribute__((ext_vector_type(8), aligned(2)));
+typedef _Float16 halfx4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 
-constexpr int WAVES = 4;
 constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float SLACK = 8.0f;
+constexpr int WAVES = 4;
 
-// One wave per query and head: lanes are keys for the scores and dims for the weighted sum.
-__global__ __launch_bounds__(64 * WAVES) void masked_attention_kernel(ServingAttentionParams p) {
-    __shared__ float qs[WAVES][128], ps[WAVES][64];
-    __shared__ long long vo[WAVES][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long row = (long long) blockIdx.x * WAVES + wave;
-    const bool live_row = row < (long long) p.batch * p.queries * p.heads;
-    const long long r = live_row ? row : 0;
-    const int head = (int) (r % p.heads), t = (int) (r / p.heads % p.queries), b = (int) (r / p.heads / p.queries);
-    const int kv_head = head / (p.heads / p.kv_heads);
-    const _Float16 *q = (const _Float16 *) p.q + b * p.q_batch + t * p.q_token + head * p.q_head;
-    for (int d = lane; d < p.width; d += 64) qs[wave][d] = (float) q[d];
-    __syncthreads();
+// ---- which keys a query sees ---------------------------------------------------------------------------------------
 
-    int lo = 0, hi, at, keys[2] = {0, 0};
-    if (p.paged) {
-        const int length = min(max(p.lengths[b], 0), p.table_tokens);
-        const int own = length - p.queries + t;
-        at = p.prefix_tokens + own;
-        keys[0] = p.prefix_tokens;
-        keys[1] = length;
-        hi = own < 0 ? 0 : at + 1;
-        if (p.window) lo = max(lo, at - p.window + 1);
+enum Stretch { PROMPT, OWN, PREFIX };  // whose keys a workgroup reads
+
+struct Row {
+    int b, t, head;
+    int at;      // place of the query, counted from the first key of the stretch
+    int lo, hi;  // the keys of the stretch that it sees
+};
+
+__device__ __forceinline__ int own_length(const ServingAttentionParams &p, int b) { return min(max(p.lengths[b], 0), p.table_tokens); }
+
+// Row `r` of kv head `kv_head`: (token, head of the group) of sequence `b`, of all sequences for the prefix
+template <int STRETCH>
+__device__ __forceinline__ Row row_of(const ServingAttentionParams &p, unsigned r, int b, int kv_head) {
+    Row w;
+    const unsigned token = p.group_div.div(r);
+    w.head = kv_head * (int) p.group_div.d + (int) (r - token * p.group_div.d);
+    w.b = b;
+    w.t = (int) token;
+    if (STRETCH == PREFIX) {
+        w.b = (int) p.queries_div.div(token);
+        w.t = (int) (token - (unsigned) w.b * p.queries_div.d);
+    }
+    w.lo = 0;
+    if (STRETCH == PROMPT) {
+        w.at = w.t + p.keys - p.queries;
+        w.hi = p.keys;
+        if (p.causal) w.hi = min(w.hi, max(w.at + 1, p.prefix ? p.prefix[w.b] : 0));
     } else {
-        at = t + p.keys - p.queries;
-        keys[1] = hi = p.keys;
-        if (p.causal) hi = min(hi, max(at + 1, p.prefix ? p.prefix[b] : 0));
-        if (p.window) lo = max(lo, at - p.window + 1);
-        if (p.spans) {
-            lo = max(lo, p.spans[2 * ((long long) b * p.queries + t)]);
-            hi = min(hi, p.spans[2 * ((long long) b * p.queries + t) + 1]);
-        }
+        const int own = own_length(p, w.b) - p.queries + w.t;  // below 0: a query of padding
+        w.at = STRETCH == OWN ? own : p.prefix_tokens + own;
+        w.hi = own < 0 ? 0 : STRETCH == OWN ? own + 1 : p.prefix_tokens;
     }
-    const float slope = p.slopes ? p.slopes[head] : 0.0f;
-    float top = -INFINITY, sum = 0.0f, acc[2] = {0.0f, 0.0f};
-    for (int part = 0; part < 2; part++) {
-        const int base = part ? keys[0] : 0;  // place of the stretch's first key
-        const int first = max(lo - base, 0), end = min(hi - base, keys[part]);
-        for (int j0 = first; j0 < end; j0 += 64) {
-            const int j = j0 + lane;
-            float s = -INFINITY;
-            long long v_at = -1;
-            if (j < end) {
-                long long k_at, scale_at = 0;
-                bool there = true;
-                if (p.paged) {
-                    const unsigned n = p.page_tokens.div((unsigned) j), in = (unsigned) j - n * p.page_tokens.d;
-                    const int page = part ? p.tables[b * p.table_stride + n] : p.prefix_table[n];
-                    there = (unsigned) page < (unsigned) p.pages;
-                    k_at = page * p.k_page + kv_head * p.k_head + in * p.k_token;
-                    v_at = page * p.v_page + kv_head * p.v_head + in * p.v_token;
-                    scale_at = ((long long) page * p.kv_heads + kv_head) * p.page_tokens.d + in;
+    if (p.window) w.lo = max(w.lo, w.at - p.window + 1);
+    if (STRETCH == PROMPT && p.spans) {
+        const int2 span = *(const int2 *) (p.spans + 2 * ((long long) w.b * p.queries + w.t));
+        w.lo = max(w.lo, span.x);
+        w.hi = min(w.hi, span.y);
+    }
+    if (w.lo >= w.hi) w.lo = w.hi = 0;
+    return w;
+}
+
+// tanh(x) = 1 - 2 / (1 + e^(2 x)): absolute error below 2^-22, and exact at both ends (e^(2 x) = 0 or infinity)
+__device__ __forceinline__ float tanh_fast(float x) {
+    return __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * (2.0f * LOG2E))), 1.0f);
+}
+
+// four keys (consecutive rows of the staged V) of one dim: 16 lanes hand in the addresses of 4 dims of 4 rows each
+__device__ __forceinline__ halfx4 lds_read_transposed(const half_t *p) {
+    return __builtin_bit_cast(halfx4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *) p));
+}
+
+__device__ __forceinline__ bool not_finite(halfx8 x) {
+    const uint4 u = __builtin_bit_cast(uint4, x);
+    unsigned any = 0;
+    for (unsigned w : {u.x, u.y, u.z, u.w}) {
+        any |= (w & 0x7c00u) == 0x7c00u;
+        any |= (w & 0x7c000000u) == 0x7c000000u;
+    }
+    return any;
+}
+
+__device__ __forceinline__ halfx8 finite_or_zero(halfx8 x) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = x[e] - x[e] == (half_t) 0.0f ? x[e] : (half_t) 0.0f;
+    return x;
+}
+
+// ---- 128 rows per workgroup ----------------------------------------------------------------------------------------
+
+// Four waves of 32 rows each walk all blocks of 64 keys, which they stage together in one of two LDS buffers, one barrier
+// per block: the block after the current one is in flight in registers meanwhile. WP: the width, padded to 64 or 128 with
+// zeros. I8: keys and values are dequantised (f32 product, one rounding to f16) as they are staged. SHAPED: with cap or
+// distance bias.
+template <int WP, int STRETCH, bool I8, bool SHAPED>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_attention_kernel(ServingAttentionParams p) {
+    constexpr int BKEYS = 64, THREADS = 64 * WAVES;
+    constexpr int PIECE = I8 ? 16 : 8;        // elements per 128 bit load
+    constexpr int C = WP / PIECE;             // loads per row
+    constexpr int VECS = BKEYS * C / THREADS;  // of K and of V, per lane and block
+    constexpr int KS = WP + 8, VS = WP == 128 ? 160 : 96;  // halves per staged row: bank-conflict free reads
+    constexpr int STAGE = BKEYS * (KS + VS);
+    constexpr int OS = WP + 8, WAVE_ROWS = 32 * OS;
+    constexpr int DT = WP / 32, QC = WP / 8;
+    static_assert(2 * STAGE >= WAVES * WAVE_ROWS && VECS >= 1, "unsupported shape");
+    constexpr bool PAGED = STRETCH != PROMPT;
+    __shared__ __attribute__((aligned(16))) half_t lds[2 * STAGE];
+    __shared__ unsigned long long gone_s[2][WAVES], bad_s[2][WAVES];
+    __shared__ int range_s[WAVES][4];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 31, h = lane >> 5;
+    // workgroups of one head of keys are a multiple of the (sequence, head) pairs apart: with 8 pairs or a multiple of them
+    // they run on one XCD and share its L2; the last tiles, with the most keys under a causal mask, come first
+    const unsigned pairs = (unsigned) (STRETCH == PREFIX ? 1 : p.batch) * p.kv_heads;
+    const unsigned pair = blockIdx.x % pairs, slab = blockIdx.x / pairs;
+    const int tile = (int) (gridDim.x / pairs) - 1 - (int) slab, kv_head = (int) (pair % p.kv_heads), b = (int) (pair / p.kv_heads);
+    const unsigned rows = (unsigned) (STRETCH == PREFIX ? p.batch : 1) * p.queries * p.group_div.d;
+    const int split = blockIdx.y, splits = gridDim.y;
+
+    const unsigned first_row = (unsigned) tile * 128 + wave * 32;
+    const unsigned row = first_row + c, row_c = min(row, rows - 1);
+    const Row w = row_of<STRETCH>(p, row_c, b, kv_head);
+
+    // ---- the blocks that any of the 128 rows needs, and those that all of them see whole
+    int from, end, whole_from, whole_end;
+    {
+        const bool sees = w.hi > w.lo;
+        int a[4] = {sees ? w.lo : INT_MAX, -(sees ? w.hi : 0), -w.lo, w.hi};
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1)
+#pragma unroll
+            for (int i = 0; i < 4; i++) a[i] = min(a[i], __shfl_xor(a[i], m));
+        if (lane == 0)
+#pragma unroll
+            for (int i = 0; i < 4; i++) range_s[wave][i] = a[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; i++) a[i] = __builtin_amdgcn_readfirstlane(min(min(range_s[0][i], range_s[1][i]), min(range_s[2][i], range_s[3][i])));
+        from = a[0];
+        end = -a[1];
+        whole_from = -a[2];
+        whole_end = a[3];
+    }
+    const int count = STRETCH == PROMPT ? p.keys : STRETCH == OWN ? own_length(p, b) : p.prefix_tokens;
+    int first_block = from < end ? from / BKEYS : 0, end_block = from < end ? (end + BKEYS - 1) / BKEYS : 0;
+    if (splits > 1) {  // this workgroup's share of the blocks
+        const int each = (end_block - first_block + splits - 1) / splits;
+        first_block = min(first_block + split * each, end_block);
+        end_block = min(first_block + each, end_block);
+    }
+
+    // ---- global -> registers -> LDS
+    const int *table = STRETCH == OWN ? p.tables + b * p.table_stride : p.prefix_table;
+    const char *kb = (const char *) p.k, *vb = (const char *) p.v;
+    constexpr int ELEM = I8 ? 1 : 2;
+    if (STRETCH == PROMPT) {
+        kb += (b * p.k_batch + kv_head * p.k_head) * ELEM;
+        vb += (b * p.v_batch + kv_head * p.v_head) * ELEM;
+    } else {
+        kb += kv_head * p.k_head * ELEM;
+        vb += kv_head * p.v_head * ELEM;
+    }
+    const int stage_row = (int) threadIdx.x / C, part = (int) threadIdx.x % C;
+    constexpr int ROW_STEP = THREADS / C;  // rows between a lane's loads
+    const bool part_live = part * PIECE < p.width;
+    uint4 kreg[VECS], vreg[VECS];
+    float kscale[VECS], vscale[VECS];
+    int pages[VECS];
+    unsigned gone = 0;  // of the block in the registers: the lane's rows that are not there
+    auto look_up = [&](int block) {  // the page numbers of a block, ahead of its loads
+        if (!PAGED) return;
+#pragma unroll
+        for (int i = 0; i < VECS; i++) {
+            const int j = block * BKEYS + stage_row + ROW_STEP * i;
+            pages[i] = j < count ? table[p.page_tokens.div((unsigned) j)] : -1;
+        }
+    };
+    auto fetch = [&](int block) {
+        gone = 0;
+#pragma unroll
+        for (int i = 0; i < VECS; i++) {
+            const int j = block * BKEYS + stage_row + ROW_STEP * i;
+            bool there = j < count;
+            long long k_at, v_at, s_at = 0;
+            if (PAGED) {
+                there = (unsigned) pages[i] < (unsigned) p.pages;
+                const unsigned in = (unsigned) j - p.page_tokens.div((unsigned) j) * p.page_tokens.d;
+                k_at = v_at = pages[i] * p.k_page + in * p.k_token;  // (one layout for both)
+                if (I8) s_at = ((long long) pages[i] * p.kv_heads + kv_head) * p.page_tokens.d + in;
+            } else {
+                k_at = j * p.k_token;
+                v_at = j * p.v_token;
+            }
+            if (!there) gone |= 1u << i;
+            kreg[i] = vreg[i] = uint4{0, 0, 0, 0};
+            kscale[i] = vscale[i] = 0.0f;
+            if (there && part_live) {
+                if (I8) {
+                    kreg[i] = *(const uint4 *) (kb + k_at + 16 * part);
+                    vreg[i] = *(const uint4 *) (vb + v_at + 16 * part);
+                    kscale[i] = p.k_scales[s_at];
+                    vscale[i] = p.v_scales[s_at];
                 } else {
-                    k_at = b * p.k_batch + kv_head * p.k_head + j * p.k_token;
-                    v_at = b * p.v_batch + kv_head * p.v_head + j * p.v_token;
+                    kreg[i] = __builtin_bit_cast(uint4, *(const halfx8_any *) (kb + 2 * k_at + 16 * part));
+                    vreg[i] = __builtin_bit_cast(uint4, *(const halfx8_any *) (vb + 2 * v_at + 16 * part));
                 }
-                if (there) {
-                    float dot = 0.0f;
-                    if (p.k_scales) {
-                        for (int d = 0; d < p.width; d++) dot += qs[wave][d] * (float) ((const signed char *) p.k)[k_at + d];
-                        dot *= p.k_scales[scale_at];
-                    } else {
-                        for (int d = 0; d < p.width; d += 8) {
-                            const halfx8 x = *(const halfx8_any *) ((const _Float16 *) p.k + k_at + d);
-                            for (int i = 0; i < 8; i++) dot += qs[wave][d + i] * (float) x[i];
-                        }
+            }
+        }
+    };
+    // 16 whole numbers times their scale
+    auto dequantise = [&](uint4 x, float scale, halfx8 (&out)[2]) {
+        const unsigned u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) out[i / 2][4 * (i % 2) + e] = (half_t) ((float) (signed char) (u[i] >> (8 * e)) * scale);
+    };
+    auto stage = [&](int buffer, bool masked) {
+        half_t *ks = lds + buffer * STAGE, *vs = ks + BKEYS * KS;
+#pragma unroll
+        for (int i = 0; i < VECS; i++) {
+            const int r = stage_row + ROW_STEP * i;
+            if (I8) {
+                halfx8 two[2];
+                dequantise(kreg[i], kscale[i], two);
+                *(halfx8 *) &ks[r * KS + 16 * part] = two[0];
+                *(halfx8 *) &ks[r * KS + 16 * part + 8] = two[1];
+                dequantise(vreg[i], vscale[i], two);
+                *(halfx8 *) &vs[r * VS + 16 * part] = two[0];
+                *(halfx8 *) &vs[r * VS + 16 * part + 8] = two[1];
+            } else {
+                *(uint4 *) &ks[r * KS + 8 * part] = kreg[i];
+                *(uint4 *) &vs[r * VS + 8 * part] = vreg[i];
+            }
+        }
+        // which of the block's rows are not there, and which hold values that a product with a zero weight does not remove
+        if (PAGED || masked) {
+            unsigned long long gone_rows = 0, bad_rows = 0;
+#pragma unroll
+            for (int i = 0; i < VECS; i++) {
+                unsigned long long bad = 0;
+                if (masked && !I8) bad = __ballot(not_finite(__builtin_bit_cast(halfx8, vreg[i])));
+                const unsigned long long missing = PAGED ? __ballot((gone >> i) & 1) : 0;
+                if (bad | missing)
+#pragma unroll
+                    for (int g = 0; g < 64 / C; g++) {  // rows of this wave's i-th load
+                        const int r = wave * (64 / C) + g + ROW_STEP * i;
+                        const unsigned long long lanes = (C == 64 ? ~0ull : (1ull << C) - 1) << (g * C);
+                        if (bad & lanes) bad_rows |= 1ull << r;
+                        if (missing & lanes) gone_rows |= 1ull << r;
                     }
-                    s = dot * p.scale;
-                    if (p.cap > 0.0f) s = p.cap * tanhf(s / p.cap);
-                    s -= slope * fabsf((float) (at - (base + j)));
-                } else {
-                    v_at = -1;
+            }
+            if (lane == 0) {
+                gone_s[buffer][wave] = gone_rows;
+                bad_s[buffer][wave] = bad_rows;
+            }
+        }
+    };
+
+    if (first_block < end_block) {
+        look_up(first_block);
+        fetch(first_block);
+        look_up(min(first_block + 1, end_block - 1));
+    }
+
+    // ---- Q: the wave's 32 rows, whole lines at a time, through the wave's part of LDS; lane (query c, half h) holds elements
+    // 16 t + 8 h .. + 7 for step t
+    halfx8 qf[WP / 16];
+    {
+        half_t *qs = lds + wave * WAVE_ROWS;
+#pragma unroll
+        for (int i = 0; i < 32 * QC / 64; i++) {
+            const int e = lane + 64 * i, r = e / QC, d = 8 * (e % QC);
+            const Row o = row_of<STRETCH>(p, min(first_row + r, rows - 1), b, kv_head);
+            halfx8 x = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (first_row + r < rows && d < p.width)
+                x = *(const halfx8_any *) ((const half_t *) p.q + (o.b * p.q_batch + o.t * p.q_token + o.head * p.q_head + d));
+            *(halfx8 *) &qs[r * OS + d] = x;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < WP / 16; t++) qf[t] = *(const halfx8 *) &qs[c * OS + 16 * t + 8 * h];
+        __syncthreads();  // (the buffers of K and V lie over these rows)
+    }
+
+    floatx16 oacc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; t++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) oacc[t][v] = 0.0f;
+    float ref = -INFINITY, sum = 0.0f;  // sum: this half's share of the keys
+    const float scale2 = p.scale * LOG2E, slope2 = SHAPED && p.slopes ? p.slopes[w.head] * LOG2E : 0.0f;
+    const bool capped = SHAPED && p.cap > 0.0f;
+    const float to_cap = capped ? p.scale / p.cap : 0.0f, cap2 = p.cap * LOG2E;
+    const int v_corner = BKEYS * KS + (4 * h + (lane & 15) / 4) * VS + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+
+    for (int block = first_block; block < end_block; block++) {
+        const int buffer = block & 1, key0 = block * BKEYS;
+        bool masked = key0 < whole_from || key0 + BKEYS > whole_end;
+        stage(buffer, masked);
+        if (block + 1 < end_block) {
+            fetch(block + 1);
+            look_up(min(block + 2, end_block - 1));
+        }
+        __syncthreads();
+        unsigned long long gone_rows = 0, bad_rows = 0;
+        if (PAGED || masked)
+#pragma unroll
+            for (int i = 0; i < WAVES; i++) {
+                gone_rows |= gone_s[buffer][i];
+                bad_rows |= bad_s[buffer][i];
+            }
+        gone_rows = ((unsigned long long) __builtin_amdgcn_readfirstlane((unsigned) (gone_rows >> 32)) << 32) | (unsigned) __builtin_amdgcn_readfirstlane((unsigned) gone_rows);
+        bad_rows = ((unsigned long long) __builtin_amdgcn_readfirstlane((unsigned) (bad_rows >> 32)) << 32) | (unsigned) __builtin_amdgcn_readfirstlane((unsigned) bad_rows);
+        masked |= gone_rows != 0;
+
+        const half_t *ks = lds + buffer * STAGE;
+        floatx16 st[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) st[u][v] = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int t = 0; t < WP / 16; t++) {
+                const halfx8 a = *(const halfx8 *) &ks[(32 * u + c) * KS + 16 * t + 8 * h];
+                st[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qf[t], st[u], 0, 0, 0);
+            }
+        // register v of tile u: key 32 u + 8 (v / 4) + 4 h + v % 4
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            if (SHAPED) {
+                const float away = (float) (w.at - (key0 + 32 * u + 4 * h));
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const float x = capped ? cap2 * tanh_fast(st[u][v] * to_cap) : st[u][v] * scale2;
+                    st[u][v] = __builtin_fmaf(-slope2, fabsf(away - (float) (8 * (v / 4) + v % 4)), x);
+                }
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; v++) st[u][v] *= scale2;
+            }
+            if (masked) {
+                const unsigned missing = (unsigned) (gone_rows >> (32 * u)) >> (4 * h);
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const int e = 8 * (v / 4) + v % 4, j = key0 + 32 * u + 4 * h + e;
+                    if ((unsigned) (j - w.lo) >= (unsigned) (w.hi - w.lo) || ((missing >> e) & 1)) st[u][v] = -INFINITY;
                 }
             }
-            float block_top = s;
-            for (int m = 32; m; m >>= 1) block_top = fmaxf(block_top, __shfl_xor(block_top, m));
-            const float new_top = fmaxf(top, block_top), ref = new_top == -INFINITY ? 0.0f : new_top;
-            const float alpha = exp2f((top - ref) * LOG2E);
-            float e = exp2f((s - ref) * LOG2E);
-            top = new_top;
-            float block_sum = e;
-            for (int m = 32; m; m >>= 1) block_sum += __shfl_xor(block_sum, m);
-            sum = sum * alpha + block_sum;
-            if (v_at >= 0 && p.v_scales) {
-                const unsigned n = p.page_tokens.div((unsigned) j), in = (unsigned) j - n * p.page_tokens.d;
-                const int page = part ? p.tables[b * p.table_stride + n] : p.prefix_table[n];
-                e *= p.v_scales[((long long) page * p.kv_heads + kv_head) * p.page_tokens.d + in];
+#pragma unroll
+            for (int v = 0; v < 16; v++) top = fmaxf(top, st[u][v]);
+        }
+        if (__any(top > ref + SLACK)) {
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float new_ref = fmaxf(ref, top);
+            const float alpha = __builtin_amdgcn_exp2f(ref - (new_ref == -INFINITY ? 0.0f : new_ref));
+            ref = new_ref;
+            sum *= alpha;
+#pragma unroll
+            for (int t = 0; t < DT; t++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) oacc[t][v] *= alpha;
+        }
+        const float minus = ref == -INFINITY ? 0.0f : ref;
+        halfx8 pv[4];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                const float e = __builtin_amdgcn_exp2f(st[u][v] - minus);
+                sum += e;
+                pv[2 * u + v / 8][v % 8] = (half_t) e;
             }
-            ps[wave][lane] = e;
-            vo[wave][lane] = v_at;
-            __builtin_amdgcn_wave_barrier();
-            for (int i = 0; i < 2; i++) {
-                const int d = lane + 64 * i;
-                acc[i] *= alpha;
-                if (d >= p.width) continue;
-                for (int u = 0; u < min(64, end - j0); u++)
-                    if (vo[wave][u] >= 0)
-                        acc[i] += ps[wave][u] * (p.v_scales ? (float) ((const signed char *) p.v)[vo[wave][u] + d] : (float) ((const _Float16 *) p.v)[vo[wave][u] + d]);
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            halfx8 a[DT];
+#pragma unroll
+            for (int t = 0; t < DT; t++) {
+                const halfx4 lo = lds_read_transposed(ks + v_corner + (16 * s) * VS + 32 * t);
+                const halfx4 hi = lds_read_transposed(ks + v_corner + (16 * s + 8) * VS + 32 * t);
+                a[t] = halfx8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             }
-            __builtin_amdgcn_wave_barrier();
+            if (bad_rows != 0)
+#pragma unroll
+                for (int t = 0; t < DT; t++) a[t] = finite_or_zero(a[t]);
+#pragma unroll
+            for (int t = 0; t < DT; t++) oacc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[t], pv[s], oacc[t], 0, 0, 0);
+        }
+        // Infinities or NaN among the values of a block that not every row sees whole: a weight of zero does not remove them
+        // from a product, so they are left out above and added here for the queries that see their key.
+        for (unsigned long long left = bad_rows; left; left &= left - 1) {
+            const int key = __builtin_ctzll(left);
+            if ((unsigned) (key0 + key - w.lo) < (unsigned) (w.hi - w.lo))
+#pragma unroll
+                for (int t = 0; t < DT; t++)
+#pragma unroll
+                    for (int a = 0; a < 4; a++) {
+                        const halfx4 x = *(const halfx4 *) &ks[BKEYS * KS + key * VS + 32 * t + 8 * a + 4 * h];
+#pragma unroll
+                        for (int u = 0; u < 4; u++) oacc[t][4 * a + u] += (float) x[u] - (float) x[u] == 0.0f ? 0.0f : (float) x[u];
+                    }
         }
     }
-    if (!live_row) return;
-    _Float16 *o = (_Float16 *) p.out + b * p.o_batch + t * p.o_token + head * p.o_head;
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-    for (int i = 0; i < 2; i++)
-        if (lane + 64 * i < p.width) o[lane + 64 * i] = (_Float16) (acc[i] * inv);
+
+    sum += __shfl_xor(sum, 32);
+    if (p.part_values) {
+        // a part of the softmax: reference, sum and the sums of values as they are
+        if (row < rows) {
+            const long long at = ((long long) pair * splits + split) * rows + row;
+            float *o = p.part_values + at * WP;
+#pragma unroll
+            for (int t = 0; t < DT; t++)
+#pragma unroll
+                for (int a = 0; a < 4; a++)
+                    *(floatx4 *) (o + 32 * t + 8 * a + 4 * h) = floatx4{oacc[t][4 * a], oacc[t][4 * a + 1], oacc[t][4 * a + 2], oacc[t][4 * a + 3]};
+            if (h == 0) *(float2 *) (p.part_stats + 2 * at) = float2{ref, sum};
+        }
+        return;
+    }
+    // ---- the result: normalised, rounded, through the wave's rows of LDS into whole rows
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    __syncthreads();  // (every wave is done with the buffers)
+    half_t *os = lds + wave * WAVE_ROWS;
+#pragma unroll
+    for (int t = 0; t < DT; t++)
+#pragma unroll
+        for (int a = 0; a < 4; a++) {
+            halfx4 x;
+#pragma unroll
+            for (int u = 0; u < 4; u++) x[u] = (half_t) (oacc[t][4 * a + u] * inv);
+            *(halfx4 *) &os[c * OS + 32 * t + 8 * a + 4 * h] = x;
+        }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 32 * QC / 64; i++) {
+        const int e = lane + 64 * i, r = e / QC, d = 8 * (e % QC);
+        if (first_row + r >= rows || d >= p.width) continue;
+        const Row o = row_of<STRETCH>(p, first_row + r, b, kv_head);
+        *(halfx8_any *) ((half_t *) p.out + (o.b * p.o_batch + o.t * p.o_token + o.head * p.o_head + d)) = *(const halfx8 *) &os[r * OS + d];
+    }
+}
+
+// ---- up to 16 NT rows per workgroup --------------------------------------------------------------------------------
+
+// Decoding: bound by the bytes of the cache, which pass through once. A workgroup takes a stretch of keys of one sequence
+// and head, its four waves every fourth step of 32 keys; nothing is staged in LDS, so that many waves fit a compute unit and
+// keep the memory busy between them. Both products take 16 keys or dims by 16 rows (v_mfma_f32_16x16x32_f16):
+//   S^T = K Q^T      lane (key i = lane % 16, g = lane / 16) reads 16 byte pieces of key i, 64 bytes of a row per load of four
+//                    lanes; the order of a row's elements in the product is free, Q is loaded in the same one
+//   O^T += V^T P^T   the accumulators of two tiles of S^T are the operand, keys 4 g + e and 16 + 4 g + e; lane (i, g) reads
+//                    elements i DPL .. + DPL - 1 of those 8 keys and turns them in registers: product dt has dim i DPL + dt
+// Whole numbers become f16 without a conversion instruction: q + 128 in the low byte of 0x6400 is 1152 + q, the
+// subtraction is exact. The scale of a key is applied to its score, that of a value to its weight, in f32; the reference
+// of the softmax follows score + log2(value scale), which keeps the scaled weights inside the range of f16.
+
+// Which keys a workgroup takes, decided on the device, where the lengths are: stretches (the prefix when it is done here, then
+// every sequence's own keys) are cut into items of about the same size, ROW_ITEMS of them over all heads, and workgroup x
+// takes item x / kv_heads. The grid covers the largest number of items that any lengths can give.
+constexpr int ROW_ITEMS = 1024, ROW_MIN_KEYS = 128, ROW_THREADS = 64 * WAVES;
+
+__device__ __forceinline__ int2 stretch_range(const ServingAttentionParams &p, int seg) {  // the keys that any of its rows may see
+    if (seg < 0) return int2{0, p.prefix_tokens};
+    const int n = own_length(p, seg);
+    return int2{p.window ? max(0, n - p.queries + 1 - p.window) & ~31 : 0, n};
+}
+
+struct Item {
+    int seg, from, end, items;
+};
+
+// segments -1 (the prefix, when `with_prefix`) and 0 .. batch - 1; false when there is no such item
+__device__ __forceinline__ bool find_item(const ServingAttentionParams &p, bool with_prefix, int item, Item &out) {
+    __shared__ long long wave_steps[WAVES];
+    __shared__ int wave_sums[WAVES];
+    __shared__ Item found;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int first = with_prefix ? -1 : 0;
+    long long steps = 0;  // of 32 keys, of all stretches (64 bits: many long tables may share pages)
+    for (int seg = first + (int) threadIdx.x; seg < p.batch; seg += ROW_THREADS) {
+        const int2 r = stretch_range(p, seg);
+        steps += (r.y - r.x + 31) / 32;
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) steps += __shfl_xor(steps, m);
+    if (lane == 0) wave_steps[wave] = steps;
+    if (threadIdx.x == 0) found.seg = -2;
+    __syncthreads();
+    steps = wave_steps[0] + wave_steps[1] + wave_steps[2] + wave_steps[3];
+    // steps per item; no stretch has more than 2^26
+    const int each = max(ROW_MIN_KEYS / 32, (int) min((steps * p.kv_heads + ROW_ITEMS - 1) / ROW_ITEMS, 1ll << 26));
+    int base = 0;
+    for (int seg0 = first; seg0 < p.batch; seg0 += ROW_THREADS) {
+        const int seg = seg0 + (int) threadIdx.x;
+        int n = 0;
+        int2 r = {0, 0};
+        if (seg < p.batch) {
+            r = stretch_range(p, seg);
+            n = max(1, ((r.y - r.x + 31) / 32 + each - 1) / each);
+        }
+        int sums = n;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int other = __shfl_up(sums, m);
+            if (lane >= m) sums += other;
+        }
+        __syncthreads();
+        if (lane == 63) wave_sums[wave] = sums;
+        __syncthreads();
+        int before = base + sums - n;
+        for (int w = 0; w < wave; w++) before += wave_sums[w];
+        if (n > 0 && item >= before && item < before + n) {
+            // the items of a stretch have the same number of steps, but for the last
+            const int per = 32 * (((r.y - r.x + 31) / 32 + n - 1) / n), from = r.x + (item - before) * per;
+            found = Item{seg, min(from, r.y), min(from + per, r.y), n};
+            if (item == before) ((int2 *) p.part_items)[seg + 1] = int2{before, n};
+        }
+        base += wave_sums[0] + wave_sums[1] + wave_sums[2] + wave_sums[3];
+    }
+    __syncthreads();
+    out = Item{__builtin_amdgcn_readfirstlane(found.seg), __builtin_amdgcn_readfirstlane(found.from), __builtin_amdgcn_readfirstlane(found.end),
+               __builtin_amdgcn_readfirstlane(found.items)};
+    return out.seg != -2;
+}
+
+__device__ __forceinline__ unsigned pk_sub_1152(unsigned x) {
+    const halfx2 bias = {(half_t) -1152.0f, (half_t) -1152.0f};
+    return __builtin_bit_cast(unsigned, __builtin_bit_cast(halfx2, x) + bias);
+}
+
+// 8 whole numbers of 8 bits as f16, in the order 0 2 1 3 4 6 5 7
+__device__ __forceinline__ halfx8 widen(unsigned a, unsigned b) {
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    return __builtin_bit_cast(halfx8, uint4{pk_sub_1152((a & 0x00ff00ffu) | 0x64006400u), pk_sub_1152(((a >> 8) & 0x00ff00ffu) | 0x64006400u),
+                                            pk_sub_1152((b & 0x00ff00ffu) | 0x64006400u), pk_sub_1152(((b >> 8) & 0x00ff00ffu) | 0x64006400u)});
+}
+
+// PAGE16: pages are multiples of 16 tokens, so that a tile of 16 keys lies in one page, whose number the whole wave shares
+template <int WP, int NT, bool I8, bool SHAPED, bool PAGE16>
+__global__ __launch_bounds__(ROW_THREADS) void row_attention_kernel(ServingAttentionParams p, int with_prefix) {
+    constexpr int ELEM = I8 ? 1 : 2;
+    constexpr int KP = WP * ELEM / 64;    // 16 byte pieces of a key per lane
+    constexpr int DPL = WP / 16;          // dims of a value per lane
+    constexpr int VW = DPL * ELEM / 4;    // 32 bit words of a value per lane
+    constexpr int STEPS = WP / 32;
+    constexpr int OS = WP + 4;
+    __shared__ __attribute__((aligned(16))) float os[WAVES][16 * NT][OS];
+    __shared__ float refs[WAVES][16 * NT], sums[WAVES][16 * NT];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, g = lane >> 4;
+    const int kv_head = (int) (blockIdx.x % (unsigned) p.kv_heads);
+    Item item;
+    if (!find_item(p, with_prefix, (int) (blockIdx.x / (unsigned) p.kv_heads), item)) return;
+    const bool is_prefix = item.seg < 0;
+    const int b = is_prefix ? 0 : item.seg;
+    const int count = is_prefix ? p.prefix_tokens : own_length(p, b);
+    const int rows = (is_prefix ? p.batch : 1) * p.queries * (int) p.group_div.d;
+    const int *table = is_prefix ? p.prefix_table : p.tables + b * p.table_stride;
+
+    // ---- the rows: lane i of a tile of 16 owns row 16 n + i
+    halfx8 qf[NT][STEPS];
+    int at[NT], lo[NT], hi[NT];
+    float slope2[NT];
+    int whole_from = 0, whole_end = INT_MAX, any_from = INT_MAX, any_end = 0;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int r = 16 * n + i;
+        const Row w = is_prefix ? row_of<PREFIX>(p, min(r, rows - 1), 0, kv_head) : row_of<OWN>(p, min(r, rows - 1), b, kv_head);
+        at[n] = w.at;
+        lo[n] = w.lo;
+        hi[n] = w.hi;
+        slope2[n] = SHAPED && p.slopes ? p.slopes[w.head] * LOG2E : 0.0f;
+        whole_from = max(whole_from, w.lo);
+        whole_end = min(whole_end, w.hi);
+        if (w.hi > w.lo) {
+            any_from = min(any_from, w.lo);
+            any_end = max(any_end, w.hi);
+        }
+        const half_t *q = (const half_t *) p.q + (w.b * p.q_batch + w.t * p.q_token + w.head * p.q_head);
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            const int d = I8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
+            halfx8 x = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (r < rows && d < p.width) x = *(const halfx8_any *) (q + d);
+            qf[n][s] = I8 ? halfx8{x[0], x[2], x[1], x[3], x[4], x[6], x[5], x[7]} : x;
+        }
+    }
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) {
+        whole_from = max(whole_from, __shfl_xor(whole_from, m));
+        whole_end = min(whole_end, __shfl_xor(whole_end, m));
+        any_from = min(any_from, __shfl_xor(any_from, m));
+        any_end = max(any_end, __shfl_xor(any_end, m));
+    }
+    whole_from = __builtin_amdgcn_readfirstlane(whole_from);
+    whole_end = __builtin_amdgcn_readfirstlane(whole_end);
+    any_from = __builtin_amdgcn_readfirstlane(any_from);
+    any_end = __builtin_amdgcn_readfirstlane(any_end);
+    int from = max(item.from, any_from & ~31), end = min(item.end, any_end);
+    if (from >= end) from = end = 0;  // (nothing to see: any_from may be INT_MAX, nothing may be added to it)
+
+    floatx4 oacc[NT][DPL];
+    float ref[NT], sum[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        ref[n] = -INFINITY;
+        sum[n] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DPL; d++) oacc[n][d] = floatx4{0, 0, 0, 0};
+    }
+    const float scale2 = p.scale * LOG2E;
+    const bool capped = SHAPED && p.cap > 0.0f;
+    const float to_cap = capped ? p.scale / p.cap : 0.0f, cap2 = p.cap * LOG2E;
+    const char *kb = (const char *) p.k + kv_head * p.k_head * ELEM, *vb = (const char *) p.v + kv_head * p.v_head * ELEM;
+    const bool v_live = i * DPL < p.width;
+
+    uint4 kreg[2][KP];
+    unsigned vreg[8][VW];
+    float kscale[8], vscale[8];
+    unsigned gone = 0;  // keys of the lane's 8 (4 u + e: key 16 u + 4 g + e) that are not there
+
+    // K, and the scales, of the step at key0
+    auto page_of = [&](int j) { return j < count ? table[p.page_tokens.div((unsigned) j)] : -1; };
+    auto k_piece = [&](int u, long long row_at, bool there) {
+#pragma unroll
+        for (int c = 0; c < KP; c++) {
+            const int byte = 64 * c + 16 * g;
+            kreg[u][c] = there && byte < p.width * ELEM ? *(const uint4 *) (kb + row_at * ELEM + byte) : uint4{0, 0, 0, 0};
+        }
+    };
+    auto v_piece = [&](int e, long long row_at, bool there) {
+        const char *at_v = vb + row_at * ELEM + i * DPL * ELEM;
+#pragma unroll
+        for (int x = 0; x < VW; x++) vreg[e][x] = 0;
+        if (there && v_live) {
+            if (VW == 1) vreg[e][0] = *(const unsigned *) at_v;
+            if (VW == 2) {
+                const uint2 x = *(const uint2 *) at_v;
+                vreg[e][0] = x.x;
+                vreg[e][VW > 1 ? 1 : 0] = x.y;
+            }
+            if (VW == 4) {
+                const uint4 x = *(const uint4 *) at_v;
+                vreg[e][0] = x.x;
+                vreg[e][VW > 1 ? 1 : 0] = x.y;
+                vreg[e][VW > 2 ? 2 : 0] = x.z;
+                vreg[e][VW > 2 ? 3 : 0] = x.w;
+            }
+        }
+    };
+    int pages[2];
+    auto look_up = [&](int key0) {
+        if (PAGE16)
+#pragma unroll
+            for (int u = 0; u < 2; u++) pages[u] = page_of(min(key0, end - 1) / 32 * 32 + 16 * u);
+    };
+    auto fetch = [&](int key0) {
+        gone = 0;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int tile0 = key0 + 16 * u;
+            if (PAGE16) {
+                const int page = __builtin_amdgcn_readfirstlane(pages[u]);
+                const bool there = (unsigned) page < (unsigned) p.pages;
+                const unsigned in = (unsigned) tile0 - p.page_tokens.div((unsigned) tile0) * p.page_tokens.d;
+                const long long k0 = page * p.k_page + in * p.k_token, v0 = page * p.v_page + in * p.v_token;
+                const long long s0 = ((long long) page * p.kv_heads + kv_head) * p.page_tokens.d + in + 4 * g;
+                k_piece(u, k0 + i * p.k_token, there);
+                if (!there) gone |= 15u << (4 * u);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    v_piece(4 * u + e, v0 + (4 * g + e) * p.v_token, there && tile0 + 4 * g + e < count);
+                    kscale[4 * u + e] = I8 && there ? p.k_scales[s0 + e] : 1.0f;
+                    vscale[4 * u + e] = I8 && there ? p.v_scales[s0 + e] : 1.0f;
+                }
+            } else {
+                const int j = tile0 + i, page = page_of(j);
+                const unsigned in = (unsigned) j - p.page_tokens.div((unsigned) j) * p.page_tokens.d;
+                k_piece(u, page * p.k_page + in * p.k_token, (unsigned) page < (unsigned) p.pages);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int jv = tile0 + 4 * g + e, page_v = page_of(jv);
+                    const bool there = (unsigned) page_v < (unsigned) p.pages;
+                    const unsigned in_v = (unsigned) jv - p.page_tokens.div((unsigned) jv) * p.page_tokens.d;
+                    const long long s = ((long long) page_v * p.kv_heads + kv_head) * p.page_tokens.d + in_v;
+                    v_piece(4 * u + e, page_v * p.v_page + in_v * p.v_token, there);
+                    if (!there) gone |= 1u << (4 * u + e);
+                    kscale[4 * u + e] = I8 && there ? p.k_scales[s] : 1.0f;
+                    vscale[4 * u + e] = I8 && there ? p.v_scales[s] : 1.0f;
+                }
+            }
+        }
+    };
+
+    int key0 = from + 32 * wave;
+    constexpr int STRIDE = 32 * WAVES;
+    if (key0 < end) look_up(key0);
+    while (key0 < end) {
+        fetch(key0);
+        look_up(key0 + STRIDE);
+        const bool masked = key0 < whole_from || key0 + 32 > min(whole_end, end) || __any(gone != 0);
+        floatx4 st[NT][2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            halfx8 a[STEPS];
+#pragma unroll
+            for (int s = 0; s < STEPS; s++) {
+                if (I8) {
+                    const uint4 x = kreg[u][s / 2];
+                    a[s] = s % 2 ? widen(x.z, x.w) : widen(x.x, x.y);
+                } else {
+                    a[s] = __builtin_bit_cast(halfx8, kreg[u][I8 ? 0 : s]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                st[n][u] = floatx4{0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < STEPS; s++) st[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[s], qf[n][s], st[n][u], 0, 0, 0);
+            }
+        }
+        float value_log[8];
+        if (I8)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                vscale[e] = fmaxf(vscale[e], 0x1p-40f);  // (values below 2^-33 are zeros of an f16 result)
+                value_log[e] = __builtin_amdgcn_logf(vscale[e]);
+            }
+        halfx8 weights[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            float top = -INFINITY, s2[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int key = key0 + 16 * (e / 4) + 4 * g + e % 4;
+                float x = st[n][e / 4][e % 4];
+                if (I8) x *= kscale[e];
+                if (SHAPED) {
+                    x = capped ? cap2 * tanh_fast(x * to_cap) : x * scale2;
+                    x = __builtin_fmaf(-slope2[n], fabsf((float) (at[n] - key)), x);
+                } else {
+                    x *= scale2;
+                }
+                if (masked && ((unsigned) (key - lo[n]) >= (unsigned) (hi[n] - lo[n]) || key >= end || ((gone >> e) & 1))) x = -INFINITY;
+                s2[e] = x;
+                top = fmaxf(top, I8 ? x + value_log[e] : x);
+            }
+            if (__any(top > ref[n] + SLACK)) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float new_ref = fmaxf(ref[n], top);
+                const float alpha = __builtin_amdgcn_exp2f(ref[n] - (new_ref == -INFINITY ? 0.0f : new_ref));
+                ref[n] = new_ref;
+                sum[n] *= alpha;
+#pragma unroll
+                for (int d = 0; d < DPL; d++) oacc[n][d] *= alpha;
+            }
+            const float minus = ref[n] == -INFINITY ? 0.0f : ref[n];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float x = __builtin_amdgcn_exp2f(s2[e] - minus);
+                sum[n] += x;
+                weights[n][e] = (half_t) (I8 ? x * vscale[e] : x);
+            }
+        }
+        unsigned bad = 0;  // keys of the lane's 8 whose values hold an infinity or NaN, where not every row sees every key
+        if (!I8 && masked) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                bool any = false;
+#pragma unroll
+                for (int x = 0; x < VW; x++) any |= (vreg[e][x] & 0x7c00u) == 0x7c00u || (vreg[e][x] & 0x7c000000u) == 0x7c000000u;
+                // (of the 16 lanes of a group)
+                if ((__ballot(any) >> (16 * g)) & 0xffffu) bad |= 1u << e;
+            }
+        }
+        const bool any_bad = !I8 && __any(bad != 0);
+#pragma unroll
+        for (int d = 0; d < DPL; d++) {
+            unsigned pair[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (I8) {
+                    const unsigned sel = (unsigned) (d % 4) | 0x0c00u | (unsigned) (4 + d % 4) << 16 | 0x0c000000u;
+                    pair[k] = pk_sub_1152(__builtin_amdgcn_perm(vreg[2 * k + 1][d / 4] ^ 0x80808080u, vreg[2 * k][d / 4] ^ 0x80808080u, sel) | 0x64006400u);
+                } else {
+                    pair[k] = __builtin_amdgcn_perm(vreg[2 * k + 1][I8 ? 0 : d / 2], vreg[2 * k][I8 ? 0 : d / 2], d % 2 ? 0x07060302u : 0x05040100u);
+                }
+            }
+            const halfx8 a = __builtin_bit_cast(halfx8, uint4{pair[0], pair[1], pair[2], pair[3]});
+            if (!any_bad) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) oacc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, weights[n], oacc[n][d], 0, 0, 0);
+            } else {
+                // (as in the kernel above: a key of its own product, for the queries that see it)
+                halfx8 good = a;
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if ((bad >> e) & 1) good[e] = (half_t) 0.0f;
+#pragma unroll
+                for (int n = 0; n < NT; n++) oacc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(good, weights[n], oacc[n][d], 0, 0, 0);
+#pragma unroll 1
+                for (int key = 0; key < 32; key++) {
+                    const int of_group = (key % 16) / 4, e_of = 4 * (key / 16) + key % 4;
+                    if (__any(g == of_group && ((bad >> e_of) & 1)) == 0) continue;
+                    halfx8 one;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) one[e] = g == of_group && e == e_of ? a[e] : (half_t) 0.0f;
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const floatx4 its = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, weights[n], floatx4{0, 0, 0, 0}, 0, 0, 0);
+                        const bool seen = (unsigned) (key0 + key - lo[n]) < (unsigned) (hi[n] - lo[n]);
+#pragma unroll
+                        for (int v = 0; v < 4; v++) oacc[n][d][v] += seen ? its[v] : 0.0f;
+                    }
+                }
+            }
+        }
+        key0 += STRIDE;
+    }
+
+    // ---- the four waves' parts into one
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        sum[n] += __shfl_xor(sum[n], 16);
+        sum[n] += __shfl_xor(sum[n], 32);
+        if (g == 0) {
+            refs[wave][16 * n + i] = ref[n];
+            sums[wave][16 * n + i] = sum[n];
+        }
+        // register v of product d: dim (4 g + v) DPL + d of row i
+#pragma unroll
+        for (int v = 0; v < 4; v++)
+#pragma unroll
+            for (int d = 0; d < DPL; d += 4)
+                *(floatx4 *) &os[wave][16 * n + i][(4 * g + v) * DPL + d] = floatx4{oacc[n][d][v], oacc[n][d + 1][v], oacc[n][d + 2][v], oacc[n][d + 3][v]};
+    }
+    __syncthreads();
+    const bool direct = !is_prefix && p.prefix_tokens == 0 && item.items == 1;
+    for (int e = threadIdx.x; e < rows * (WP / 4); e += ROW_THREADS) {
+        const int r = e / (WP / 4), d = 4 * (e % (WP / 4));
+        float top = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) top = fmaxf(top, refs[w][r]);
+        floatx4 x = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const float weight = __builtin_amdgcn_exp2f(refs[w][r] - (top == -INFINITY ? 0.0f : top));
+            total += weight * sums[w][r];
+            x += weight * *(const floatx4 *) &os[w][r][d];
+        }
+        if (direct) {
+            const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+            const Row w = row_of<OWN>(p, r, b, kv_head);
+            if (d < p.width)
+                *(halfx4_any *) ((half_t *) p.out + (w.b * p.o_batch + w.t * p.o_token + w.head * p.o_head + d)) =
+                    halfx4{(half_t) (x[0] * inv), (half_t) (x[1] * inv), (half_t) (x[2] * inv), (half_t) (x[3] * inv)};
+        } else {
+            const long long part = is_prefix ? p.row_prefix_part : p.row_own_part;
+            const long long at_part = part + ((long long) ((int) (blockIdx.x / (unsigned) p.kv_heads)) * p.kv_heads + kv_head) * rows + r;
+            *(floatx4 *) (p.part_values + at_part * WP + d) = x;
+            if (d == 0) *(float2 *) (p.part_stats + 2 * at_part) = float2{top, total};
+        }
+    }
+}
+
+// ---- parts -> results ----------------------------------------------------------------------------------------------
+
+// A wave per row of the result. WP / 64 elements per lane.
+template <int WP>
+__global__ __launch_bounds__(64 * WAVES) void join_attention_kernel(ServingAttentionParams p) {
+    constexpr int N = WP / 64;
+    const int lane = threadIdx.x & 63;
+    const unsigned row = __builtin_amdgcn_readfirstlane(blockIdx.x * WAVES + (threadIdx.x >> 6));
+    if (row >= (unsigned) p.batch * p.queries * p.heads) return;
+    const unsigned token = row / (unsigned) p.heads, head = row - token * p.heads;
+    const unsigned b = p.queries_div.div(token), t = token - b * p.queries_div.d;
+    const unsigned kv_head = p.group_div.div(head), in_group = head - kv_head * p.group_div.d;
+    const long long own_rows = (long long) p.queries * p.group_div.d, prefix_rows = p.batch * own_rows;
+    const long long own_row = t * p.group_div.d + in_group, prefix_row = b * own_rows + own_row;
+    // where the parts of either stretch start, how far apart they are and how many there are
+    long long at[2] = {0, 0}, apart[2] = {0, 0};
+    int count[2] = {0, 0};
+    if (p.prefix_splits > 0) {
+        at[0] = kv_head * p.prefix_splits * prefix_rows + prefix_row;
+        apart[0] = prefix_rows;
+        count[0] = p.prefix_splits;
+    } else if (p.prefix_tokens > 0) {
+        const int2 items = ((const int2 *) p.part_items)[0];
+        at[0] = p.row_prefix_part + (long long) (items.x * p.kv_heads + kv_head) * prefix_rows + prefix_row;
+        apart[0] = p.kv_heads * prefix_rows;
+        count[0] = items.y;
+    }
+    if (p.own_splits > 0) {
+        at[1] = p.row_own_part + (long long) (b * p.kv_heads + kv_head) * p.own_splits * own_rows + own_row;
+        apart[1] = own_rows;
+        count[1] = p.own_splits;
+    } else {
+        const int2 items = ((const int2 *) p.part_items)[b + 1];
+        if (p.prefix_tokens == 0 && items.y == 1) return;  // (written where it was computed)
+        at[1] = p.row_own_part + (long long) (items.x * p.kv_heads + kv_head) * own_rows + own_row;
+        apart[1] = p.kv_heads * own_rows;
+        count[1] = items.y;
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+        for (int i = lane; i < count[s]; i += 64) top = fmaxf(top, p.part_stats[2 * (at[s] + i * apart[s])]);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+    if (top == -INFINITY) top = 0.0f;
+    float total = 0.0f, x[N] = {};
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+        for (int i0 = 0; i0 < count[s]; i0 += 64) {
+            float weight = 0.0f;
+            if (i0 + lane < count[s]) {
+                const float2 st = *(const float2 *) (p.part_stats + 2 * (at[s] + (i0 + lane) * apart[s]));
+                weight = __builtin_amdgcn_exp2f(st.x - top);
+                total += weight * st.y;
+            }
+            const float *from = p.part_values + (at[s] + i0 * apart[s]) * WP + N * lane;
+            const int n = min(64, count[s] - i0);
+#pragma unroll 4
+            for (int i = 0; i < n; i++) {
+                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), i));
+#pragma unroll
+                for (int k = 0; k < N; k++) x[k] += w * from[i * apart[s] * WP + k];
+            }
+        }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) total += __shfl_xor(total, m);
+    const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+    half_t *o = (half_t *) p.out + (b * p.o_batch + t * p.o_token + head * p.o_head);
+#pragma unroll
+    for (int k = 0; k < N; k++)
+        if (N * lane + k < p.width) o[N * lane + k] = (half_t) (x[k] * inv);
+}
+
+// ---- plans ---------------------------------------------------------------------------------------------------------
+
+struct Plan {
+    int own_rows;             // per sequence and head of keys
+    long long prefix_rows;
+    bool own_in_rows, prefix_in_rows;  // which kernel
+    long long own_tiles, prefix_tiles;
+    int own_splits, prefix_splits;     // of the tile kernel
+    long long items;                   // of the row kernel, at most
+    bool join;
+    long long prefix_parts, own_parts;  // rows of partial results
+    int wp;
+};
+
+// Keys are shared by several workgroups while tiles alone leave compute units idle (two workgroups fit each), down to
+// parts of four blocks: below, a part costs more to write and to join than it saves.
+int splits_for(long long workgroups, long long keys) {
+    constexpr long long WANTED = 512;
+    if (workgroups >= WANTED || workgroups == 0) return 1;
+    return (int) std::max(1ll, std::min((WANTED + workgroups - 1) / workgroups, keys / 256));
+}
+
+Plan plan_for(const ServingAttentionParams &p) {
+    Plan l = {};
+    l.wp = p.width <= 64 ? 64 : 128;
+    l.own_rows = p.queries * (p.heads / p.kv_heads);
+    l.prefix_rows = (long long) p.batch * l.own_rows;
+    // a tile of 16 or 32 rows keeps the keys streaming; more rows are worth staging them for
+    l.own_in_rows = p.paged && l.own_rows <= 32;
+    l.prefix_in_rows = p.prefix_tokens > 0 && l.prefix_rows <= 32;
+    const long long pairs = (long long) p.batch * p.kv_heads;
+    if (!l.own_in_rows) {
+        l.own_tiles = (l.own_rows + 127) / 128;
+        l.own_splits = splits_for(l.own_tiles * pairs, p.paged ? p.table_tokens : p.keys);
+        l.own_parts = l.own_splits * pairs * l.own_rows;
+    }
+    if (p.prefix_tokens > 0 && !l.prefix_in_rows) {
+        l.prefix_tiles = (l.prefix_rows + 127) / 128;
+        l.prefix_splits = splits_for(l.prefix_tiles * p.kv_heads, p.prefix_tokens);
+        l.prefix_parts = (long long) l.prefix_splits * p.kv_heads * l.prefix_rows;
+    }
+    if (l.own_in_rows) {
+        // the stretches and the items beyond one of each, see find_item
+        const long long stretches = p.batch + (l.prefix_in_rows ? 1 : 0);
+        long long by_keys = p.batch * std::max(1ll, ((long long) p.table_tokens + ROW_MIN_KEYS - 1) / ROW_MIN_KEYS);
+        if (l.prefix_in_rows) by_keys += std::max(1, (p.prefix_tokens + ROW_MIN_KEYS - 1) / ROW_MIN_KEYS);
+        l.items = std::min(stretches + ROW_ITEMS / p.kv_heads, by_keys);
+        l.own_parts = l.items * p.kv_heads * l.own_rows;
+        if (l.prefix_in_rows) l.prefix_parts = l.items * p.kv_heads * l.prefix_rows;
+    }
+    l.join = p.prefix_tokens > 0 || (l.own_in_rows ? l.items > p.batch : l.own_splits > 1);
+    if (!l.join) l.own_parts = 0;
+    return l;
+}
+
+size_t round256(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+template <int WP, int STRETCH, bool I8>
+int launch_tiles(const ServingAttentionParams &p, unsigned workgroups, int splits, hipStream_t stream) {
+    if (p.cap > 0.0f || p.slopes) hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, true>), dim3(workgroups, (unsigned) splits), dim3(64 * WAVES), 0, stream, p);
+    else hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, false>), dim3(workgroups, (unsigned) splits), dim3(64 * WAVES), 0, stream, p);
+    return (int) hipGetLastError();
+}
+
+template <int WP>
+int launch_tiles_for(const ServingAttentionParams &p, int stretch, unsigned workgroups, int splits, hipStream_t stream) {
+    if (stretch == PROMPT) return launch_tiles<WP, PROMPT, false>(p, workgroups, splits, stream);
+    if (stretch == OWN) return p.k_scales ? launch_tiles<WP, OWN, true>(p, workgroups, splits, stream) : launch_tiles<WP, OWN, false>(p, workgroups, splits, stream);
+    return p.k_scales ? launch_tiles<WP, PREFIX, true>(p, workgroups, splits, stream) : launch_tiles<WP, PREFIX, false>(p, workgroups, splits, stream);
+}
+
+template <int WP, int NT, bool I8>
+int launch_rows(const ServingAttentionParams &p, unsigned workgroups, int with_prefix, hipStream_t stream) {
+    const bool shaped = p.cap > 0.0f || p.slopes, page16 = p.page_tokens.d % 16 == 0;
+    const dim3 grid(workgroups), block(ROW_THREADS);
+    if (shaped && page16) hipLaunchKernelGGL((row_attention_kernel<WP, NT, I8, true, true>), grid, block, 0, stream, p, with_prefix);
+    else if (shaped) hipLaunchKernelGGL((row_attention_kernel<WP, NT, I8, true, false>), grid, block, 0, stream, p, with_prefix);
+    else if (page16) hipLaunchKernelGGL((row_attention_kernel<WP, NT, I8, false, true>), grid, block, 0, stream, p, with_prefix);
+    else hipLaunchKernelGGL((row_attention_kernel<WP, NT, I8, false, false>), grid, block, 0, stream, p, with_prefix);
+    return (int) hipGetLastError();
+}
+
+template <int WP>
+int launch_rows_for(const ServingAttentionParams &p, unsigned workgroups, bool two_tiles, int with_prefix, hipStream_t stream) {
+    if (p.k_scales) return two_tiles ? launch_rows<WP, 2, true>(p, workgroups, with_prefix, stream) : launch_rows<WP, 1, true>(p, workgroups, with_prefix, stream);
+    return two_tiles ? launch_rows<WP, 2, false>(p, workgroups, with_prefix, stream) : launch_rows<WP, 1, false>(p, workgroups, with_prefix, stream);
 }
 
 }  // namespace
 
-size_t serving_attention_workspace(const ServingAttentionParams &) { return 0; }
+// partial values, then their references and sums, then the items of the row kernel
+size_t serving_attention_workspace(const ServingAttentionParams &p) {
+    const Plan l = plan_for(p);
+    const size_t parts = (size_t) (l.prefix_parts + l.own_parts);
+    size_t bytes = round256(parts * l.wp * 4) + round256(parts * 8);
+    if (l.own_in_rows) bytes += round256(((size_t) p.batch + 1) * 8);
+    return bytes;
+}
 
-int launch_serving_attention(const ServingAttentionParams &p, void *, ihipStream_t *stream) {
-    const long long rows = (long long) p.batch * p.queries * p.heads;
-    hipLaunchKernelGGL(masked_attention_kernel, dim3((unsigned) ((rows + WAVES - 1) / WAVES)), dim3(64 * WAVES), 0, stream, p);
-    return (int) hipGetLastError();
+int launch_serving_attention(const ServingAttentionParams &given, void *workspace, ihipStream_t *stream) {
+    ServingAttentionParams p = given;
+    const Plan l = plan_for(p);
+    const size_t parts = (size_t) (l.prefix_parts + l.own_parts);
+    p.group_div = FastDiv((uint32_t) (p.heads / p.kv_heads));
+    p.queries_div = FastDiv((uint32_t) p.queries);
+    float *values = (float *) workspace, *stats = (float *) ((char *) workspace + round256(parts * l.wp * 4));
+    p.part_items = l.own_in_rows ? (int32_t *) ((char *) stats + round256(parts * 8)) : nullptr;
+    p.row_prefix_part = 0;
+    p.row_own_part = l.prefix_parts;
+    p.prefix_splits = l.prefix_splits;
+    p.own_splits = l.own_splits;
+    const long long pairs = (long long) p.batch * p.kv_heads;
+    if (l.prefix_tiles > 0) {
+        p.part_values = values;
+        p.part_stats = stats;
+        const unsigned workgroups = (unsigned) (l.prefix_tiles * p.kv_heads);
+        const int e = l.wp == 64 ? launch_tiles_for<64>(p, PREFIX, workgroups, l.prefix_splits, stream) : launch_tiles_for<128>(p, PREFIX, workgroups, l.prefix_splits, stream);
+        if (e != 0) return e;
+    }
+    if (!l.own_in_rows) {
+        p.part_values = l.join ? values + l.prefix_parts * l.wp : nullptr;
+        p.part_stats = l.join ? stats + 2 * l.prefix_parts : nullptr;
+        const unsigned workgroups = (unsigned) (l.own_tiles * pairs);
+        const int stretch = p.paged ? OWN : PROMPT;
+        const int e = l.wp == 64 ? launch_tiles_for<64>(p, stretch, workgroups, l.own_splits, stream) : launch_tiles_for<128>(p, stretch, workgroups, l.own_splits, stream);
+        if (e != 0) return e;
+    } else {
+        p.part_values = values;
+        p.part_stats = stats;
+        const unsigned workgroups = (unsigned) (l.items * p.kv_heads);
+        const bool two_tiles = (l.prefix_in_rows ? l.prefix_rows : l.own_rows) > 16;
+        const int e = l.wp == 64 ? launch_rows_for<64>(p, workgroups, two_tiles, l.prefix_in_rows, stream) : launch_rows_for<128>(p, workgroups, two_tiles, l.prefix_in_rows, stream);
+        if (e != 0) return e;
+    }
+    if (l.join) {
+        p.part_values = values;
+        p.part_stats = stats;
+        const unsigned workgroups = (unsigned) (((long long) p.batch * p.queries * p.heads + WAVES - 1) / WAVES);
+        if (l.wp == 64) hipLaunchKernelGGL(join_attention_kernel<64>, dim3(workgroups), dim3(64 * WAVES), 0, stream, p);
+        else hipLaunchKernelGGL(join_attention_kernel<128>, dim3(workgroups), dim3(64 * WAVES), 0, stream, p);
+        return (int) hipGetLastError();
+    }
+    return 0;
 }
 
 }  // namespace kn

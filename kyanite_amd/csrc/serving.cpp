@@ -2,6 +2,7 @@
 // launch parameters of the kernels declared in serving_kernels.h.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -189,7 +190,7 @@ bool plan_cached_attention(const knhip_cached_attention_args *args, ServingAtten
     p.cap = a.cap;
     p.slopes = a.slopes;
     p.causal = 1;
-    p.window = a.window;
+    p.window = std::min(a.window, 1 << 30);  // (no place is further away; keeps differences of places inside 32 bits)
     return false;
 }
 
@@ -232,7 +233,7 @@ bool plan_attention(const knhip_attention_args *args, ServingAttentionParams &p)
     p.cap = a.cap;
     p.slopes = a.slopes;
     p.causal = a.causal != 0;
-    p.window = a.window;
+    p.window = std::min(a.window, 1 << 30);  // (no place is further away; keeps differences of places inside 32 bits)
     p.spans = a.spans;
     p.prefix = a.prefix;
     return false;

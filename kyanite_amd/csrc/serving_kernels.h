@@ -65,6 +65,12 @@ struct ServingAttentionParams {
     const float *slopes;
     int causal, window;
     const int32_t *spans, *prefix;  // prompts only
+    // set by the launcher: rows that share a head of keys, partial results (in rows of the padded width) and where they lie
+    FastDiv group_div, queries_div;
+    float *part_values, *part_stats;  // [row][width], [row][reference, sum]
+    int32_t *part_items;  // [stretch][first item, items], the prefix first
+    long long row_prefix_part, row_own_part;
+    int prefix_splits, own_splits;
 };
 int launch_serving_attention(const ServingAttentionParams &p, void *workspace, ihipStream_t *stream);
 size_t serving_attention_workspace(const ServingAttentionParams &p);
