@@ -301,9 +301,9 @@ int knhip_attention(int device, void *stream, const knhip_attention_args *args, 
  * first index at which the sum of the kept w, taken in the order of the indices, exceeds uniform[r] times the whole sum;
  * its probability is its share of that sum. -inf and NaN are never drawn, +inf counts as infinitely more probable than any
  * finite logit; a row without anything to draw gives token -1 and probability 0. uniform lies in [0, 1) (other values
- * count as the nearest one in it). The w are f64, held in 64 bit fixed point: rounded to multiples of 2^-(62 - l) for a vocab
- * of up to 2^l, so that their sums are exact and the same in any order (a w below half a step, 2^-43 or less, is never
- * drawn). Parameters with a NULL address are off for every row (temperature: 1). vocab: up to 2^20. */
+ * count as the nearest one in it). The w are f64, held in 64 bit fixed point: rounded to multiples of 2^-min(51, 62 - l) for a
+ * vocab of up to 2^l, so that their sums are exact and the same in any order (a w below half a step, 2^-43 or less, is
+ * never drawn). Parameters with a NULL address are off for every row (temperature: 1). vocab: up to 2^20. */
 typedef struct {
     int dtype; /* KNHIP_F16 or KNHIP_F32 */
     int rows, vocab;

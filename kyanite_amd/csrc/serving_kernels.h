@@ -85,6 +85,7 @@ struct SampleParams {
     const int32_t *top_k;
     int32_t *tokens;
     float *probabilities;
+    int bits;  // set by the launcher: of the fixed point weights
 };
 int launch_sample(const SampleParams &p, void *workspace, ihipStream_t *stream);
 size_t sample_workspace(const SampleParams &p);

@@ -61,7 +61,7 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
         top = x.max()
         with np.errstate(invalid="ignore"):
             w = np.where(x == top, 1.0, 0.0 if top == np.inf else np.exp((x - top) / t))
-        real, step = w, 2.0 ** (math.ceil(math.log2(len(x))) - 62)
+        real, step = w, 2.0 ** -min(51, 62 - math.ceil(math.log2(len(x))))
         w = np.round(w / step) * step  # the fixed point of the definition: smaller weights are never drawn
         order = np.argsort(-x, kind="stable")
         order = order[x[order] > -np.inf]
