@@ -5,14 +5,15 @@
 // argument are f64: the nearest of 10^5 borders between tokens is then missed once in 10^10 rows or so.
 //
 // A row belongs to one workgroup of 16 waves, each of which owns a contiguous part of it. Rows that fit are held in LDS
-// (f16: 60000 logits), so that they are read once. The filters end in one threshold, the last token that stays in the order of
-// falling logits (ties: rising index). It is found without sorting:
+// (f16: 60000 logits), so that they are read once; what then bounds a row is the arithmetic per logit of one compute unit.
+// The filters end in one threshold, the last token that stays in the order of falling logits (ties: rising index):
 //   1. a histogram over the distance to the maximum, 2048 buckets over the distances at which w is not zero, counts for
 //      top_k, masses for top_p. (Buckets on the bits of x would put most of a row into two dozen of them: the atomics of a
 //      wave would queue. Over the distance a normal distribution fills hundreds.)
-//   2. the bucket where the count or the mass is reached; its tokens, usually a hundred, are ranked against each other.
-// A bucket with more than 1024 tokens (flat rows) is searched by the bits of x instead, 8 at a time.
-// The token is then found in two steps: the wave whose part holds the target, and the place inside that part.
+//   2. the tokens of the bucket where the count or the mass is reached, usually a hundred, are sorted.
+// With top_k, all tokens down to that bucket are sorted instead where they are 2048 at most, and the other filters and the
+// draw work on that list alone. A bucket with more than 2048 tokens (flat rows) is searched by the bits of x, 8 at a time.
+// Without a list the token is found in two steps: the wave whose part holds the target, and the place inside that part.
 #include <hip/hip_runtime.h>
 
 #include "../serving_kernels.h"
@@ -22,8 +23,8 @@ namespace kn {
 namespace {
 
 constexpr int THREADS = 1024, NWAVES = THREADS / 64;
-constexpr int BUCKETS = 2 * THREADS, CANDIDATES = THREADS;
-constexpr int CACHE_BYTES = 120 * 1024;
+constexpr int BUCKETS = 2 * THREADS, LISTED = 2 * THREADS;
+constexpr int CACHE_BYTES = 116 * 1024;
 
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 typedef _Float16 halfx8_any __attribute__((ext_vector_type(8), aligned(2)));
@@ -31,12 +32,12 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned long long mass_t;
 
-// NaN counts as -inf, -0 as +0
-__device__ __forceinline__ float plain(float x) { return x != x ? -INFINITY : x + 0.0f; }
+// NaN counts as -inf
+__device__ __forceinline__ float plain(float x) { return fmaxf(x, -INFINITY); }
 
-// the bits of x as an unsigned number that grows with x
+// the bits of x as an unsigned number that grows with x (-0 as +0, the two are equal)
 __device__ __forceinline__ unsigned key_of(float x) {
-    const unsigned u = __builtin_bit_cast(unsigned, x);
+    const unsigned u = __builtin_bit_cast(unsigned, x + 0.0f);
     return u ^ ((unsigned) ((int) u >> 31) | 0x80000000u);
 }
 
@@ -109,14 +110,18 @@ struct Weigher {
     __device__ __forceinline__ mass_t operator()(float x) const { return whole(real(x)); }
 };
 
+__device__ __forceinline__ float logit_of(unsigned key) {
+    return __builtin_bit_cast(float, key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+
 struct Shared {
     mass_t hist[BUCKETS];
-    unsigned cand_key[CANDIDATES], cand_index[CANDIDATES];
-    mass_t cand_mass[CANDIDATES];
+    mass_t list[LISTED];  // key and, below it, the complement of the index: falling order is the order of the filters
+    float queue[NWAVES][128];
     double roots[64];
     mass_t wave_mass[NWAVES];
     float wave_top[NWAVES];
-    int cand_count, bucket;
+    int list_count, bucket;
     mass_t above;
     unsigned last_key;  // the threshold: the last token that stays
     int last_index;
@@ -137,6 +142,43 @@ __device__ __forceinline__ mass_t wave_sum(mass_t v) {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
     return v;
+}
+
+// sums over the threads of the workgroup up to and with this one; `shared`: a place per wave
+__device__ __forceinline__ mass_t block_scan(mass_t v, mass_t *shared) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    v = wave_scan(v, lane);
+    __syncthreads();
+    if (lane == 63) shared[wave] = v;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) v += shared[w];
+    return v;
+}
+
+// the first `count` entries of the list into falling (or rising) order
+__device__ __forceinline__ void sort_list(mass_t *list, int count, bool rising) {
+    int size = 2;
+    while (size < count) size *= 2;
+    __syncthreads();
+    for (int i = count + (int) threadIdx.x; i < size; i += THREADS) list[i] = rising ? ~0ull : 0;
+    for (int run = 2; run <= size; run *= 2)
+        for (int step = run / 2; step > 0; step /= 2) {
+            __syncthreads();
+            if ((int) threadIdx.x < size / 2) {
+                const int i = 2 * (int) threadIdx.x - ((int) threadIdx.x & (step - 1)), j = i + step;
+                const mass_t a = list[i], b = list[j];
+                const bool up = rising == ((i & run) == 0);
+                if (up ? a > b : a < b) {
+                    list[i] = b;
+                    list[j] = a;
+                }
+            }
+        }
+    __syncthreads();
+}
+
+__device__ __forceinline__ mass_t target_of(float u, mass_t total) {
+    return (mass_t) ((double) (u >= 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f) * (double) total);
 }
 
 template <bool F16, bool CACHED>
@@ -161,6 +203,15 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
             for (int a = 0; a < AHEAD; a++) f((n + 64 * a) * N, unpack<F16>(raw[a]));
         }
         for (; n < end; n += 64) f(n * N, unpack<F16>(CACHED ? cache[n] : load_raw<F16>(row, n, p.vocab)));
+    };
+
+    // the same with all lanes of the wave together, f(first index, values, whether there are any)
+    auto each_in_step = [&](auto f) {
+        for (int n0 = begin; n0 < end; n0 += 64) {
+            const int n = n0 + lane;
+            const bool live = n < end;
+            f(n * N, unpack<F16>(CACHED ? cache[live ? n : begin] : load_raw<F16>(row, live ? n : begin, p.vocab)), live);
+        }
     };
 
     // ---- the maximum (and the row into LDS)
@@ -218,221 +269,308 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     const Weigher weigh{top, 92.332482616893656877 / (double) t, p.bits, sh.roots};
     const int k = p.top_k ? p.top_k[r] : 0;
     const float top_p = p.top_p ? p.top_p[r] : 1.0f;
-    const double min_w = p.min_p ? __builtin_ldexp((double) p.min_p[r], p.bits) : 0.0;
     // distances at which w may be more than zero: exp(-range / T) 2^bits = 1 / 4
     const float range = t * (0.6931472f * (p.bits + 2)), per_bucket = fminf(BUCKETS / range, 3e38f);
-    const bool spread = range < 1e37f;
-    auto bucket_of = [&](float x) {
-        const float away = x == top ? 0.0f : top - x;
-        return away < range ? min((int) (away * per_bucket), BUCKETS - 1) : BUCKETS;
-    };
+    const bool spread = range < 1e37f && top < INFINITY;
+    auto bucket_of = [&](float x) { return (unsigned) ((top - x) * per_bucket); };  // (saturates: -inf falls behind the last)
     unsigned last_key = 0;  // what stays: larger keys, and this key up to last_index
     int last_index = p.vocab;
+    bool restricted = false;
     auto stays = [&](unsigned key, int i) { return key > last_key || (key == last_key && i <= last_index); };
+    const double mass_wanted = top_p < 1.0f ? fmax((double) top_p, 0.0) : 1.0;
+    const double min_w = p.min_p ? __builtin_ldexp((double) p.min_p[r], p.bits) : 0.0;
 
-    // The threshold at which `enough(tokens, mass)`, called with what lies at and above a token, first holds, among what stays
-    // so far; tokens without weight have no part in it. `by_mass`: whether masses are needed.
-    auto tighten = [&](bool by_mass, auto enough) {
-        bool found = false;
-        if (spread) {
-            __syncthreads();
-            for (int b = threadIdx.x; b < BUCKETS; b += THREADS) sh.hist[b] = 0;
-            if (threadIdx.x == 0) {
-                sh.cand_count = 0;
-                sh.bucket = BUCKETS;
-            }
-            __syncthreads();
-            each([&](int i, const Vec<F16> &v) {
+    // ---- the histogram of what stays so far, and the bucket where enough is reached
+    auto fill_hist = [&](bool by_mass) {
+        __syncthreads();
+        for (int b = threadIdx.x; b < BUCKETS; b += THREADS) sh.hist[b] = 0;
+        if (threadIdx.x == 0) {
+            sh.list_count = 0;
+            sh.bucket = BUCKETS;
+        }
+        __syncthreads();
+        each([&](int i, const Vec<F16> &v) {
 #pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const int b = bucket_of(v.x[e]);
-                    if (b < BUCKETS && stays(key_of(v.x[e]), i + e)) {
-                        if (by_mass) atomicAdd(&sh.hist[b], weigh(v.x[e]));
-                        else atomicAdd((unsigned *) &sh.hist[b], 1u);
-                    }
-                }
-            });
-            __syncthreads();
-            // a thread takes two neighbouring buckets
-            const mass_t a = sh.hist[2 * threadIdx.x], both = a + sh.hist[2 * threadIdx.x + 1];
-            mass_t sums = wave_scan(both, lane);
-            if (lane == 63) sh.wave_mass[wave] = sums;
-            __syncthreads();
-            mass_t before = sums - both;
-            for (int w = 0; w < wave; w++) before += sh.wave_mass[w];
-            auto reached = [&](mass_t m) { return by_mass ? enough(0u, m) : enough((unsigned) m, (mass_t) 0); };
-            if (both && !reached(before) && reached(before + both)) {
-                const bool second = a == 0 || !reached(before + a);
-                sh.bucket = 2 * threadIdx.x + second;
-                sh.above = before + (second ? a : 0);
+            for (int e = 0; e < N; e++) {
+                const unsigned b = bucket_of(v.x[e]);
+                if (b >= BUCKETS || (restricted && !stays(key_of(v.x[e]), i + e))) continue;
+                if (by_mass) atomicAdd(&sh.hist[b], weigh(v.x[e]));
+                else atomicAdd((unsigned *) &sh.hist[b], 1u);
             }
-            if (threadIdx.x == 0 && reached(0)) {  // (a top_p of zero: the largest stays)
-                sh.bucket = 0;
-                sh.above = 0;
+        });
+        __syncthreads();
+    };
+    // sh.bucket, sh.above: the first bucket at whose end `need` is reached, and what lies before it; BUCKETS when it never is.
+    // Masses: `need` is mass_wanted of all. Returns `need`.
+    auto find_bucket = [&](bool by_mass, mass_t need) {
+        // a thread takes two neighbouring buckets
+        const mass_t a = sh.hist[2 * threadIdx.x], both = a + sh.hist[2 * threadIdx.x + 1];
+        const mass_t sums = block_scan(both, sh.wave_mass), before = sums - both;
+        if (by_mass) {
+            mass_t all = 0;
+            for (int w = 0; w < NWAVES; w++) all += sh.wave_mass[w];
+            need = (mass_t) __builtin_ceil(mass_wanted * (double) all);
+            if (need == 0) need = 1;  // (the most probable token stays)
+        }
+        if (before < need && need <= before + both) {
+            const bool second = before + a < need;
+            sh.bucket = 2 * threadIdx.x + second;
+            sh.above = before + (second ? a : 0);
+        }
+        __syncthreads();
+        return need;
+    };
+    // the tokens of the buckets from..to among what stays, as far as they fit
+    auto gather = [&](unsigned from, unsigned to) {
+        each([&](int i, const Vec<F16> &v) {
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const unsigned b = bucket_of(v.x[e]);
+                if (b < from || b > to) continue;
+                const unsigned key = key_of(v.x[e]);
+                if (restricted && !stays(key, i + e)) continue;
+                const int c = atomicAdd(&sh.list_count, 1);
+                if (c < LISTED) sh.list[c] = (mass_t) key << 32 | ~(unsigned) (i + e);
+            }
+        });
+        __syncthreads();
+    };
+    auto mass_of_entry = [&](mass_t entry) { return weigh(logit_of((unsigned) (entry >> 32))); };
+
+    // the threshold by the bits of x, 8 from the top at a time: slow, for any row
+    auto search = [&](bool by_mass, mass_t need) {
+        mass_t *masses = sh.hist;
+        unsigned *counts = (unsigned *) (sh.hist + 256);
+        unsigned prefix = 0, above_count = 0;
+        mass_t above_mass = 0;
+        auto enough = [&](unsigned count, mass_t mass) { return (by_mass ? mass : (mass_t) count) >= need; };
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            __syncthreads();
+            if (threadIdx.x < 256) {
+                masses[threadIdx.x] = 0;
+                counts[threadIdx.x] = 0;
             }
             __syncthreads();
-            const int bucket = sh.bucket;
-            if (bucket == BUCKETS) return;  // everything that weighs anything stays
-            const mass_t above = sh.above;
             each([&](int i, const Vec<F16> &v) {
 #pragma unroll
                 for (int e = 0; e < N; e++) {
                     const unsigned key = key_of(v.x[e]);
-                    if (bucket_of(v.x[e]) != bucket || !stays(key, i + e)) continue;
-                    const int c = atomicAdd(&sh.cand_count, 1);
-                    if (c >= CANDIDATES) continue;
-                    sh.cand_key[c] = key;
-                    sh.cand_index[c] = i + e;
-                    sh.cand_mass[c] = by_mass ? weigh(v.x[e]) : 1;
+                    if (v.x[e] == -INFINITY || !stays(key, i + e) || (shift < 24 && (key >> (shift + 8)) != prefix)) continue;
+                    atomicAdd(&counts[(key >> shift) & 255], 1u);
+                    if (by_mass) atomicAdd(&masses[(key >> shift) & 255], weigh(v.x[e]));
                 }
             });
             __syncthreads();
-            const int count = sh.cand_count;
-            found = count <= CANDIDATES;
-            if (found && (int) threadIdx.x < count) {
-                const unsigned key = sh.cand_key[threadIdx.x], index = sh.cand_index[threadIdx.x];
-                mass_t first = above;
-                for (int c = 0; c < count; c++)
-                    if (sh.cand_key[c] > key || (sh.cand_key[c] == key && sh.cand_index[c] < index)) first += sh.cand_mass[c];
-                const mass_t with = first + sh.cand_mass[threadIdx.x];
-                // (the largest token stays even if nothing is wanted)
-                if ((!reached(first) || (bucket == 0 && first == 0)) && reached(with) && (with > first || first == 0)) {
-                    sh.last_key = key;
-                    sh.last_index = (int) index;
+            if (threadIdx.x == 0) {
+                int last = -1, digit = 255;
+                for (; digit >= 0; digit--) {
+                    if (counts[digit] == 0) continue;
+                    last = digit;
+                    if (enough(above_count + counts[digit], above_mass + masses[digit])) break;
+                    above_count += counts[digit];
+                    above_mass += masses[digit];
                 }
+                if (digit < 0) {  // all of them: end at the lowest
+                    above_count -= counts[last];
+                    above_mass -= masses[last];
+                    digit = last;
+                }
+                sh.search_prefix = (prefix << 8) | (unsigned) digit;
+                sh.search_count = above_count;
+                sh.search_mass = above_mass;
             }
             __syncthreads();
+            prefix = sh.search_prefix;
+            above_count = sh.search_count;
+            above_mass = sh.search_mass;
         }
-        if (!found) {
-            // by the bits of x, from the top: the digit at which it is enough, four times
-            mass_t *masses = sh.hist;
-            unsigned *counts = (unsigned *) (sh.hist + 256);
-            unsigned prefix = 0, above_count = 0;
-            mass_t above_mass = 0;
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                __syncthreads();
-                if (threadIdx.x < 256) {
-                    masses[threadIdx.x] = 0;
-                    counts[threadIdx.x] = 0;
-                }
-                __syncthreads();
-                each([&](int i, const Vec<F16> &v) {
-#pragma unroll
-                    for (int e = 0; e < N; e++) {
-                        const unsigned key = key_of(v.x[e]);
-                        if (v.x[e] == -INFINITY || !stays(key, i + e) || (shift < 24 && (key >> (shift + 8)) != prefix)) continue;
-                        atomicAdd(&counts[(key >> shift) & 255], 1u);
-                        if (by_mass) atomicAdd(&masses[(key >> shift) & 255], weigh(v.x[e]));
-                    }
-                });
-                __syncthreads();
-                if (threadIdx.x == 0) {
-                    int last = -1, digit = 255;
-                    for (; digit >= 0; digit--) {
-                        if (counts[digit] == 0) continue;
-                        last = digit;
-                        if (enough(above_count + counts[digit], above_mass + masses[digit])) break;
-                        above_count += counts[digit];
-                        above_mass += masses[digit];
-                    }
-                    if (digit < 0) {  // all of them: end at the lowest
-                        above_count -= counts[last];
-                        above_mass -= masses[last];
-                        digit = last;
-                    }
-                    sh.search_prefix = (prefix << 8) | (unsigned) digit;
-                    sh.search_count = above_count;
-                    sh.search_mass = above_mass;
-                }
-                __syncthreads();
-                prefix = sh.search_prefix;
-                above_count = sh.search_count;
-                above_mass = sh.search_mass;
-            }
-            // how many of the tokens with this key stay, then the index of the last of them
-            const unsigned equal = counts[prefix & 255];
-            const mass_t one = by_mass ? masses[prefix & 255] / equal : 0;
-            unsigned few = 1, most = equal;
-            while (few < most) {
-                const unsigned middle = (few + most) / 2;
-                if (enough(above_count + middle, above_mass + middle * one)) most = middle;
-                else few = middle + 1;
-            }
-            int mine = 0;
-            each([&](int i, const Vec<F16> &v) {
-#pragma unroll
-                for (int e = 0; e < N; e++) mine += key_of(v.x[e]) == prefix && stays(prefix, i + e);
-            });
-            __syncthreads();
-            mine = (int) wave_sum((mass_t) mine);
-            if (lane == 0) sh.wave_mass[wave] = (mass_t) mine;
-            if (threadIdx.x == 0) sh.last_key = prefix;
-            __syncthreads();
-            int before = 0;
-            for (int w = 0; w < wave; w++) before += (int) sh.wave_mass[w];
-            if (before < (int) most && (int) most <= before + mine) {  // in this wave's part
-                for (int i0 = begin * N; i0 < end * N; i0 += 64) {
-                    const int i = i0 + lane;
-                    const bool hit = i < min(end * N, p.vocab) && key_of(load_one<F16>(row, i)) == prefix && stays(prefix, i);
-                    const unsigned long long hits = __ballot(hit);
-                    if (before + __popcll(hits) >= (int) most) {
-                        if (hit && before + __popcll(hits & ((2ull << lane) - 1)) == (int) most) sh.last_index = i;
-                        break;
-                    }
-                    before += __popcll(hits);
-                }
-            }
-            __syncthreads();
+        // how many of the tokens with this key stay, then the index of the last of them
+        const unsigned equal = counts[prefix & 255];
+        const mass_t one = by_mass ? masses[prefix & 255] / equal : 0;
+        unsigned few = 1, most = equal;
+        while (few < most) {
+            const unsigned middle = (few + most) / 2;
+            if (enough(above_count + middle, above_mass + middle * one)) most = middle;
+            else few = middle + 1;
         }
-        last_key = sh.last_key;
-        last_index = sh.last_index;
-        __syncthreads();
-    };
-    if (k > 0 && k < p.vocab) tighten(false, [&](unsigned tokens, mass_t) { return tokens >= (unsigned) k; });
-    auto weight_of = [&](float x, int i) -> mass_t {
-        if (x == -INFINITY || !stays(key_of(x), i)) return 0;
-        const double w = weigh.real(x);
-        return w >= min_w || x == top ? Weigher::whole(w) : 0;
-    };
-    auto part_mass = [&](auto weight) {  // of this wave; all waves' in sh.wave_mass
-        mass_t mass = 0;
+        int mine = 0;
         each([&](int i, const Vec<F16> &v) {
 #pragma unroll
-            for (int e = 0; e < N; e++) mass += weight(v.x[e], i + e);
+            for (int e = 0; e < N; e++) mine += key_of(v.x[e]) == prefix && stays(prefix, i + e);
         });
+        __syncthreads();
+        mine = (int) wave_sum((mass_t) mine);
+        if (lane == 0) sh.wave_mass[wave] = (mass_t) mine;
+        if (threadIdx.x == 0) sh.last_key = prefix;
+        __syncthreads();
+        int before = 0;
+        for (int w = 0; w < wave; w++) before += (int) sh.wave_mass[w];
+        if (before < (int) most && (int) most <= before + mine) {  // in this wave's part
+            for (int i0 = begin * N; i0 < end * N; i0 += 64) {
+                const int i = i0 + lane;
+                const bool hit = i < min(end * N, p.vocab) && key_of(load_one<F16>(row, i)) == prefix && stays(prefix, i);
+                const unsigned long long hits = __ballot(hit);
+                if (before + __popcll(hits) >= (int) most) {
+                    if (hit && before + __popcll(hits & ((2ull << lane) - 1)) == (int) most) sh.last_index = i;
+                    break;
+                }
+                before += __popcll(hits);
+            }
+        }
+        __syncthreads();
+    };
+    // ---- the filters, counts and then masses (one loop, so that each piece of code is there once)
+#pragma unroll 1
+    for (int filter = 0; filter < 2; filter++) {
+        const bool by_mass = filter == 1;
+        if (by_mass ? !(top_p < 1.0f) : !(k > 0 && k < p.vocab)) continue;
+        mass_t need = (mass_t) k;
+        bool found = false;
+        if (spread) {
+            fill_hist(by_mass);
+            need = find_bucket(by_mass, need);
+            const int bucket = sh.bucket;
+            const mass_t above = sh.above;
+            if (bucket == BUCKETS) continue;  // everything that weighs anything stays
+            if (!by_mass && above + sh.hist[bucket] <= LISTED) {
+                // ---- few tokens: a list, in falling order for the filters, in the order of the indices for the draw
+                gather(0, (unsigned) bucket);
+                const int count = sh.list_count, most = min(k, count);
+                sort_list(sh.list, count, false);
+                mass_t entry[2], w[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int i = 2 * (int) threadIdx.x + e;
+                    entry[e] = i < most ? sh.list[i] : 0;
+                    w[e] = i < most ? mass_of_entry(entry[e]) : 0;
+                }
+                mass_t with = block_scan(w[0] + w[1], sh.wave_mass), all = 0;
+                for (int i = 0; i < NWAVES; i++) all += sh.wave_mass[i];
+                mass_t before = with - w[0] - w[1];
+                const mass_t need = top_p < 1.0f ? max((mass_t) __builtin_ceil(mass_wanted * (double) all), 1ull) : ~0ull;
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int i = 2 * (int) threadIdx.x + e;
+                    const float x = logit_of((unsigned) (entry[e] >> 32));
+                    const bool kept = i < most && before < need && (x == top || weigh.real(x) >= min_w);
+                    before += w[e];
+                    // index first now; what does not stay goes to the end
+                    if (i < count) sh.list[i] = kept ? (mass_t) ~(unsigned) entry[e] << 32 | (entry[e] >> 32) : ~0ull;
+                }
+                sort_list(sh.list, count, true);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int i = 2 * (int) threadIdx.x + e;
+                    entry[e] = i < count ? sh.list[i] : ~0ull;
+                    w[e] = entry[e] == ~0ull ? 0 : weigh(logit_of((unsigned) entry[e]));
+                }
+                with = block_scan(w[0] + w[1], sh.wave_mass);
+                mass_t total = 0;
+                for (int i = 0; i < NWAVES; i++) total += sh.wave_mass[i];
+                const mass_t target = target_of(p.uniform[r], total);
+                before = with - w[0] - w[1];
+                if (before <= target && target < with) {
+                    const int e = target < before + w[0] ? 0 : 1;
+                    p.tokens[r] = (int) ((e ? entry[1] : entry[0]) >> 32);
+                    if (p.probabilities) p.probabilities[r] = (float) ((double) (e ? w[1] : w[0]) / (double) total);
+                }
+                return;
+            }
+            gather((unsigned) bucket, (unsigned) bucket);
+            const int count = sh.list_count;
+            if (count <= LISTED) {
+                found = true;
+                sort_list(sh.list, count, false);
+                mass_t entry[2], w[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int i = 2 * (int) threadIdx.x + e;
+                    entry[e] = i < count ? sh.list[i] : 0;
+                    w[e] = i >= count ? 0 : by_mass ? mass_of_entry(entry[e]) : 1;
+                }
+                const mass_t with = above + block_scan(w[0] + w[1], sh.wave_mass), before = with - w[0] - w[1];
+                if (before < need && need <= with) {
+                    const mass_t last = need <= before + w[0] ? entry[0] : entry[1];
+                    sh.last_key = (unsigned) (last >> 32);
+                    sh.last_index = (int) ~(unsigned) last;
+                }
+                __syncthreads();
+            }
+        } else if (by_mass) {
+            mass_t mass = 0;
+            each([&](int i, const Vec<F16> &v) {
+#pragma unroll
+                for (int e = 0; e < N; e++)
+                    if (stays(key_of(v.x[e]), i + e)) mass += weigh(v.x[e]);
+            });
+            mass = wave_sum(mass);
+            __syncthreads();
+            if (lane == 0) sh.wave_mass[wave] = mass;
+            __syncthreads();
+            mass_t all = 0;
+            for (int w = 0; w < NWAVES; w++) all += sh.wave_mass[w];
+            need = max((mass_t) __builtin_ceil(mass_wanted * (double) all), 1ull);
+        }
+        if (!found) search(by_mass, need);
+        last_key = sh.last_key;
+        last_index = sh.last_index;
+        restricted = true;
+    }
+
+    auto part_masses = [&] {  // sh.wave_mass: the masses of the waves' parts
+        // The tokens that stay are queued in LDS until there are 64 of them: where few of them stay, a wave would
+        // otherwise weigh 64 for the sake of some.
+        mass_t mass = 0;
+        int queued = 0;
+        float *queue = sh.queue[wave];
+        auto kept = [&](float x) -> mass_t {
+            const double w = weigh.real(x);
+            return w >= min_w || x == top ? Weigher::whole(w) : 0;
+        };
+        each_in_step([&](int i, const Vec<F16> &v, bool live) {
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const bool hit = live && v.x[e] > -INFINITY && (!restricted || stays(key_of(v.x[e]), i + e));
+                const unsigned long long hits = __ballot(hit);
+                if (hit) queue[queued + __popcll(hits & ((1ull << lane) - 1))] = v.x[e];
+                queued += __popcll(hits);
+                if (queued >= 64) {
+                    __builtin_amdgcn_wave_barrier();
+                    mass += kept(queue[lane]);
+                    const float rest = queue[64 + lane];
+                    __builtin_amdgcn_wave_barrier();
+                    queue[lane] = rest;
+                    queued -= 64;
+                }
+            }
+        });
+        __builtin_amdgcn_wave_barrier();
+        if (lane < queued) mass += kept(queue[lane]);
         mass = wave_sum(mass);
         __syncthreads();
         if (lane == 0) sh.wave_mass[wave] = mass;
         __syncthreads();
     };
-    if (top_p < 1.0f) {
-        part_mass([&](float x, int i) -> mass_t { return x == -INFINITY || !stays(key_of(x), i) ? 0 : weigh(x); });
-        mass_t all = 0;
-        for (int w = 0; w < NWAVES; w++) all += sh.wave_mass[w];
-        const mass_t need = (mass_t) __builtin_ceil(fmax((double) top_p, 0.0) * (double) all);
-        tighten(true, [&](unsigned, mass_t mass) { return mass >= need; });
-    }
-
     // ---- the draw
-    part_mass(weight_of);
+    part_masses();
     mass_t total = 0;
     for (int w = 0; w < NWAVES; w++) total += sh.wave_mass[w];
-    const float u = p.uniform[r];
-    const mass_t target = (mass_t) ((double) (u >= 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f) * (double) total);
+    const mass_t target = target_of(p.uniform[r], total);
     int chosen = 0;
     mass_t before = 0;
     while (chosen < NWAVES - 1 && before + sh.wave_mass[chosen] <= target) before += sh.wave_mass[chosen++];
-    __syncthreads();
     // the part that holds the target, shared by all threads
+    auto weight_of = [&](float x, int i) -> mass_t {
+        if (x == -INFINITY || !stays(key_of(x), i)) return 0;
+        const double w = weigh.real(x);
+        return w >= min_w || x == top ? Weigher::whole(w) : 0;
+    };
     const int from = chosen * part * N, to = min(from + part * N, p.vocab), per = (to - from + THREADS - 1) / THREADS;
     const int mine = min(from + (int) threadIdx.x * per, to), mine_end = min(mine + per, to);
     mass_t mass = 0;
     for (int i = mine; i < mine_end; i++) mass += weight_of(load_one<F16>(row, i), i);
-    const mass_t sums = wave_scan(mass, lane);
-    if (lane == 63) sh.wave_mass[wave] = sums;
-    __syncthreads();
-    before += sums - mass;
-    for (int w = 0; w < wave; w++) before += sh.wave_mass[w];
+    before += block_scan(mass, sh.wave_mass) - mass;
     if (!(before <= target && target < before + mass)) return;
     for (int i = mine; i < mine_end; i++) {
         const mass_t w = weight_of(load_one<F16>(row, i), i);
