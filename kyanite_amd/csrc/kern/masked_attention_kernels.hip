@@ -35,6 +35,7 @@ typedef _Float16 halfx8_any __attribute__((ext_vector_type(8), aligned(2)));
 typedef _Float16 halfx4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -54,8 +55,9 @@ struct Row {
 __device__ __forceinline__ int own_length(const ServingAttentionParams &p, int b) { return min(max(p.lengths[b], 0), p.table_tokens); }
 
 // Row `r` of kv head `kv_head`: (token, head of the group) of sequence `b`, of all sequences for the prefix
+// (`length`: of the sequence, when the caller has it)
 template <int STRETCH>
-__device__ __forceinline__ Row row_of(const ServingAttentionParams &p, unsigned r, int b, int kv_head) {
+__device__ __forceinline__ Row row_of(const ServingAttentionParams &p, unsigned r, int b, int kv_head, int length = -1) {
     Row w;
     const unsigned token = p.group_div.div(r);
     w.head = kv_head * (int) p.group_div.d + (int) (r - token * p.group_div.d);
@@ -71,7 +73,7 @@ __device__ __forceinline__ Row row_of(const ServingAttentionParams &p, unsigned 
         w.hi = p.keys;
         if (p.causal) w.hi = min(w.hi, max(w.at + 1, p.prefix ? p.prefix[w.b] : 0));
     } else {
-        const int own = own_length(p, w.b) - p.queries + w.t;  // below 0: a query of padding
+        const int own = (STRETCH == OWN && length >= 0 ? length : own_length(p, w.b)) - p.queries + w.t;  // below 0: a query of padding
         w.at = STRETCH == OWN ? own : p.prefix_tokens + own;
         w.hi = own < 0 ? 0 : STRETCH == OWN ? own + 1 : p.prefix_tokens;
     }
@@ -472,8 +474,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 // ---- up to 16 NT rows per workgroup --------------------------------------------------------------------------------
 
 // Decoding: bound by the bytes of the cache, which pass through once. A workgroup takes a stretch of keys of one sequence
-// and head, its four waves every fourth step of 32 keys; nothing is staged in LDS, so that many waves fit a compute unit and
-// keep the memory busy between them. Both products take 16 keys or dims by 16 rows (v_mfma_f32_16x16x32_f16):
+// and head, its eight waves every eighth step of 32 keys; nothing is staged in LDS. The registers of a step's keys are
+// loaded again as soon as the scores are there, those of its values as soon as they are summed, so that a wave always has
+// loads in flight. Both products take 16 keys or dims by 16 rows (v_mfma_f32_16x16x32_f16):
 //   S^T = K Q^T      lane (key i = lane % 16, g = lane / 16) reads 16 byte pieces of key i, 64 bytes of a row per load of four
 //                    lanes; the order of a row's elements in the product is free, Q is loaded in the same one
 //   O^T += V^T P^T   the accumulators of two tiles of S^T are the operand, keys 4 g + e and 16 + 4 g + e; lane (i, g) reads
@@ -484,71 +487,68 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 
 // Which keys a workgroup takes, decided on the device, where the lengths are: stretches (the prefix when it is done here, then
 // every sequence's own keys) are cut into items of about the same size, ROW_ITEMS of them over all heads, and workgroup x
-// takes item x / kv_heads. The grid covers the largest number of items that any lengths can give.
-constexpr int ROW_ITEMS = 1024, ROW_MIN_KEYS = 128, ROW_THREADS = 64 * WAVES;
-
-__device__ __forceinline__ int2 stretch_range(const ServingAttentionParams &p, int seg) {  // the keys that any of its rows may see
-    if (seg < 0) return int2{0, p.prefix_tokens};
-    const int n = own_length(p, seg);
-    return int2{p.window ? max(0, n - p.queries + 1 - p.window) & ~31 : 0, n};
-}
+// takes item x / kv_heads. The grid covers the largest number of items that any lengths can give. Parts of less than
+// ROW_MIN_KEYS keys are not made: four steps per wave take less time than the launch that joins two parts.
+constexpr int ROW_ITEMS = 512, ROW_MIN_KEYS = 1024, ROW_WAVES = 8, ROW_THREADS = 64 * ROW_WAVES;
 
 struct Item {
-    int seg, from, end, items;
+    int seg, length, from, end, items;
 };
 
-// segments -1 (the prefix, when `with_prefix`) and 0 .. batch - 1; false when there is no such item
-__device__ __forceinline__ bool find_item(const ServingAttentionParams &p, bool with_prefix, int item, Item &out) {
-    __shared__ long long wave_steps[WAVES];
-    __shared__ int wave_sums[WAVES];
-    __shared__ Item found;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int first = with_prefix ? -1 : 0;
+// segments -1 (the prefix, when `with_prefix`) and 0 .. batch - 1; false when there is no such item. Every wave works it out
+// for itself, a lane per segment.
+__device__ __forceinline__ bool find_item(const ServingAttentionParams &p, int with_prefix, int item, Item &out) {
+    const int lane = threadIdx.x & 63, segs = p.batch + with_prefix;
+    auto range = [&](int s) {  // (length, first key that any row may see: a multiple of 32)
+        if (s >= segs) return int2{0, 0};
+        if (s < with_prefix) return int2{p.prefix_tokens, 0};
+        const int n = own_length(p, s - with_prefix);
+        return int2{n, p.window ? max(0, n - p.queries + 1 - p.window) & ~31 : 0};
+    };
+    const int2 first = range(lane);
     long long steps = 0;  // of 32 keys, of all stretches (64 bits: many long tables may share pages)
-    for (int seg = first + (int) threadIdx.x; seg < p.batch; seg += ROW_THREADS) {
-        const int2 r = stretch_range(p, seg);
-        steps += (r.y - r.x + 31) / 32;
+    for (int s0 = 0; s0 < segs; s0 += 64) {
+        const int2 r = s0 ? range(s0 + lane) : first;
+        steps += (r.x - r.y + 31) / 32;
     }
+    if (segs <= 64) {
+        unsigned few = (unsigned) steps;  // (at most 64 stretches of 2^25 steps)
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) steps += __shfl_xor(steps, m);
-    if (lane == 0) wave_steps[wave] = steps;
-    if (threadIdx.x == 0) found.seg = -2;
-    __syncthreads();
-    steps = wave_steps[0] + wave_steps[1] + wave_steps[2] + wave_steps[3];
+        for (int m = 1; m < 64; m <<= 1) few += __shfl_xor(few, m);
+        steps = few;
+    } else {
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) steps += __shfl_xor(steps, m);
+    }
     // steps per item; no stretch has more than 2^26
     const int each = max(ROW_MIN_KEYS / 32, (int) min((steps * p.kv_heads + ROW_ITEMS - 1) / ROW_ITEMS, 1ll << 26));
     int base = 0;
-    for (int seg0 = first; seg0 < p.batch; seg0 += ROW_THREADS) {
-        const int seg = seg0 + (int) threadIdx.x;
-        int n = 0;
-        int2 r = {0, 0};
-        if (seg < p.batch) {
-            r = stretch_range(p, seg);
-            n = max(1, ((r.y - r.x + 31) / 32 + each - 1) / each);
-        }
+    for (int s0 = 0; s0 < segs; s0 += 64) {
+        const int2 r = s0 ? range(s0 + lane) : first;
+        const int own_steps = (r.x - r.y + 31) / 32, n = s0 + lane < segs ? max(1, (own_steps + each - 1) / each) : 0;
         int sums = n;
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) {
             const int other = __shfl_up(sums, m);
             if (lane >= m) sums += other;
         }
-        __syncthreads();
-        if (lane == 63) wave_sums[wave] = sums;
-        __syncthreads();
-        int before = base + sums - n;
-        for (int w = 0; w < wave; w++) before += wave_sums[w];
-        if (n > 0 && item >= before && item < before + n) {
+        const int before = base + sums - n;
+        const unsigned long long hit = __ballot(n > 0 && item >= before && item < before + n);
+        if (hit) {
             // the items of a stretch have the same number of steps, but for the last
-            const int per = 32 * (((r.y - r.x + 31) / 32 + n - 1) / n), from = r.x + (item - before) * per;
-            found = Item{seg, min(from, r.y), min(from + per, r.y), n};
-            if (item == before) ((int2 *) p.part_items)[seg + 1] = int2{before, n};
+            const int l = __builtin_ctzll(hit), begin = __builtin_amdgcn_readlane(r.y, l), nth = item - __builtin_amdgcn_readlane(before, l);
+            out.items = __builtin_amdgcn_readlane(n, l);
+            out.seg = s0 + l - with_prefix;
+            out.length = __builtin_amdgcn_readlane(r.x, l);
+            const int per = 32 * ((__builtin_amdgcn_readlane(own_steps, l) + out.items - 1) / out.items);
+            out.from = min(begin + nth * per, out.length);
+            out.end = min(begin + nth * per + per, out.length);
+            if (nth == 0 && threadIdx.x == 0) ((int2 *) p.part_items)[out.seg + 1] = int2{item, out.items};
+            return true;
         }
-        base += wave_sums[0] + wave_sums[1] + wave_sums[2] + wave_sums[3];
+        base += __builtin_amdgcn_readlane(sums, 63);
     }
-    __syncthreads();
-    out = Item{__builtin_amdgcn_readfirstlane(found.seg), __builtin_amdgcn_readfirstlane(found.from), __builtin_amdgcn_readfirstlane(found.end),
-               __builtin_amdgcn_readfirstlane(found.items)};
-    return out.seg != -2;
+    return false;
 }
 
 __device__ __forceinline__ unsigned pk_sub_1152(unsigned x) {
@@ -564,7 +564,25 @@ __device__ __forceinline__ halfx8 widen(unsigned a, unsigned b) {
                                             pk_sub_1152((b & 0x00ff00ffu) | 0x64006400u), pk_sub_1152(((b >> 8) & 0x00ff00ffu) | 0x64006400u)});
 }
 
-// PAGE16: pages are multiples of 16 tokens, so that a tile of 16 keys lies in one page, whose number the whole wave shares
+template <int WORDS>
+__device__ __forceinline__ void load_words(const char *from, unsigned (&to)[WORDS]) {
+    if constexpr (WORDS == 1) to[0] = *(const unsigned *) from;
+    if constexpr (WORDS == 2) {
+        const uint2 x = *(const uint2 *) from;
+        to[0] = x.x;
+        to[1] = x.y;
+    }
+    if constexpr (WORDS == 4) {
+        const uint4 x = *(const uint4 *) from;
+        to[0] = x.x;
+        to[1] = x.y;
+        to[2] = x.z;
+        to[3] = x.w;
+    }
+}
+
+// PAGE16: pages are multiples of 16 tokens and a tile of 16 keys spans less than 2 GiB, so that a tile lies in one page, whose
+// number and address the whole wave shares, and lanes differ by 32 bit offsets
 template <int WP, int NT, bool I8, bool SHAPED, bool PAGE16>
 __global__ __launch_bounds__(ROW_THREADS) void row_attention_kernel(ServingAttentionParams p, int with_prefix) {
     constexpr int ELEM = I8 ? 1 : 2;
@@ -573,18 +591,29 @@ __global__ __launch_bounds__(ROW_THREADS) void row_attention_kernel(ServingAtten
     constexpr int VW = DPL * ELEM / 4;    // 32 bit words of a value per lane
     constexpr int STEPS = WP / 32;
     constexpr int OS = WP + 4;
-    __shared__ __attribute__((aligned(16))) float os[WAVES][16 * NT][OS];
-    __shared__ float refs[WAVES][16 * NT], sums[WAVES][16 * NT];
+    __shared__ __attribute__((aligned(16))) float os[ROW_WAVES][16 * NT][OS];
+    __shared__ float refs[ROW_WAVES][16 * NT], sums[ROW_WAVES][16 * NT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
-    const int kv_head = (int) (blockIdx.x % (unsigned) p.kv_heads);
+    const int global_item = (int) (blockIdx.x / (unsigned) p.kv_heads), kv_head = (int) (blockIdx.x % (unsigned) p.kv_heads);
     Item item;
-    if (!find_item(p, with_prefix, (int) (blockIdx.x / (unsigned) p.kv_heads), item)) return;
+    if (!find_item(p, with_prefix, global_item, item)) return;
     const bool is_prefix = item.seg < 0;
-    const int b = is_prefix ? 0 : item.seg;
-    const int count = is_prefix ? p.prefix_tokens : own_length(p, b);
+    const int b = is_prefix ? 0 : item.seg, count = item.length;
     const int rows = (is_prefix ? p.batch : 1) * p.queries * (int) p.group_div.d;
     const int *table = is_prefix ? p.prefix_table : p.tables + b * p.table_stride;
+
+    int pages[2] = {0, 0};
+    auto look_up = [&](int key0) {  // the pages of a step's tiles, ahead of their loads; behind the last key: none
+        if (PAGE16)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int j = key0 + 16 * u;
+                pages[u] = j < item.end ? table[p.page_tokens.div((unsigned) j)] : -1;
+            }
+    };
+    constexpr int STRIDE = 32 * ROW_WAVES;
+    if (item.from < item.end) look_up(item.from + 32 * wave);
 
     // ---- the rows: lane i of a tile of 16 owns row 16 n + i
     halfx8 qf[NT][STEPS];
@@ -594,7 +623,7 @@ __global__ __launch_bounds__(ROW_THREADS) void row_attention_kernel(ServingAtten
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const int r = 16 * n + i;
-        const Row w = is_prefix ? row_of<PREFIX>(p, min(r, rows - 1), 0, kv_head) : row_of<OWN>(p, min(r, rows - 1), b, kv_head);
+        const Row w = is_prefix ? row_of<PREFIX>(p, min(r, rows - 1), 0, kv_head) : row_of<OWN>(p, min(r, rows - 1), b, kv_head, count);
         at[n] = w.at;
         lo[n] = w.lo;
         hi[n] = w.hi;
@@ -641,92 +670,116 @@ __global__ __launch_bounds__(ROW_THREADS) void row_attention_kernel(ServingAtten
     const bool capped = SHAPED && p.cap > 0.0f;
     const float to_cap = capped ? p.scale / p.cap : 0.0f, cap2 = p.cap * LOG2E;
     const char *kb = (const char *) p.k + kv_head * p.k_head * ELEM, *vb = (const char *) p.v + kv_head * p.v_head * ELEM;
-    const bool v_live = i * DPL < p.width;
+    const bool v_live = i * DPL < p.width, k_whole = p.width == WP;
 
     uint4 kreg[2][KP];
     unsigned vreg[8][VW];
-    float kscale[8], vscale[8];
-    unsigned gone = 0;  // keys of the lane's 8 (4 u + e: key 16 u + 4 g + e) that are not there
-
-    // K, and the scales, of the step at key0
-    auto page_of = [&](int j) { return j < count ? table[p.page_tokens.div((unsigned) j)] : -1; };
-    auto k_piece = [&](int u, long long row_at, bool there) {
+    floatx4 kscale[2], vscale[2];
 #pragma unroll
-        for (int c = 0; c < KP; c++) {
-            const int byte = 64 * c + 16 * g;
-            kreg[u][c] = there && byte < p.width * ELEM ? *(const uint4 *) (kb + row_at * ELEM + byte) : uint4{0, 0, 0, 0};
-        }
-    };
-    auto v_piece = [&](int e, long long row_at, bool there) {
-        const char *at_v = vb + row_at * ELEM + i * DPL * ELEM;
+    for (int u = 0; u < 2; u++) {
+        kscale[u] = vscale[u] = floatx4{1, 1, 1, 1};
+#pragma unroll
+        for (int c = 0; c < KP; c++) kreg[u][c] = uint4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++)
 #pragma unroll
         for (int x = 0; x < VW; x++) vreg[e][x] = 0;
-        if (there && v_live) {
-            if (VW == 1) vreg[e][0] = *(const unsigned *) at_v;
-            if (VW == 2) {
-                const uint2 x = *(const uint2 *) at_v;
-                vreg[e][0] = x.x;
-                vreg[e][VW > 1 ? 1 : 0] = x.y;
-            }
-            if (VW == 4) {
-                const uint4 x = *(const uint4 *) at_v;
-                vreg[e][0] = x.x;
-                vreg[e][VW > 1 ? 1 : 0] = x.y;
-                vreg[e][VW > 2 ? 2 : 0] = x.z;
-                vreg[e][VW > 2 ? 3 : 0] = x.w;
+    unsigned gone = 0, gone_next = 0;  // keys of the lane's 8 (4 u + e: key 16 u + 4 g + e) that are not there
+    const unsigned k_lane = PAGE16 ? (unsigned) (i * (int) p.k_token * ELEM + 16 * g) : 0;
+    const unsigned v_lane = PAGE16 ? (unsigned) ((4 * g * (int) p.v_token + i * DPL) * ELEM) : 0;
+
+    // the places of a step's tiles: page and token inside it (PAGE16)
+    int page_next[2] = {-1, -1};
+    unsigned in_next[2] = {0, 0};
+    auto place = [&](int key0) {
+        if (PAGE16) {
+            gone_next = 0;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const unsigned j = (unsigned) (key0 + 16 * u);
+                page_next[u] = __builtin_amdgcn_readfirstlane(pages[u]);
+                in_next[u] = j - p.page_tokens.div(j) * p.page_tokens.d;
+                if ((unsigned) page_next[u] >= (unsigned) p.pages) gone_next |= 15u << (4 * u);
             }
         }
     };
-    int pages[2];
-    auto look_up = [&](int key0) {
-        if (PAGE16)
-#pragma unroll
-            for (int u = 0; u < 2; u++) pages[u] = page_of(min(key0, end - 1) / 32 * 32 + 16 * u);
-    };
-    auto fetch = [&](int key0) {
-        gone = 0;
+    auto load_k = [&](int key0) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const int tile0 = key0 + 16 * u;
             if (PAGE16) {
-                const int page = __builtin_amdgcn_readfirstlane(pages[u]);
-                const bool there = (unsigned) page < (unsigned) p.pages;
-                const unsigned in = (unsigned) tile0 - p.page_tokens.div((unsigned) tile0) * p.page_tokens.d;
-                const long long k0 = page * p.k_page + in * p.k_token, v0 = page * p.v_page + in * p.v_token;
-                const long long s0 = ((long long) page * p.kv_heads + kv_head) * p.page_tokens.d + in + 4 * g;
-                k_piece(u, k0 + i * p.k_token, there);
-                if (!there) gone |= 15u << (4 * u);
+                if ((gone_next >> (4 * u)) & 1) continue;
+                const char *base = kb + (page_next[u] * p.k_page + in_next[u] * p.k_token) * ELEM;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    v_piece(4 * u + e, v0 + (4 * g + e) * p.v_token, there && tile0 + 4 * g + e < count);
-                    kscale[4 * u + e] = I8 && there ? p.k_scales[s0 + e] : 1.0f;
-                    vscale[4 * u + e] = I8 && there ? p.v_scales[s0 + e] : 1.0f;
-                }
+                for (int c = 0; c < KP; c++)
+                    if (k_whole || 64 * c + 16 * g < p.width * ELEM) kreg[u][c] = *(const uint4 *) (base + (k_lane + 64 * c));
             } else {
-                const int j = tile0 + i, page = page_of(j);
-                const unsigned in = (unsigned) j - p.page_tokens.div((unsigned) j) * p.page_tokens.d;
-                k_piece(u, page * p.k_page + in * p.k_token, (unsigned) page < (unsigned) p.pages);
+                const int j = key0 + 16 * u + i, pg = j < count ? table[p.page_tokens.div((unsigned) j)] : -1;
+                const unsigned at_j = (unsigned) j - p.page_tokens.div((unsigned) j) * p.page_tokens.d;
+                const char *base = kb + (pg * p.k_page + at_j * p.k_token) * ELEM;
+                if ((unsigned) pg < (unsigned) p.pages)
+#pragma unroll
+                    for (int c = 0; c < KP; c++)
+                        if (64 * c + 16 * g < p.width * ELEM) kreg[u][c] = *(const uint4 *) (base + 64 * c + 16 * g);
+            }
+        }
+    };
+    auto load_scales = [&](int key0) {
+        if (!I8) return;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            if (PAGE16) {
+                if ((gone_next >> (4 * u)) & 1) continue;
+                const long long s = ((long long) page_next[u] * p.kv_heads + kv_head) * p.page_tokens.d + in_next[u];
+                kscale[u] = *(const floatx4_any *) ((const char *) (p.k_scales + s) + (unsigned) (16 * g));
+                vscale[u] = *(const floatx4_any *) ((const char *) (p.v_scales + s) + (unsigned) (16 * g));
+            }
+        }
+    };
+    auto load_v = [&](int key0) {
+        if (!PAGE16) gone_next = 0;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            if (PAGE16) {
+                if ((gone_next >> (4 * u)) & 1) continue;
+                const char *base = vb + (page_next[u] * p.v_page + in_next[u] * p.v_token) * ELEM;
+                if (v_live)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) load_words(base + (long long) e * p.v_token * ELEM + v_lane, vreg[4 * u + e]);
+            } else {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const int jv = tile0 + 4 * g + e, page_v = page_of(jv);
-                    const bool there = (unsigned) page_v < (unsigned) p.pages;
-                    const unsigned in_v = (unsigned) jv - p.page_tokens.div((unsigned) jv) * p.page_tokens.d;
-                    const long long s = ((long long) page_v * p.kv_heads + kv_head) * p.page_tokens.d + in_v;
-                    v_piece(4 * u + e, page_v * p.v_page + in_v * p.v_token, there);
-                    if (!there) gone |= 1u << (4 * u + e);
-                    kscale[4 * u + e] = I8 && there ? p.k_scales[s] : 1.0f;
-                    vscale[4 * u + e] = I8 && there ? p.v_scales[s] : 1.0f;
+                    const int j = key0 + 16 * u + 4 * g + e, pg = j < count ? table[p.page_tokens.div((unsigned) j)] : -1;
+                    const unsigned at_j = (unsigned) j - p.page_tokens.div((unsigned) j) * p.page_tokens.d;
+                    if ((unsigned) pg < (unsigned) p.pages) {
+                        if (v_live) load_words(vb + (pg * p.v_page + at_j * p.v_token + i * DPL) * ELEM, vreg[4 * u + e]);
+                        if (I8) {
+                            const long long s = ((long long) pg * p.kv_heads + kv_head) * p.page_tokens.d + at_j;
+                            kscale[u][e] = p.k_scales[s];
+                            vscale[u][e] = p.v_scales[s];
+                        }
+                    } else {
+                        gone_next |= 1u << (4 * u + e);
+                    }
                 }
             }
         }
     };
 
     int key0 = from + 32 * wave;
-    constexpr int STRIDE = 32 * WAVES;
-    if (key0 < end) look_up(key0);
-    while (key0 < end) {
-        fetch(key0);
+    if (key0 < end) {
+        if (from != item.from) look_up(key0);
+        place(key0);
+        load_k(key0);
+        load_scales(key0);
+        load_v(key0);
         look_up(key0 + STRIDE);
+    }
+    while (key0 < end) {
+        gone = gone_next;
+        const int next = key0 + STRIDE;
+        const bool more = next < end;
+        if (more) place(next);
         const bool masked = key0 < whole_from || key0 + 32 > min(whole_end, end) || __any(gone != 0);
         floatx4 st[NT][2];
 #pragma unroll
@@ -748,12 +801,13 @@ __global__ __launch_bounds__(ROW_THREADS) void row_attention_kernel(ServingAtten
                 for (int s = 0; s < STEPS; s++) st[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[s], qf[n][s], st[n][u], 0, 0, 0);
             }
         }
+        if (more) load_k(next);
         float value_log[8];
         if (I8)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                vscale[e] = fmaxf(vscale[e], 0x1p-40f);  // (values below 2^-33 are zeros of an f16 result)
-                value_log[e] = __builtin_amdgcn_logf(vscale[e]);
+                vscale[e / 4][e % 4] = fmaxf(vscale[e / 4][e % 4], 0x1p-40f);  // (values below 2^-33 are zeros of an f16 result)
+                value_log[e] = __builtin_amdgcn_logf(vscale[e / 4][e % 4]);
             }
         halfx8 weights[NT];
 #pragma unroll
@@ -763,7 +817,7 @@ __global__ __launch_bounds__(ROW_THREADS) void row_attention_kernel(ServingAtten
             for (int e = 0; e < 8; e++) {
                 const int key = key0 + 16 * (e / 4) + 4 * g + e % 4;
                 float x = st[n][e / 4][e % 4];
-                if (I8) x *= kscale[e];
+                if (I8) x *= kscale[e / 4][e % 4];
                 if (SHAPED) {
                     x = capped ? cap2 * tanh_fast(x * to_cap) : x * scale2;
                     x = __builtin_fmaf(-slope2[n], fabsf((float) (at[n] - key)), x);
@@ -789,16 +843,21 @@ __global__ __launch_bounds__(ROW_THREADS) void row_attention_kernel(ServingAtten
             for (int e = 0; e < 8; e++) {
                 const float x = __builtin_amdgcn_exp2f(s2[e] - minus);
                 sum[n] += x;
-                weights[n][e] = (half_t) (I8 ? x * vscale[e] : x);
+                weights[n][e] = (half_t) (I8 ? x * vscale[e / 4][e % 4] : x);
             }
         }
+        if (more && PAGE16) load_scales(next);
         unsigned bad = 0;  // keys of the lane's 8 whose values hold an infinity or NaN, where not every row sees every key
         if (!I8 && masked) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
+                const bool there = key0 + 16 * (e / 4) + 4 * g + e % 4 < count && !((gone >> e) & 1);
                 bool any = false;
 #pragma unroll
-                for (int x = 0; x < VW; x++) any |= (vreg[e][x] & 0x7c00u) == 0x7c00u || (vreg[e][x] & 0x7c000000u) == 0x7c000000u;
+                for (int x = 0; x < VW; x++) {
+                    if (!there) vreg[e][x] = 0;
+                    any |= (vreg[e][x] & 0x7c00u) == 0x7c00u || (vreg[e][x] & 0x7c000000u) == 0x7c000000u;
+                }
                 // (of the 16 lanes of a group)
                 if ((__ballot(any) >> (16 * g)) & 0xffffu) bad |= 1u << e;
             }
@@ -817,38 +876,41 @@ __global__ __launch_bounds__(ROW_THREADS) void row_attention_kernel(ServingAtten
                 }
             }
             const halfx8 a = __builtin_bit_cast(halfx8, uint4{pair[0], pair[1], pair[2], pair[3]});
-            if (!any_bad) {
+            const halfx8 good = any_bad ? finite_or_zero(a) : a;
 #pragma unroll
-                for (int n = 0; n < NT; n++) oacc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, weights[n], oacc[n][d], 0, 0, 0);
-            } else {
-                // (as in the kernel above: a key of its own product, for the queries that see it)
-                halfx8 good = a;
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if ((bad >> e) & 1) good[e] = (half_t) 0.0f;
-#pragma unroll
-                for (int n = 0; n < NT; n++) oacc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(good, weights[n], oacc[n][d], 0, 0, 0);
+            for (int n = 0; n < NT; n++) oacc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(good, weights[n], oacc[n][d], 0, 0, 0);
+        }
+        if (any_bad) {
+            // (as in the kernel above: what is not finite is added for the queries that see its key)
 #pragma unroll 1
-                for (int key = 0; key < 32; key++) {
-                    const int of_group = (key % 16) / 4, e_of = 4 * (key / 16) + key % 4;
-                    if (__any(g == of_group && ((bad >> e_of) & 1)) == 0) continue;
-                    halfx8 one;
+            for (int key = 0; key < 32; key++) {
+                const int group = (key % 16) / 4, nth = 4 * (key / 16) + key % 4;
+                if (!__any(g == group && ((bad >> nth) & 1))) continue;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) one[e] = g == of_group && e == e_of ? a[e] : (half_t) 0.0f;
+                for (int d = 0; d < DPL; d++)
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        const floatx4 its = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, weights[n], floatx4{0, 0, 0, 0}, 0, 0, 0);
-                        const bool seen = (unsigned) (key0 + key - lo[n]) < (unsigned) (hi[n] - lo[n]);
+                    for (int v = 0; v < 4; v++) {
+                        // register v of product d: dim (4 g + v) DPL + d, which lane (4 g + v, group) holds
+                        unsigned word = 0;
 #pragma unroll
-                        for (int v = 0; v < 4; v++) oacc[n][d][v] += seen ? its[v] : 0.0f;
+                        for (int e = 0; e < 8; e++)
+                            if (e == nth) word = vreg[e][I8 ? 0 : d / 2];
+                        const unsigned got = __shfl(word, 16 * group + 4 * g + v);
+                        const float x = (float) __builtin_bit_cast(half_t, (unsigned short) (d % 2 ? got >> 16 : got));
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+                            if ((unsigned) (key0 + key - lo[n]) < (unsigned) (hi[n] - lo[n])) oacc[n][d][v] += x - x == 0.0f ? 0.0f : x;
                     }
-                }
             }
         }
-        key0 += STRIDE;
+        if (more) {
+            load_v(next);
+            look_up(next + STRIDE);
+        }
+        key0 = next;
     }
 
-    // ---- the four waves' parts into one
+    // ---- the waves' parts into one
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         sum[n] += __shfl_xor(sum[n], 16);
@@ -870,23 +932,23 @@ __global__ __launch_bounds__(ROW_THREADS) void row_attention_kernel(ServingAtten
         const int r = e / (WP / 4), d = 4 * (e % (WP / 4));
         float top = -INFINITY, total = 0.0f;
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) top = fmaxf(top, refs[w][r]);
+        for (int w = 0; w < ROW_WAVES; w++) top = fmaxf(top, refs[w][r]);
         floatx4 x = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) {
+        for (int w = 0; w < ROW_WAVES; w++) {
             const float weight = __builtin_amdgcn_exp2f(refs[w][r] - (top == -INFINITY ? 0.0f : top));
             total += weight * sums[w][r];
             x += weight * *(const floatx4 *) &os[w][r][d];
         }
         if (direct) {
             const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
-            const Row w = row_of<OWN>(p, r, b, kv_head);
+            const Row w = row_of<OWN>(p, r, b, kv_head, count);
             if (d < p.width)
                 *(halfx4_any *) ((half_t *) p.out + (w.b * p.o_batch + w.t * p.o_token + w.head * p.o_head + d)) =
                     halfx4{(half_t) (x[0] * inv), (half_t) (x[1] * inv), (half_t) (x[2] * inv), (half_t) (x[3] * inv)};
         } else {
             const long long part = is_prefix ? p.row_prefix_part : p.row_own_part;
-            const long long at_part = part + ((long long) ((int) (blockIdx.x / (unsigned) p.kv_heads)) * p.kv_heads + kv_head) * rows + r;
+            const long long at_part = part + ((long long) global_item * p.kv_heads + kv_head) * rows + r;
             *(floatx4 *) (p.part_values + at_part * WP + d) = x;
             if (d == 0) *(float2 *) (p.part_stats + 2 * at_part) = float2{top, total};
         }
@@ -1039,7 +1101,7 @@ int launch_tiles_for(const ServingAttentionParams &p, int stretch, unsigned work
 
 template <int WP, int NT, bool I8>
 int launch_rows(const ServingAttentionParams &p, unsigned workgroups, int with_prefix, hipStream_t stream) {
-    const bool shaped = p.cap > 0.0f || p.slopes, page16 = p.page_tokens.d % 16 == 0;
+    const bool shaped = p.cap > 0.0f || p.slopes, page16 = p.page_tokens.d % 16 == 0 && p.k_token <= 1 << 25;
     const dim3 grid(workgroups), block(ROW_THREADS);
     if (shaped && page16) hipLaunchKernelGGL((row_attention_kernel<WP, NT, I8, true, true>), grid, block, 0, stream, p, with_prefix);
     else if (shaped) hipLaunchKernelGGL((row_attention_kernel<WP, NT, I8, true, false>), grid, block, 0, stream, p, with_prefix);

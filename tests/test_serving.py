@@ -167,6 +167,11 @@ def _cached_case(device, c, seed=0):
     fill(slots(prefix_table, P))
     for b, n in enumerate(lengths):
         fill(slots(tables[b], min(max(n, 0), table_pages * page)))
+    poisoned = c.get("poison", False)  # the last token of every sequence: only its own query sees it
+    if poisoned:
+        for b, n in enumerate(lengths):
+            if n > 0:
+                cache.put(slots(tables[b], n)[-1:], np.full((1, N, W), np.nan, np.float16), np.full((1, N, W), -np.inf, np.float16))
     lost = c.get("lost", ())  # (sequence or -1 for the prefix, page of its table): not there
     gone = {}
     for b, i in lost:
@@ -204,6 +209,8 @@ def _cached_case(device, c, seed=0):
             k, v = np.concatenate([kp, ko]), np.concatenate([vp, vo])
             at = P + n - T + np.arange(T)
             places = np.arange(P + n)
+            if poisoned and n > 0:
+                k[-1], v[-1] = 0, 0
             visible = (places <= at[:, None]) & (at[:, None] >= P) & there
             if window:
                 visible &= places > at[:, None] - window
@@ -217,7 +224,7 @@ def _cached_case(device, c, seed=0):
                 bound[b, h] = e
         return out, bound
 
-    return dict(args=args, dev=dev, cache=cache, out_mem=out_mem, expected=expected, W=W)
+    return dict(args=args, dev=dev, cache=cache, out_mem=out_mem, expected=expected, W=W, compared=T - 1 if poisoned else T)
 
 
 CACHED_CASES = {
@@ -249,6 +256,13 @@ CACHED_CASES = {
     "negative_scale": dict(dtype=DType.I8, kv=1, group=1, width=64, page=16, lengths=[90], scale=-0.2),
     "peaked": dict(dtype=DType.F16, kv=1, group=4, width=128, page=16, lengths=[600, 50], size=30.0),
     "narrow": dict(dtype=DType.I8, kv=2, group=2, width=16, page=16, lengths=[70, 5]),
+    "newest_is_not_finite": dict(dtype=DType.F16, kv=2, group=4, width=128, page=16, lengths=[40, 7, 33, 0, 700], queries=3, poison=True),
+    "newest_is_not_finite_odd_pages": dict(dtype=DType.F16, kv=1, group=3, width=64, page=5, lengths=[40, 300], queries=7, poison=True, prefix=20),
+    "newest_is_not_finite_tiles": dict(dtype=DType.F16, kv=1, group=4, width=64, page=16, lengths=[100, 50, 290], queries=50, poison=True),
+    "long_windows": dict(dtype=DType.I8, kv=1, group=2, width=64, page=16, lengths=[3, 100, 0], queries=5, window=(1 << 31) - 1, prefix=40),
+    "many_sequences": dict(dtype=DType.I8, kv=1, group=2, width=64, page=16, lengths=[(13 * i) % 70 for i in range(150)]),
+    "long_and_short": dict(dtype=DType.I8, kv=1, group=2, width=64, page=16, lengths=[9000, 5, 0, 2500]),
+    "long_f16_wide_rows": dict(dtype=DType.F16, kv=1, group=4, width=128, page=16, lengths=[5000, 40], queries=8),
     "many_heads_of_one": dict(dtype=DType.I8, kv=1, group=71, width=64, page=16, lengths=[300, 4]),
 }
 
@@ -272,7 +286,8 @@ def test_cached_attention(name, hip_device):
     for round_ in range(2):  # on the same workspace
         kn.cached_attention(hip_device, stream, c["args"], workspace)
         stream.synchronize()
-        _check(c["dev"][1].to_array(np.float16, c["out_mem"].shape), out, bound, c["W"], f"{name}, call {round_}")
+        got, n = c["dev"][1].to_array(np.float16, c["out_mem"].shape), c["compared"]
+        _check(got[:, :, :n], out[:, :, :n], bound[:, :, :n], c["W"], f"{name}, call {round_}")
 
 
 # ---- attention of prompts ------------------------------------------------------------------------------------------
@@ -301,6 +316,7 @@ PROMPT_CASES = {
     "bias_both_sides": dict(queries=150, heads=2, kv=2, width=64, slopes=True),
     "window": dict(queries=400, heads=2, kv=1, width=128, causal=True, window=37),
     "window_of_one": dict(queries=130, heads=1, kv=1, width=64, causal=True, window=1),
+    "longest_window": dict(queries=50, keys=20, heads=1, kv=1, width=64, window=(1 << 31) - 1),
     "window_not_causal": dict(queries=200, heads=1, kv=1, width=64, window=20),
     "documents": dict(batch=2, queries=500, heads=2, kv=2, width=128, causal=True, spans=[[3, 130, 131, 300], [64, 128, 448]]),
     "documents_not_causal": dict(queries=300, heads=2, kv=1, width=64, spans=[[100, 164]]),
