@@ -7,7 +7,7 @@
 //
 // The rows of a product are the queries that read the same head of keys: all heads of its group times all tokens, so
 // that a block of keys is fetched once for them. Three kernels:
-//   tile_attention_kernel   128 rows per workgroup: prompts, prompts over a cache, and the shared prefix of a batch, whose
+//   tile_attention_kernel   32 rows per wave, 128 or 256 per workgroup: prompts, prompts over a cache, and the shared prefix of a batch, whose
 //                           rows are the queries of ALL sequences
 //   row_attention_kernel    up to 16 or 32 rows per workgroup: the few queries of one sequence over its own keys
 //   join_attention_kernel   the softmax of parts: keys are split between workgroups where rows are few, and a sequence with
@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "../serving_kernels.h"
 
@@ -113,15 +114,31 @@ __device__ __forceinline__ halfx8 finite_or_zero(halfx8 x) {
     return x;
 }
 
-// ---- 128 rows per workgroup ----------------------------------------------------------------------------------------
+// four words of two whole numbers plus 1152 each -> f16
+__device__ __forceinline__ unsigned pk_sub_1152(unsigned x) {
+    const halfx2 bias = {(half_t) -1152.0f, (half_t) -1152.0f};
+    return __builtin_bit_cast(unsigned, __builtin_bit_cast(halfx2, x) + bias);
+}
 
-// Four waves of 32 rows each walk all blocks of 64 keys, which they stage together in one of two LDS buffers, one barrier
-// per block: the block after the current one is in flight in registers meanwhile. WP: the width, padded to 64 or 128 with
-// zeros. I8: keys and values are dequantised (f32 product, one rounding to f16) as they are staged. SHAPED: with cap or
-// distance bias.
-template <int WP, int STRETCH, bool I8, bool SHAPED>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_attention_kernel(ServingAttentionParams p) {
-    constexpr int BKEYS = 64, THREADS = 64 * WAVES;
+// 8 whole numbers of 8 bits as f16, in the order 0 2 1 3 4 6 5 7, without a conversion instruction: q + 128 in the low byte
+// of 0x6400 is 1152 + q, the subtraction is exact
+__device__ __forceinline__ halfx8 widen(unsigned a, unsigned b) {
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    return __builtin_bit_cast(halfx8, uint4{pk_sub_1152((a & 0x00ff00ffu) | 0x64006400u), pk_sub_1152(((a >> 8) & 0x00ff00ffu) | 0x64006400u),
+                                            pk_sub_1152((b & 0x00ff00ffu) | 0x64006400u), pk_sub_1152(((b >> 8) & 0x00ff00ffu) | 0x64006400u)});
+}
+
+// ---- 32 rows per wave, 4 or 8 waves per workgroup ------------------------------------------------------------------
+
+// The waves walk all blocks of 64 keys, which they stage together in one of two LDS buffers, one barrier per block: the
+// block after the current one is in flight in registers meanwhile. WP: the width, padded to 64 or 128 with zeros. SHAPED: with
+// cap or distance bias. I8: keys and values are staged as the whole numbers they are, exact in f16; the scale of a key is
+// applied to its scores, that of a value to its weights, both in f32. The scaled weights keep inside f16 by a power of two
+// that the waves of a workgroup share: it starts from the first block and grows when a scale passes it by 2^6.
+template <int WP, int STRETCH, bool I8, bool SHAPED, int TW>
+__global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_attention_kernel(ServingAttentionParams p) {
+    constexpr int BKEYS = 64, THREADS = 64 * TW;
     constexpr int PIECE = I8 ? 16 : 8;        // elements per 128 bit load
     constexpr int C = WP / PIECE;             // loads per row
     constexpr int VECS = BKEYS * C / THREADS;  // of K and of V, per lane and block
@@ -129,11 +146,14 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     constexpr int STAGE = BKEYS * (KS + VS);
     constexpr int OS = WP + 8, WAVE_ROWS = 32 * OS;
     constexpr int DT = WP / 32, QC = WP / 8;
-    static_assert(2 * STAGE >= WAVES * WAVE_ROWS && VECS >= 1, "unsupported shape");
     constexpr bool PAGED = STRETCH != PROMPT;
-    __shared__ __attribute__((aligned(16))) half_t lds[2 * STAGE];
-    __shared__ unsigned long long gone_s[2][WAVES], bad_s[2][WAVES];
-    __shared__ int range_s[WAVES][4];
+    constexpr int LDS_HALVES = 2 * STAGE > TW * WAVE_ROWS ? 2 * STAGE : TW * WAVE_ROWS;
+    static_assert(WP != 128 || VECS >= 1, "unsupported shape");
+    __shared__ __attribute__((aligned(16))) half_t lds[LDS_HALVES];
+    __shared__ __attribute__((aligned(16))) float kscale_s[2][BKEYS], vscale_s[2][BKEYS];
+    __shared__ unsigned long long gone_s[2][TW], bad_s[2][TW];
+    __shared__ int big_s[2][TW];
+    __shared__ int range_s[TW][4];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 31, h = lane >> 5;
@@ -145,11 +165,11 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     const unsigned rows = (unsigned) (STRETCH == PREFIX ? p.batch : 1) * p.queries * p.group_div.d;
     const int split = blockIdx.y, splits = gridDim.y;
 
-    const unsigned first_row = (unsigned) tile * 128 + wave * 32;
+    const unsigned first_row = (unsigned) tile * (32 * TW) + wave * 32;
     const unsigned row = first_row + c, row_c = min(row, rows - 1);
     const Row w = row_of<STRETCH>(p, row_c, b, kv_head);
 
-    // ---- the blocks that any of the 128 rows needs, and those that all of them see whole
+    // ---- the blocks that any of the rows needs, and those that all of them see whole
     int from, end, whole_from, whole_end;
     {
         const bool sees = w.hi > w.lo;
@@ -163,13 +183,18 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
             for (int i = 0; i < 4; i++) range_s[wave][i] = a[i];
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; i++) a[i] = __builtin_amdgcn_readfirstlane(min(min(range_s[0][i], range_s[1][i]), min(range_s[2][i], range_s[3][i])));
+        for (int i = 0; i < 4; i++) {
+            int m = range_s[0][i];
+#pragma unroll
+            for (int j = 1; j < TW; j++) m = min(m, range_s[j][i]);
+            a[i] = __builtin_amdgcn_readfirstlane(m);
+        }
         from = a[0];
         end = -a[1];
         whole_from = -a[2];
         whole_end = a[3];
     }
-    const int count = STRETCH == PROMPT ? p.keys : STRETCH == OWN ? own_length(p, b) : p.prefix_tokens;
+    const int count = __builtin_amdgcn_readfirstlane(STRETCH == PROMPT ? p.keys : STRETCH == OWN ? own_length(p, b) : p.prefix_tokens);
     int first_block = from < end ? from / BKEYS : 0, end_block = from < end ? (end + BKEYS - 1) / BKEYS : 0;
     if (splits > 1) {  // this workgroup's share of the blocks
         const int each = (end_block - first_block + splits - 1) / splits;
@@ -191,10 +216,13 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     const int stage_row = (int) threadIdx.x / C, part = (int) threadIdx.x % C;
     constexpr int ROW_STEP = THREADS / C;  // rows between a lane's loads
     const bool part_live = part * PIECE < p.width;
+    const long long k_lane = stage_row * p.k_token * ELEM + 16 * part, v_lane = stage_row * p.v_token * ELEM + 16 * part;  // prompts
     uint4 kreg[VECS], vreg[VECS];
     float kscale[VECS], vscale[VECS];
     int pages[VECS];
     unsigned gone = 0;  // of the block in the registers: the lane's rows that are not there
+#pragma unroll
+    for (int i = 0; i < VECS; i++) kreg[i] = vreg[i] = uint4{0, 0, 0, 0};  // (what a row has behind the width stays zero)
     auto look_up = [&](int block) {  // the page numbers of a block, ahead of its loads
         if (!PAGED) return;
 #pragma unroll
@@ -205,6 +233,16 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     };
     auto fetch = [&](int block) {
         gone = 0;
+        if (!PAGED && (block + 1) * BKEYS <= count) {
+            if (part_live)
+#pragma unroll
+                for (int i = 0; i < VECS; i++) {
+                    const long long r = block * BKEYS + ROW_STEP * i;
+                    kreg[i] = __builtin_bit_cast(uint4, *(const halfx8_any *) (kb + r * p.k_token * ELEM + k_lane));
+                    vreg[i] = __builtin_bit_cast(uint4, *(const halfx8_any *) (vb + r * p.v_token * ELEM + v_lane));
+                }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < VECS; i++) {
             const int j = block * BKEYS + stage_row + ROW_STEP * i;
@@ -219,10 +257,11 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
                 k_at = j * p.k_token;
                 v_at = j * p.v_token;
             }
-            if (!there) gone |= 1u << i;
-            kreg[i] = vreg[i] = uint4{0, 0, 0, 0};
-            kscale[i] = vscale[i] = 0.0f;
-            if (there && part_live) {
+            if (!there) {
+                gone |= 1u << i;
+                kreg[i] = vreg[i] = uint4{0, 0, 0, 0};
+                kscale[i] = vscale[i] = 0.0f;
+            } else if (part_live) {
                 if (I8) {
                     kreg[i] = *(const uint4 *) (kb + k_at + 16 * part);
                     vreg[i] = *(const uint4 *) (vb + v_at + 16 * part);
@@ -235,27 +274,28 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
             }
         }
     };
-    // 16 whole numbers times their scale
-    auto dequantise = [&](uint4 x, float scale, halfx8 (&out)[2]) {
-        const unsigned u[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) out[i / 2][4 * (i % 2) + e] = (half_t) ((float) (signed char) (u[i] >> (8 * e)) * scale);
-    };
+    // A scale of zero or less goes into Q (times -1, 0 or 1), so that the scores are multiplied by a positive number
+    const float sign = p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f;
+    const float scale2 = p.scale == 0.0f ? 1.0f : fabsf(p.scale) * LOG2E;
+    const bool capped = SHAPED && p.cap > 0.0f;
+    const float to_cap = capped ? scale2 / (LOG2E * p.cap) : 0.0f, cap2 = p.cap * LOG2E;
+    float value_unit = 0x1p60f;  // I8: what the scales of values are multiplied by, a power of two
     auto stage = [&](int buffer, bool masked) {
         half_t *ks = lds + buffer * STAGE, *vs = ks + BKEYS * KS;
+        bool big = false;
 #pragma unroll
         for (int i = 0; i < VECS; i++) {
             const int r = stage_row + ROW_STEP * i;
             if (I8) {
-                halfx8 two[2];
-                dequantise(kreg[i], kscale[i], two);
-                *(halfx8 *) &ks[r * KS + 16 * part] = two[0];
-                *(halfx8 *) &ks[r * KS + 16 * part + 8] = two[1];
-                dequantise(vreg[i], vscale[i], two);
-                *(halfx8 *) &vs[r * VS + 16 * part] = two[0];
-                *(halfx8 *) &vs[r * VS + 16 * part + 8] = two[1];
+                *(halfx8 *) &ks[r * KS + 16 * part] = widen(kreg[i].x, kreg[i].y);
+                *(halfx8 *) &ks[r * KS + 16 * part + 8] = widen(kreg[i].z, kreg[i].w);
+                *(halfx8 *) &vs[r * VS + 16 * part] = widen(vreg[i].x, vreg[i].y);
+                *(halfx8 *) &vs[r * VS + 16 * part + 8] = widen(vreg[i].z, vreg[i].w);
+                if (part == 0) {
+                    kscale_s[buffer][r] = kscale[i] * (capped ? to_cap : scale2);
+                    vscale_s[buffer][r] = vscale[i] * value_unit;
+                    big |= vscale[i] * value_unit > 64.0f;
+                }
             } else {
                 *(uint4 *) &ks[r * KS + 8 * part] = kreg[i];
                 *(uint4 *) &vs[r * VS + 8 * part] = vreg[i];
@@ -268,19 +308,21 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
             for (int i = 0; i < VECS; i++) {
                 unsigned long long bad = 0;
                 if (masked && !I8) bad = __ballot(not_finite(__builtin_bit_cast(halfx8, vreg[i])));
-                const unsigned long long missing = PAGED ? __ballot((gone >> i) & 1) : 0;
+                const unsigned long long missing = __ballot((gone >> i) & 1);
                 if (bad | missing)
 #pragma unroll
                     for (int g = 0; g < 64 / C; g++) {  // rows of this wave's i-th load
                         const int r = wave * (64 / C) + g + ROW_STEP * i;
-                        const unsigned long long lanes = (C == 64 ? ~0ull : (1ull << C) - 1) << (g * C);
+                        const unsigned long long lanes = ((1ull << C) - 1) << (g * C);
                         if (bad & lanes) bad_rows |= 1ull << r;
                         if (missing & lanes) gone_rows |= 1ull << r;
                     }
             }
+            const int any_big = I8 ? __any(big) : 0;
             if (lane == 0) {
                 gone_s[buffer][wave] = gone_rows;
                 bad_s[buffer][wave] = bad_rows;
+                if (I8) big_s[buffer][wave] = any_big;
             }
         }
     };
@@ -292,7 +334,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
     }
 
     // ---- Q: the wave's 32 rows, whole lines at a time, through the wave's part of LDS; lane (query c, half h) holds elements
-    // 16 t + 8 h .. + 7 for step t
+    // 16 t + 8 h .. + 7 for step t, in the order of the staged keys
     halfx8 qf[WP / 16];
     {
         half_t *qs = lds + wave * WAVE_ROWS;
@@ -302,8 +344,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
             const Row o = row_of<STRETCH>(p, min(first_row + r, rows - 1), b, kv_head);
             halfx8 x = {0, 0, 0, 0, 0, 0, 0, 0};
             if (first_row + r < rows && d < p.width)
-                x = *(const halfx8_any *) ((const half_t *) p.q + (o.b * p.q_batch + o.t * p.q_token + o.head * p.q_head + d));
-            *(halfx8 *) &qs[r * OS + d] = x;
+                x = *(const halfx8_any *) ((const half_t *) p.q + (o.b * p.q_batch + o.t * p.q_token + o.head * p.q_head + d)) * (half_t) sign;
+            *(halfx8 *) &qs[r * OS + d] = I8 ? halfx8{x[0], x[2], x[1], x[3], x[4], x[6], x[5], x[7]} : x;
         }
         __syncthreads();
 #pragma unroll
@@ -317,10 +359,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
         for (int v = 0; v < 16; v++) oacc[t][v] = 0.0f;
     float ref = -INFINITY, sum = 0.0f;  // sum: this half's share of the keys
-    const float scale2 = p.scale * LOG2E, slope2 = SHAPED && p.slopes ? p.slopes[w.head] * LOG2E : 0.0f;
-    const bool capped = SHAPED && p.cap > 0.0f;
-    const float to_cap = capped ? p.scale / p.cap : 0.0f, cap2 = p.cap * LOG2E;
+    const float slope2 = SHAPED && p.slopes ? p.slopes[w.head] * LOG2E : 0.0f;
     const int v_corner = BKEYS * KS + (4 * h + (lane & 15) / 4) * VS + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    constexpr bool LOG2_UNITS = SHAPED || I8;  // the scores have their factor before the exponential
 
     for (int block = first_block; block < end_block; block++) {
         const int buffer = block & 1, key0 = block * BKEYS;
@@ -331,18 +372,59 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
             look_up(min(block + 2, end_block - 1));
         }
         __syncthreads();
-        unsigned long long gone_rows = 0, bad_rows = 0;
-        if (PAGED || masked)
+        half_t *ks = lds + buffer * STAGE;
+        unsigned long long gone_rows = 0;
+        if (PAGED || masked) {
+            unsigned long long bad_rows = 0;
+            int big = 0;
 #pragma unroll
-            for (int i = 0; i < WAVES; i++) {
+            for (int i = 0; i < TW; i++) {
                 gone_rows |= gone_s[buffer][i];
-                bad_rows |= bad_s[buffer][i];
+                if (!I8) bad_rows |= bad_s[buffer][i];
+                if (I8) big |= big_s[buffer][i];
             }
-        gone_rows = ((unsigned long long) __builtin_amdgcn_readfirstlane((unsigned) (gone_rows >> 32)) << 32) | (unsigned) __builtin_amdgcn_readfirstlane((unsigned) gone_rows);
-        bad_rows = ((unsigned long long) __builtin_amdgcn_readfirstlane((unsigned) (bad_rows >> 32)) << 32) | (unsigned) __builtin_amdgcn_readfirstlane((unsigned) bad_rows);
-        masked |= gone_rows != 0;
+            gone_rows = ((unsigned long long) __builtin_amdgcn_readfirstlane((unsigned) (gone_rows >> 32)) << 32) | (unsigned) __builtin_amdgcn_readfirstlane((unsigned) gone_rows);
+            masked |= gone_rows != 0;
+            if (I8 && __builtin_amdgcn_readfirstlane(big)) {  // (the same for all waves, which take the barriers together)
+                float most = vscale_s[buffer][lane];
+#pragma unroll
+                for (int m = 1; m < 64; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
+                const float unit = __builtin_ldexpf(1.0f, -__builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(most)));
+                value_unit *= unit;
+#pragma unroll
+                for (int t = 0; t < DT; t++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) oacc[t][v] *= unit;
+                __syncthreads();
+                if (threadIdx.x < BKEYS) vscale_s[buffer][threadIdx.x] *= unit;
+                __syncthreads();
+            }
+            bad_rows = ((unsigned long long) __builtin_amdgcn_readfirstlane((unsigned) (bad_rows >> 32)) << 32) | (unsigned) __builtin_amdgcn_readfirstlane((unsigned) bad_rows);
+            if (!I8 && bad_rows != 0) {
+                // Infinities or NaN among the values of a block that not every row sees whole: a weight of zero does not remove
+                // them from a product, so they are added here for the queries that see their key, and then taken out.
+                for (unsigned long long left = bad_rows; left; left &= left - 1) {
+                    const int key = __builtin_ctzll(left);
+                    if ((unsigned) (key0 + key - w.lo) < (unsigned) (w.hi - w.lo))
+#pragma unroll
+                        for (int t = 0; t < DT; t++)
+#pragma unroll
+                            for (int a = 0; a < 4; a++) {
+                                const halfx4 x = *(const halfx4 *) &ks[BKEYS * KS + key * VS + 32 * t + 8 * a + 4 * h];
+#pragma unroll
+                                for (int u = 0; u < 4; u++) oacc[t][4 * a + u] += (float) x[u] - (float) x[u] == 0.0f ? 0.0f : (float) x[u];
+                            }
+                }
+                __syncthreads();
+                for (int e = threadIdx.x; e < BKEYS * QC; e += THREADS) {
+                    const int r = e / QC;
+                    halfx8 *x = (halfx8 *) &ks[BKEYS * KS + r * VS + 8 * (e % QC)];
+                    if ((bad_rows >> r) & 1) *x = finite_or_zero(*x);
+                }
+                __syncthreads();
+            }
+        }
 
-        const half_t *ks = lds + buffer * STAGE;
         floatx16 st[2];
 #pragma unroll
         for (int u = 0; u < 2; u++)
@@ -359,28 +441,35 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
         float top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
+            if (I8)
+#pragma unroll
+                for (int a = 0; a < 4; a++) {
+                    const floatx4 f = *(const floatx4 *) &kscale_s[buffer][32 * u + 8 * a + 4 * h];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) st[u][4 * a + e] *= f[e];
+                }
             if (SHAPED) {
                 const float away = (float) (w.at - (key0 + 32 * u + 4 * h));
 #pragma unroll
                 for (int v = 0; v < 16; v++) {
-                    const float x = capped ? cap2 * tanh_fast(st[u][v] * to_cap) : st[u][v] * scale2;
+                    float x = st[u][v];
+                    if (!I8) x *= capped ? to_cap : scale2;
+                    if (capped) x = cap2 * tanh_fast(x);
                     st[u][v] = __builtin_fmaf(-slope2, fabsf(away - (float) (8 * (v / 4) + v % 4)), x);
                 }
-            } else {
-#pragma unroll
-                for (int v = 0; v < 16; v++) st[u][v] *= scale2;
             }
             if (masked) {
                 const unsigned missing = (unsigned) (gone_rows >> (32 * u)) >> (4 * h);
 #pragma unroll
                 for (int v = 0; v < 16; v++) {
                     const int e = 8 * (v / 4) + v % 4, j = key0 + 32 * u + 4 * h + e;
-                    if ((unsigned) (j - w.lo) >= (unsigned) (w.hi - w.lo) || ((missing >> e) & 1)) st[u][v] = -INFINITY;
+                    if ((unsigned) (j - w.lo) >= (unsigned) (w.hi - w.lo) || (PAGED && ((missing >> e) & 1))) st[u][v] = -INFINITY;
                 }
             }
 #pragma unroll
             for (int v = 0; v < 16; v++) top = fmaxf(top, st[u][v]);
         }
+        if (!LOG2_UNITS) top *= scale2;
         if (__any(top > ref + SLACK)) {
             top = fmaxf(top, __shfl_xor(top, 32));
             const float new_ref = fmaxf(ref, top);
@@ -397,10 +486,16 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const float e = __builtin_amdgcn_exp2f(st[u][v] - minus);
-                sum += e;
-                pv[2 * u + v / 8][v % 8] = (half_t) e;
+            for (int a = 0; a < 4; a++) {
+                floatx4 f = {1, 1, 1, 1};
+                if (I8) f = *(const floatx4 *) &vscale_s[buffer][32 * u + 8 * a + 4 * h];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int v = 4 * a + i;
+                    const float e = __builtin_amdgcn_exp2f(LOG2_UNITS ? st[u][v] - minus : __builtin_fmaf(st[u][v], scale2, -minus));
+                    sum += e;
+                    pv[2 * u + v / 8][v % 8] = (half_t) (I8 ? e * f[i] : e);
+                }
             }
 #pragma unroll
         for (int s = 0; s < 4; s++) {
@@ -411,29 +506,18 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
                 const halfx4 hi = lds_read_transposed(ks + v_corner + (16 * s + 8) * VS + 32 * t);
                 a[t] = halfx8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             }
-            if (bad_rows != 0)
-#pragma unroll
-                for (int t = 0; t < DT; t++) a[t] = finite_or_zero(a[t]);
 #pragma unroll
             for (int t = 0; t < DT; t++) oacc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[t], pv[s], oacc[t], 0, 0, 0);
-        }
-        // Infinities or NaN among the values of a block that not every row sees whole: a weight of zero does not remove them
-        // from a product, so they are left out above and added here for the queries that see their key.
-        for (unsigned long long left = bad_rows; left; left &= left - 1) {
-            const int key = __builtin_ctzll(left);
-            if ((unsigned) (key0 + key - w.lo) < (unsigned) (w.hi - w.lo))
-#pragma unroll
-                for (int t = 0; t < DT; t++)
-#pragma unroll
-                    for (int a = 0; a < 4; a++) {
-                        const halfx4 x = *(const halfx4 *) &ks[BKEYS * KS + key * VS + 32 * t + 8 * a + 4 * h];
-#pragma unroll
-                        for (int u = 0; u < 4; u++) oacc[t][4 * a + u] += (float) x[u] - (float) x[u] == 0.0f ? 0.0f : (float) x[u];
-                    }
         }
     }
 
     sum += __shfl_xor(sum, 32);
+    const float back = I8 ? 1.0f / value_unit : 1.0f;
+    // (dims 32 t + 8 a + 4 h + (0 .. 3) are registers 4 a .. 4 a + 3, the middle two changed over where widen() does)
+    auto dims = [&](int t, int a) {
+        return I8 ? floatx4{oacc[t][4 * a], oacc[t][4 * a + 2], oacc[t][4 * a + 1], oacc[t][4 * a + 3]}
+                  : floatx4{oacc[t][4 * a], oacc[t][4 * a + 1], oacc[t][4 * a + 2], oacc[t][4 * a + 3]};
+    };
     if (p.part_values) {
         // a part of the softmax: reference, sum and the sums of values as they are
         if (row < rows) {
@@ -442,23 +526,23 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
             for (int t = 0; t < DT; t++)
 #pragma unroll
-                for (int a = 0; a < 4; a++)
-                    *(floatx4 *) (o + 32 * t + 8 * a + 4 * h) = floatx4{oacc[t][4 * a], oacc[t][4 * a + 1], oacc[t][4 * a + 2], oacc[t][4 * a + 3]};
+                for (int a = 0; a < 4; a++) *(floatx4 *) (o + 32 * t + 8 * a + 4 * h) = dims(t, a) * back;
             if (h == 0) *(float2 *) (p.part_stats + 2 * at) = float2{ref, sum};
         }
         return;
     }
     // ---- the result: normalised, rounded, through the wave's rows of LDS into whole rows
-    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    const float inv = sum > 0.0f || sum != sum ? back / sum : 0.0f;
     __syncthreads();  // (every wave is done with the buffers)
     half_t *os = lds + wave * WAVE_ROWS;
 #pragma unroll
     for (int t = 0; t < DT; t++)
 #pragma unroll
         for (int a = 0; a < 4; a++) {
+            const floatx4 o = dims(t, a);
             halfx4 x;
 #pragma unroll
-            for (int u = 0; u < 4; u++) x[u] = (half_t) (oacc[t][4 * a + u] * inv);
+            for (int u = 0; u < 4; u++) x[u] = (half_t) (o[u] * inv);
             *(halfx4 *) &os[c * OS + 32 * t + 8 * a + 4 * h] = x;
         }
     __builtin_amdgcn_wave_barrier();
@@ -481,8 +565,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 //                    lanes; the order of a row's elements in the product is free, Q is loaded in the same one
 //   O^T += V^T P^T   the accumulators of two tiles of S^T are the operand, keys 4 g + e and 16 + 4 g + e; lane (i, g) reads
 //                    elements i DPL .. + DPL - 1 of those 8 keys and turns them in registers: product dt has dim i DPL + dt
-// Whole numbers become f16 without a conversion instruction: q + 128 in the low byte of 0x6400 is 1152 + q, the
-// subtraction is exact. The scale of a key is applied to its score, that of a value to its weight, in f32; the reference
+// The scale of a key is applied to its score, that of a value to its weight, in f32; the reference
 // of the softmax follows score + log2(value scale), which keeps the scaled weights inside the range of f16.
 
 // Which keys a workgroup takes, decided on the device, where the lengths are: stretches (the prefix when it is done here, then
@@ -549,19 +632,6 @@ __device__ __forceinline__ bool find_item(const ServingAttentionParams &p, int w
         base += __builtin_amdgcn_readlane(sums, 63);
     }
     return false;
-}
-
-__device__ __forceinline__ unsigned pk_sub_1152(unsigned x) {
-    const halfx2 bias = {(half_t) -1152.0f, (half_t) -1152.0f};
-    return __builtin_bit_cast(unsigned, __builtin_bit_cast(halfx2, x) + bias);
-}
-
-// 8 whole numbers of 8 bits as f16, in the order 0 2 1 3 4 6 5 7
-__device__ __forceinline__ halfx8 widen(unsigned a, unsigned b) {
-    a ^= 0x80808080u;
-    b ^= 0x80808080u;
-    return __builtin_bit_cast(halfx8, uint4{pk_sub_1152((a & 0x00ff00ffu) | 0x64006400u), pk_sub_1152(((a >> 8) & 0x00ff00ffu) | 0x64006400u),
-                                            pk_sub_1152((b & 0x00ff00ffu) | 0x64006400u), pk_sub_1152(((b >> 8) & 0x00ff00ffu) | 0x64006400u)});
 }
 
 template <int WORDS>
@@ -1030,6 +1100,11 @@ __global__ __launch_bounds__(64 * WAVES) void join_attention_kernel(ServingAtten
 
 // ---- plans ---------------------------------------------------------------------------------------------------------
 
+// Whole numbers are widened as they are staged, work that eight waves share better than four (16384 shared keys of width 128
+// for 256 rows of 8 heads: 51.6 -> 44.1 us); f16 only passes through, and smaller workgroups wait less for each other (8192
+// tokens of 32 heads: 884 us against 915).
+constexpr int tile_waves(int wp, bool i8) { return wp == 128 && i8 ? 8 : 4; }
+
 struct Plan {
     int own_rows;             // per sequence and head of keys
     long long prefix_rows;
@@ -1044,8 +1119,8 @@ struct Plan {
 
 // Keys are shared by several workgroups while tiles alone leave compute units idle (two workgroups fit each), down to
 // parts of four blocks: below, a part costs more to write and to join than it saves.
-int splits_for(long long workgroups, long long keys) {
-    constexpr long long WANTED = 512;
+int splits_for(long long workgroups, long long keys, int waves) {
+    const long long WANTED = 2048 / waves;
     if (workgroups >= WANTED || workgroups == 0) return 1;
     return (int) std::max(1ll, std::min((WANTED + workgroups - 1) / workgroups, keys / 256));
 }
@@ -1059,14 +1134,15 @@ Plan plan_for(const ServingAttentionParams &p) {
     l.own_in_rows = p.paged && l.own_rows <= 32;
     l.prefix_in_rows = p.prefix_tokens > 0 && l.prefix_rows <= 32;
     const long long pairs = (long long) p.batch * p.kv_heads;
+    const int tile_rows = 32 * tile_waves(l.wp, p.k_scales != nullptr);
     if (!l.own_in_rows) {
-        l.own_tiles = (l.own_rows + 127) / 128;
-        l.own_splits = splits_for(l.own_tiles * pairs, p.paged ? p.table_tokens : p.keys);
+        l.own_tiles = (l.own_rows + tile_rows - 1) / tile_rows;
+        l.own_splits = splits_for(l.own_tiles * pairs, p.paged ? p.table_tokens : p.keys, tile_waves(l.wp, p.k_scales != nullptr));
         l.own_parts = l.own_splits * pairs * l.own_rows;
     }
     if (p.prefix_tokens > 0 && !l.prefix_in_rows) {
-        l.prefix_tiles = (l.prefix_rows + 127) / 128;
-        l.prefix_splits = splits_for(l.prefix_tiles * p.kv_heads, p.prefix_tokens);
+        l.prefix_tiles = (l.prefix_rows + tile_rows - 1) / tile_rows;
+        l.prefix_splits = splits_for(l.prefix_tiles * p.kv_heads, p.prefix_tokens, tile_waves(l.wp, p.k_scales != nullptr));
         l.prefix_parts = (long long) l.prefix_splits * p.kv_heads * l.prefix_rows;
     }
     if (l.own_in_rows) {
@@ -1087,8 +1163,10 @@ size_t round256(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 template <int WP, int STRETCH, bool I8>
 int launch_tiles(const ServingAttentionParams &p, unsigned workgroups, int splits, hipStream_t stream) {
-    if (p.cap > 0.0f || p.slopes) hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, true>), dim3(workgroups, (unsigned) splits), dim3(64 * WAVES), 0, stream, p);
-    else hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, false>), dim3(workgroups, (unsigned) splits), dim3(64 * WAVES), 0, stream, p);
+    constexpr int TW = tile_waves(WP, I8);
+    const dim3 grid(workgroups, (unsigned) splits), block(64 * TW);
+    if (p.cap > 0.0f || p.slopes) hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, true, TW>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, false, TW>), grid, block, 0, stream, p);
     return (int) hipGetLastError();
 }
 
