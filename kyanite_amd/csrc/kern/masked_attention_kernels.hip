@@ -93,6 +93,27 @@ __device__ __forceinline__ float tanh_fast(float x) {
     return __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * (2.0f * LOG2E))), 1.0f);
 }
 
+// a number that is the same in all lanes, into a scalar register
+__device__ __forceinline__ float uniform(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); }
+
+// c tanh(f s) for |f s| <= 0.35 as an odd series in s, up to the 9th power: the next term is 1382 / 155925 x^10 of the result,
+// below 2.5e-7. Half the time of the exponential and the reciprocal.
+struct CapSeries {
+    float k[5];
+    __device__ __forceinline__ CapSeries(float c, float f) {
+        const float g = f * f;
+        k[0] = uniform(c * f);
+        k[1] = uniform(k[0] * g * (-1.0f / 3));
+        k[2] = uniform(k[0] * g * g * (2.0f / 15));
+        k[3] = uniform(k[0] * g * g * g * (-17.0f / 315));
+        k[4] = uniform(k[0] * g * g * g * g * (62.0f / 2835));
+    }
+};
+__device__ __forceinline__ float cap_series(float s, const CapSeries &c) {
+    const float q = s * s;
+    return s * __builtin_fmaf(q, __builtin_fmaf(q, __builtin_fmaf(q, __builtin_fmaf(q, c.k[4], c.k[3]), c.k[2]), c.k[1]), c.k[0]);
+}
+
 // four keys (consecutive rows of the staged V) of one dim: 16 lanes hand in the addresses of 4 dims of 4 rows each
 __device__ __forceinline__ halfx4 lds_read_transposed(const half_t *p) {
     return __builtin_bit_cast(halfx4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *) p));
@@ -275,10 +296,13 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         }
     };
     // A scale of zero or less goes into Q (times -1, 0 or 1), so that the scores are multiplied by a positive number
-    const float sign = p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f;
-    const float scale2 = p.scale == 0.0f ? 1.0f : fabsf(p.scale) * LOG2E;
+    const float sign = uniform(p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f);
+    const float scale2 = uniform(p.scale == 0.0f ? 1.0f : fabsf(p.scale) * LOG2E);
     const bool capped = SHAPED && p.cap > 0.0f;
-    const float to_cap = capped ? scale2 / (LOG2E * p.cap) : 0.0f, cap2 = p.cap * LOG2E;
+    const float to_cap = uniform(capped ? scale2 / (LOG2E * p.cap) : 0.0f), cap2 = uniform(p.cap * LOG2E);
+    // the series takes scores (I8: scores over the cap) up to 0.35 of the cap
+    const CapSeries series(cap2, I8 ? 1.0f : to_cap);
+    const float near_cap = I8 ? 0.35f : uniform(0.35f / to_cap);
     float value_unit = 0x1p60f;  // I8: what the scales of values are multiplied by, a power of two
     auto stage = [&](int buffer, bool masked) {
         half_t *ks = lds + buffer * STAGE, *vs = ks + BKEYS * KS;
@@ -448,15 +472,26 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
                     for (int e = 0; e < 4; e++) st[u][4 * a + e] *= f[e];
                 }
-            if (SHAPED) {
+            if (SHAPED && capped) {
+                // (the same choice for the whole wave; most scores lie far below the cap)
+                float far = fabsf(st[u][0]);
+#pragma unroll
+                for (int v = 1; v < 16; v++) far = fmaxf(far, fabsf(st[u][v]));
+                if (__all(far <= near_cap)) {
+#pragma unroll
+                    for (int v = 0; v < 16; v++) st[u][v] = cap_series(st[u][v], series);
+                } else {
+#pragma unroll
+                    for (int v = 0; v < 16; v++) st[u][v] = cap2 * tanh_fast(I8 ? st[u][v] : st[u][v] * to_cap);
+                }
+            } else if (SHAPED && !I8) {
+#pragma unroll
+                for (int v = 0; v < 16; v++) st[u][v] *= scale2;
+            }
+            if (SHAPED && p.slopes) {
                 const float away = (float) (w.at - (key0 + 32 * u + 4 * h));
 #pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    float x = st[u][v];
-                    if (!I8) x *= capped ? to_cap : scale2;
-                    if (capped) x = cap2 * tanh_fast(x);
-                    st[u][v] = __builtin_fmaf(-slope2, fabsf(away - (float) (8 * (v / 4) + v % 4)), x);
-                }
+                for (int v = 0; v < 16; v++) st[u][v] = __builtin_fmaf(-slope2, fabsf(away - (float) (8 * (v / 4) + v % 4)), st[u][v]);
             }
             if (masked) {
                 const unsigned missing = (unsigned) (gone_rows >> (32 * u)) >> (4 * h);
@@ -654,7 +689,9 @@ __device__ __forceinline__ void load_words(const char *from, unsigned (&to)[WORD
 // PAGE16: pages are multiples of 16 tokens and a tile of 16 keys spans less than 2 GiB, so that a tile lies in one page, whose
 // number and address the whole wave shares, and lanes differ by 32 bit offsets
 template <int WP, int NT, bool I8, bool SHAPED, bool PAGE16>
-__global__ __launch_bounds__(ROW_THREADS) void row_attention_kernel(ServingAttentionParams p, int with_prefix) {
+// (at least two waves per SIMD: with more registers than that leaves, the results of matrix instructions would lie in AGPRs, and
+// the compiler reads such a result too early behind a branch)
+__global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))) void row_attention_kernel(ServingAttentionParams p, int with_prefix) {
     constexpr int ELEM = I8 ? 1 : 2;
     constexpr int KP = WP * ELEM / 64;    // 16 byte pieces of a key per lane
     constexpr int DPL = WP / 16;          // dims of a value per lane
@@ -1027,11 +1064,13 @@ __global__ __launch_bounds__(ROW_THREADS) void row_attention_kernel(ServingAtten
 
 // ---- parts -> results ----------------------------------------------------------------------------------------------
 
-// A wave per row of the result. WP / 64 elements per lane.
+// A wave per row of the result. WP / 4 lanes take a part's row, 16 bytes each, so that a wave reads 2 (4) parts at a time; up
+// to 32 parts are in flight together, requested before their weights are known. Bound by the parts: they come out of the
+// caches of other XCDs.
 template <int WP>
 __global__ __launch_bounds__(64 * WAVES) void join_attention_kernel(ServingAttentionParams p) {
-    constexpr int N = WP / 64;
-    const int lane = threadIdx.x & 63;
+    constexpr int LANES = WP / 4, SIDE = 64 / LANES, AHEAD = 32 / SIDE;
+    const int lane = threadIdx.x & 63, side = lane / LANES, d = 4 * (lane % LANES);
     const unsigned row = __builtin_amdgcn_readfirstlane(blockIdx.x * WAVES + (threadIdx.x >> 6));
     if (row >= (unsigned) p.batch * p.queries * p.heads) return;
     const unsigned token = row / (unsigned) p.heads, head = row - token * p.heads;
@@ -1043,59 +1082,62 @@ __global__ __launch_bounds__(64 * WAVES) void join_attention_kernel(ServingAtten
     long long at[2] = {0, 0}, apart[2] = {0, 0};
     int count[2] = {0, 0};
     if (p.prefix_splits > 0) {
-        at[0] = kv_head * p.prefix_splits * prefix_rows + prefix_row;
+        at[0] = (long long) kv_head * p.prefix_splits * prefix_rows + prefix_row;
         apart[0] = prefix_rows;
         count[0] = p.prefix_splits;
     } else if (p.prefix_tokens > 0) {
         const int2 items = ((const int2 *) p.part_items)[0];
-        at[0] = p.row_prefix_part + (long long) (items.x * p.kv_heads + kv_head) * prefix_rows + prefix_row;
+        at[0] = p.row_prefix_part + ((long long) items.x * p.kv_heads + kv_head) * prefix_rows + prefix_row;
         apart[0] = p.kv_heads * prefix_rows;
         count[0] = items.y;
     }
     if (p.own_splits > 0) {
-        at[1] = p.row_own_part + (long long) (b * p.kv_heads + kv_head) * p.own_splits * own_rows + own_row;
+        at[1] = p.row_own_part + ((long long) b * p.kv_heads + kv_head) * p.own_splits * own_rows + own_row;
         apart[1] = own_rows;
         count[1] = p.own_splits;
     } else {
         const int2 items = ((const int2 *) p.part_items)[b + 1];
         if (p.prefix_tokens == 0 && items.y == 1) return;  // (written where it was computed)
-        at[1] = p.row_own_part + (long long) (items.x * p.kv_heads + kv_head) * own_rows + own_row;
+        at[1] = p.row_own_part + ((long long) items.x * p.kv_heads + kv_head) * own_rows + own_row;
         apart[1] = p.kv_heads * own_rows;
         count[1] = items.y;
     }
-    float top = -INFINITY;
+    float top = -INFINITY, total = 0.0f;
+    floatx4 x = {0, 0, 0, 0};
 #pragma unroll
     for (int s = 0; s < 2; s++)
-        for (int i = lane; i < count[s]; i += 64) top = fmaxf(top, p.part_stats[2 * (at[s] + i * apart[s])]);
+        for (int i0 = 0; i0 < count[s]; i0 += 32) {
+            const int n = min(32, count[s] - i0);
+            floatx4 part[AHEAD];
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-    if (top == -INFINITY) top = 0.0f;
-    float total = 0.0f, x[N] = {};
-#pragma unroll
-    for (int s = 0; s < 2; s++)
-        for (int i0 = 0; i0 < count[s]; i0 += 64) {
-            float weight = 0.0f;
-            if (i0 + lane < count[s]) {
-                const float2 st = *(const float2 *) (p.part_stats + 2 * (at[s] + (i0 + lane) * apart[s]));
-                weight = __builtin_amdgcn_exp2f(st.x - top);
-                total += weight * st.y;
+            for (int a = 0; a < AHEAD; a++) {
+                const int i = a * SIDE + side;
+                part[a] = floatx4{0, 0, 0, 0};
+                if (i < n) part[a] = *(const floatx4 *) (p.part_values + (at[s] + (i0 + i) * apart[s]) * WP + d);
             }
-            const float *from = p.part_values + (at[s] + i0 * apart[s]) * WP + N * lane;
-            const int n = min(64, count[s] - i0);
-#pragma unroll 4
-            for (int i = 0; i < n; i++) {
-                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), i));
+            float2 stats = {-INFINITY, 0.0f};
+            if (lane < n) stats = *(const float2 *) (p.part_stats + 2 * (at[s] + (i0 + lane) * apart[s]));
+            float new_top = fmaxf(top, stats.x);
 #pragma unroll
-                for (int k = 0; k < N; k++) x[k] += w * from[i * apart[s] * WP + k];
-            }
+            for (int m = 1; m < 64; m <<= 1) new_top = fmaxf(new_top, __shfl_xor(new_top, m));
+            const float ref = new_top == -INFINITY ? 0.0f : new_top, old = __builtin_amdgcn_exp2f(top - ref);
+            const float weight = __builtin_amdgcn_exp2f(stats.x - ref);
+            top = new_top;
+            total = total * old + weight * stats.y;
+            x *= old;
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++) x += __shfl(weight, a * SIDE + side) * part[a];
         }
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) total += __shfl_xor(total, m);
-    const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
-    half_t *o = (half_t *) p.out + (b * p.o_batch + t * p.o_token + head * p.o_head);
 #pragma unroll
-    for (int k = 0; k < N; k++)
-        if (N * lane + k < p.width) o[N * lane + k] = (half_t) (x[k] * inv);
+    for (int m = LANES; m < 64; m <<= 1)
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] += __shfl_xor(x[k], m);
+    const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+    if (side == 0 && d < p.width)
+        *(halfx4_any *) ((half_t *) p.out + (b * p.o_batch + t * p.o_token + head * p.o_head + d)) =
+            halfx4{(half_t) (x[0] * inv), (half_t) (x[1] * inv), (half_t) (x[2] * inv), (half_t) (x[3] * inv)};
 }
 
 // ---- plans ---------------------------------------------------------------------------------------------------------
