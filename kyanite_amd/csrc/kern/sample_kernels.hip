@@ -4,17 +4,23 @@
 // sums of them are exact and the same in any order, so counting and adding may run in any order and with atomics. exp and its
 // argument are f64: the nearest of 10^5 borders between tokens is then missed once in 10^10 rows or so.
 //
-// A row belongs to one workgroup of 16 waves, each of which owns a contiguous part of it. Rows that fit are held in LDS
-// (f16: 60000 logits), so that they are read once; what then bounds a row is the arithmetic per logit of one compute unit.
-// The filters end in one threshold, the last token that stays in the order of falling logits (ties: rising index):
-//   1. a histogram over the distance to the maximum, 2048 buckets over the distances at which w is not zero, counts for
-//      top_k, masses for top_p. (Buckets on the bits of x would put most of a row into two dozen of them: the atomics of a
-//      wave would queue. Over the distance a normal distribution fills hundreds.)
-//   2. the tokens of the bucket where the count or the mass is reached, usually a hundred, are sorted.
-// With top_k, all tokens down to that bucket are sorted instead where they are 2048 at most, and the other filters and the
-// draw work on that list alone. A bucket with more than 2048 tokens (flat rows) is searched by the bits of x, 8 at a time.
-// Without a list the token is found in two steps: the wave whose part holds the target, and the place inside that part.
+// A row belongs to one workgroup of 16 waves, each of which owns a contiguous part of it. What bounds a row is the arithmetic
+// per logit of one compute unit, and the fetch rate of one (about 40 GB/s) for rows that do not fit LDS. So a row is read
+// once where it fits (f16: 53000 logits), and the maxima of its groups of 8 logits are kept beside it, so that later passes
+// touch only groups that can matter. The filters end in one threshold, the last token that stays in the order of falling
+// logits (ties: rising index):
+//   top_k   the group maxima go into a histogram over the distance to the largest. The bucket that holds the k-th largest of
+//           them bounds the k-th largest logit from below: the groups that reach it, little more than k, are listed and
+//           sorted, and the other filters and the draw work on that list alone.
+//   top_p   (and top_k beyond what the list holds) all logits go into the histogram, masses (counts) instead of ones; the
+//           tokens of the bucket where the mass is reached, usually a hundred, are sorted.
+// The 2048 buckets span the distances at which w is not zero. (Buckets on the bits of x would put most of a row into two dozen
+// of them: the atomics of a wave would queue. Over the distance a normal distribution fills hundreds.) A bucket with more
+// than 2048 tokens (flat rows) is searched by the bits of x, 8 at a time. Without a list the token is found in two steps: the
+// wave whose part holds the target, and the place inside that part.
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "../serving_kernels.h"
 
@@ -24,7 +30,7 @@ namespace {
 
 constexpr int THREADS = 1024, NWAVES = THREADS / 64;
 constexpr int BUCKETS = 2 * THREADS, LISTED = 2 * THREADS;
-constexpr int CACHE_BYTES = 116 * 1024;
+constexpr int CACHE_BYTES = 104 * 1024, CACHED_MAXIMA_BYTES = CACHE_BYTES / 8, MAXIMA_BYTES = 112 * 1024;
 
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 typedef _Float16 halfx8_any __attribute__((ext_vector_type(8), aligned(2)));
@@ -41,26 +47,27 @@ __device__ __forceinline__ unsigned key_of(float x) {
     return u ^ ((unsigned) ((int) u >> 31) | 0x80000000u);
 }
 
-// 16 bytes of a row
+constexpr int GROUP = 8;
 template <bool F16>
-struct Vec {
-    static constexpr int N = F16 ? 8 : 4;
-    float x[N];
+struct Raw {  // a group as it lies in memory
+    uint4 v[F16 ? 1 : 2];
+};
+struct Group {
+    float x[GROUP];
 };
 
 template <bool F16>
-__device__ __forceinline__ Vec<F16> unpack(uint4 raw) {
-    Vec<F16> v;
+__device__ __forceinline__ Group unpack(const Raw<F16> &raw) {
+    Group g;
     if constexpr (F16) {
-        const halfx8 h = __builtin_bit_cast(halfx8, raw);
+        const halfx8 h = __builtin_bit_cast(halfx8, raw.v[0]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) v.x[e] = plain((float) h[e]);
+        for (int e = 0; e < 8; e++) g.x[e] = plain((float) h[e]);
     } else {
-        const floatx4 f = __builtin_bit_cast(floatx4, raw);
 #pragma unroll
-        for (int e = 0; e < 4; e++) v.x[e] = plain(f[e]);
+        for (int e = 0; e < 8; e++) g.x[e] = plain(__builtin_bit_cast(floatx4, raw.v[e / 4])[e % 4]);
     }
-    return v;
+    return g;
 }
 
 template <bool F16>
@@ -68,25 +75,34 @@ __device__ __forceinline__ float load_one(const void *row, int i) {
     return plain(F16 ? (float) ((const _Float16 *) row)[i] : ((const float *) row)[i]);
 }
 
-// vector n of a row of `vocab` logits; what lies behind its end reads as -inf
+// group n of a row of `vocab` logits; what lies behind its end reads as -inf
 template <bool F16>
-__device__ __forceinline__ uint4 load_raw(const void *row, int n, int vocab) {
-    constexpr int N = Vec<F16>::N;
-    if (n * N + N <= vocab) {
-        if constexpr (F16) return __builtin_bit_cast(uint4, *(const halfx8_any *) ((const _Float16 *) row + n * N));
-        else return __builtin_bit_cast(uint4, *(const floatx4_any *) ((const float *) row + n * N));
+__device__ __forceinline__ Raw<F16> load_group(const void *row, int n, int vocab) {
+    Raw<F16> raw;
+    if (n * GROUP + GROUP <= vocab) {
+        if constexpr (F16) {
+            raw.v[0] = __builtin_bit_cast(uint4, *(const halfx8_any *) ((const _Float16 *) row + n * GROUP));
+        } else {
+            raw.v[0] = __builtin_bit_cast(uint4, *(const floatx4_any *) ((const float *) row + n * GROUP));
+            raw.v[1] = __builtin_bit_cast(uint4, *(const floatx4_any *) ((const float *) row + n * GROUP + 4));
+        }
+        return raw;
     }
     if constexpr (F16) {
         halfx8 h;
 #pragma unroll
-        for (int e = 0; e < 8; e++) h[e] = n * N + e < vocab ? ((const _Float16 *) row)[n * N + e] : (_Float16) -INFINITY;
-        return __builtin_bit_cast(uint4, h);
+        for (int e = 0; e < 8; e++) h[e] = n * GROUP + e < vocab ? ((const _Float16 *) row)[n * GROUP + e] : (_Float16) -INFINITY;
+        raw.v[0] = __builtin_bit_cast(uint4, h);
     } else {
-        floatx4 f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) f[e] = n * N + e < vocab ? ((const float *) row)[n * N + e] : -INFINITY;
-        return __builtin_bit_cast(uint4, f);
+        for (int e = 0; e < 8; e += 4) {
+            floatx4 f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) f[k] = n * GROUP + e + k < vocab ? ((const float *) row)[n * GROUP + e + k] : -INFINITY;
+            raw.v[e / 4] = __builtin_bit_cast(uint4, f);
+        }
     }
+    return raw;
 }
 
 // exp((x - top) / T) 2^bits for x <= top. 2^(n / 64 + r / 64) with |r| <= 1/2: a table of 64 roots of two, and the series of
@@ -96,18 +112,24 @@ struct Weigher {
     double per;  // 64 log2(e) / T
     int bits;
     const double *roots;
-    __device__ __forceinline__ double real(float x) const {
+    // (exact at x = top: the argument is zero)
+    __device__ __forceinline__ double core(double t) const {
         constexpr double L = 0.010830424696249145;  // ln(2) / 64
-        const double t = fmax(((double) x - (double) top) * per, -64.0 * 1000);
-        const double n = __builtin_rint(t), z = (t - n) * L;
+        const double n = __builtin_rint(t), y = t - n;
         const int i = (int) n;
-        const double s = __builtin_fma(z, __builtin_fma(z, __builtin_fma(z, __builtin_fma(z, __builtin_fma(z, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0), 1.0);
-        const double w = __builtin_ldexp(roots[i & 63] * s, (i >> 6) + bits);
-        return x == top ? __builtin_ldexp(1.0, bits) : top == INFINITY || x == -INFINITY ? 0.0 : w;
+        const double s = __builtin_fma(y, __builtin_fma(y, __builtin_fma(y, __builtin_fma(y, __builtin_fma(y, L * L * L * L * L / 120, L * L * L * L / 24), L * L * L / 6), L * L / 2), L), 1.0);
+        return __builtin_ldexp(roots[i & 63] * s, (i >> 6) + bits);
+    }
+    __device__ __forceinline__ double real(float x) const {
+        if (top == INFINITY || x == -INFINITY) return x == top ? __builtin_ldexp(1.0, bits) : 0.0;
+        return core(fmax(((double) x - (double) top) * per, -64.0 * 1000));
     }
     // (bits <= 51: adding 2^52 rounds to a whole number and leaves it in the low bits)
     static __device__ __forceinline__ mass_t whole(double w) { return __builtin_bit_cast(mass_t, w + 0x1p52) & ((1ull << 52) - 1); }
     __device__ __forceinline__ mass_t operator()(float x) const { return whole(real(x)); }
+    // the same for finite logits within the distance of the histogram
+    __device__ __forceinline__ double near_real(float x) const { return core(((double) x - (double) top) * per); }
+    __device__ __forceinline__ mass_t near(float x) const { return whole(near_real(x)); }
 };
 
 __device__ __forceinline__ float logit_of(unsigned key) {
@@ -119,7 +141,7 @@ struct Shared {
     mass_t list[LISTED];  // key and, below it, the complement of the index: falling order is the order of the filters
     float queue[NWAVES][128];
     double roots[64];
-    mass_t wave_mass[NWAVES];
+    mass_t wave_mass[NWAVES], part_mass[NWAVES];
     float wave_top[NWAVES];
     int list_count, bucket;
     mass_t above;
@@ -155,15 +177,20 @@ __device__ __forceinline__ mass_t block_scan(mass_t v, mass_t *shared) {
     return v;
 }
 
-// the first `count` entries of the list into falling (or rising) order
+// The first `count` entries of the list into falling (or rising) order: a bitonic network, a thread per pair. Steps of 64 and
+// less stay inside the 128 entries of a wave and need no barrier.
 __device__ __forceinline__ void sort_list(mass_t *list, int count, bool rising) {
     int size = 2;
     while (size < count) size *= 2;
     __syncthreads();
     for (int i = count + (int) threadIdx.x; i < size; i += THREADS) list[i] = rising ? ~0ull : 0;
+    __syncthreads();
+    bool shared = false;  // whether other waves have written since the last barrier
     for (int run = 2; run <= size; run *= 2)
         for (int step = run / 2; step > 0; step /= 2) {
-            __syncthreads();
+            if (step > 64 || shared) __syncthreads();
+            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            shared = step > 64;
             if ((int) threadIdx.x < size / 2) {
                 const int i = 2 * (int) threadIdx.x - ((int) threadIdx.x & (step - 1)), j = i + step;
                 const mass_t a = list[i], b = list[j];
@@ -183,60 +210,65 @@ __device__ __forceinline__ mass_t target_of(float u, mass_t total) {
 
 template <bool F16, bool CACHED>
 __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
-    constexpr int N = Vec<F16>::N;
     __shared__ Shared sh;
-    __shared__ uint4 cache[CACHED ? CACHE_BYTES / 16 : 1];
+    __shared__ Raw<F16> cache[CACHED ? CACHE_BYTES / sizeof(Raw<F16>) : 1];
+    // the maxima of the groups; rows of more than that hold none
+    using maximum_t = std::conditional_t<F16, _Float16, float>;
+    constexpr int MAXIMA = (CACHED ? CACHED_MAXIMA_BYTES : MAXIMA_BYTES) / sizeof(maximum_t);
+    __shared__ maximum_t maxima[MAXIMA];
     const int r = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const void *row = (const char *) p.logits + r * p.row_stride * (F16 ? 2 : 4);
-    const int vectors = (p.vocab + N - 1) / N, part = (vectors + NWAVES - 1) / NWAVES;
-    const int begin = min(wave * part, vectors), end = min(begin + part, vectors);  // of this wave, in vectors
+    const int groups = (p.vocab + GROUP - 1) / GROUP, part = (groups + NWAVES - 1) / NWAVES;
+    const int begin = min(wave * part, groups), end = min(begin + part, groups);  // of this wave, in groups
+    const bool has_maxima = CACHED || groups <= MAXIMA;
+    auto group_at = [&](int n) { return CACHED ? cache[n] : load_group<F16>(row, n, p.vocab); };
 
-    // f(first index, values) for the vectors of this wave
+    // f(first index, logits) for the groups of this wave
     auto each = [&](auto f) {
         int n = begin + lane;
-        constexpr int AHEAD = 4;
+        constexpr int AHEAD = 2;
         for (; n + 64 * (AHEAD - 1) < end; n += 64 * AHEAD) {
-            uint4 raw[AHEAD];
+            Raw<F16> raw[AHEAD];
 #pragma unroll
-            for (int a = 0; a < AHEAD; a++) raw[a] = CACHED ? cache[n + 64 * a] : load_raw<F16>(row, n + 64 * a, p.vocab);
+            for (int a = 0; a < AHEAD; a++) raw[a] = group_at(n + 64 * a);
 #pragma unroll
-            for (int a = 0; a < AHEAD; a++) f((n + 64 * a) * N, unpack<F16>(raw[a]));
+            for (int a = 0; a < AHEAD; a++) f((n + 64 * a) * GROUP, unpack<F16>(raw[a]));
         }
-        for (; n < end; n += 64) f(n * N, unpack<F16>(CACHED ? cache[n] : load_raw<F16>(row, n, p.vocab)));
+        for (; n < end; n += 64) f(n * GROUP, unpack<F16>(group_at(n)));
     };
 
-    // the same with all lanes of the wave together, f(first index, values, whether there are any)
-    auto each_in_step = [&](auto f) {
-        for (int n0 = begin; n0 < end; n0 += 64) {
-            const int n = n0 + lane;
-            const bool live = n < end;
-            f(n * N, unpack<F16>(CACHED ? cache[live ? n : begin] : load_raw<F16>(row, live ? n : begin, p.vocab)), live);
-        }
-    };
-
-    // ---- the maximum (and the row into LDS)
+    // ---- the maximum, of the row and of its groups (and the row into LDS)
     float top = -INFINITY;
     {
         int n = begin + lane;
-        constexpr int AHEAD = 8;
-        auto take = [&](int at, uint4 raw) {
+        constexpr int AHEAD = F16 ? 8 : 4;
+        auto take = [&](int at, const Raw<F16> &raw) {
             if (CACHED) cache[at] = raw;
-            const Vec<F16> v = unpack<F16>(raw);
+            const Group g = unpack<F16>(raw);
+            float m = g.x[0];
 #pragma unroll
-            for (int e = 0; e < N; e++) top = fmaxf(top, v.x[e]);
+            for (int e = 1; e < GROUP; e++) m = fmaxf(m, g.x[e]);
+            if (has_maxima) maxima[at] = (maximum_t) m;
+            top = fmaxf(top, m);
         };
         for (; n + 64 * (AHEAD - 1) < end; n += 64 * AHEAD) {
-            uint4 raw[AHEAD];
+            Raw<F16> raw[AHEAD];
 #pragma unroll
-            for (int a = 0; a < AHEAD; a++) raw[a] = load_raw<F16>(row, n + 64 * a, p.vocab);
+            for (int a = 0; a < AHEAD; a++) raw[a] = load_group<F16>(row, n + 64 * a, p.vocab);
 #pragma unroll
             for (int a = 0; a < AHEAD; a++) take(n + 64 * a, raw[a]);
         }
-        for (; n < end; n += 64) take(n, load_raw<F16>(row, n, p.vocab));
+        for (; n < end; n += 64) take(n, load_group<F16>(row, n, p.vocab));
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
         if (lane == 0) sh.wave_top[wave] = top;
         if (threadIdx.x < 64) sh.roots[threadIdx.x] = exp2(threadIdx.x * (1.0 / 64));
+        for (int b = threadIdx.x; b < BUCKETS; b += THREADS) sh.hist[b] = 0;
+        if (threadIdx.x == 0) {
+            sh.list_count = 0;
+            sh.bucket = BUCKETS;
+            sh.last_index = p.vocab;
+        }
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < NWAVES; w++) top = fmaxf(top, sh.wave_top[w]);
@@ -250,14 +282,18 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     }
     const float t = p.temperature ? p.temperature[r] : 1.0f;
     if (!(t > 0.0f)) {  // the first of the largest
-        if (threadIdx.x == 0) sh.last_index = p.vocab;
-        __syncthreads();
         int first = p.vocab;
-        each([&](int i, const Vec<F16> &v) {
+        auto look = [&](int i, const Group &g) {
 #pragma unroll
-            for (int e = N - 1; e >= 0; e--)
-                if (v.x[e] == top) first = min(first, i + e);
-        });
+            for (int e = GROUP - 1; e >= 0; e--)
+                if (g.x[e] == top) first = min(first, i + e);
+        };
+        if (has_maxima) {
+            for (int n = threadIdx.x; n < groups; n += THREADS)
+                if ((float) maxima[n] == top && n * GROUP < first) look(n * GROUP, unpack<F16>(group_at(n)));
+        } else {
+            each(look);
+        }
         if (first < p.vocab) atomicMin(&sh.last_index, first);
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -269,6 +305,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     const Weigher weigh{top, 92.332482616893656877 / (double) t, p.bits, sh.roots};
     const int k = p.top_k ? p.top_k[r] : 0;
     const float top_p = p.top_p ? p.top_p[r] : 1.0f;
+    const double min_w = p.min_p ? __builtin_ldexp((double) p.min_p[r], p.bits) : 0.0;
     // distances at which w may be more than zero: exp(-range / T) 2^bits = 1 / 4
     const float range = t * (0.6931472f * (p.bits + 2)), per_bucket = fminf(BUCKETS / range, 3e38f);
     const bool spread = range < 1e37f && top < INFINITY;
@@ -278,10 +315,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     bool restricted = false;
     auto stays = [&](unsigned key, int i) { return key > last_key || (key == last_key && i <= last_index); };
     const double mass_wanted = top_p < 1.0f ? fmax((double) top_p, 0.0) : 1.0;
-    const double min_w = p.min_p ? __builtin_ldexp((double) p.min_p[r], p.bits) : 0.0;
 
-    // ---- the histogram of what stays so far, and the bucket where enough is reached
-    auto fill_hist = [&](bool by_mass) {
+    // ---- the bucket of the histogram where enough is reached
+    auto clear_hist = [&] {
         __syncthreads();
         for (int b = threadIdx.x; b < BUCKETS; b += THREADS) sh.hist[b] = 0;
         if (threadIdx.x == 0) {
@@ -289,20 +325,11 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
             sh.bucket = BUCKETS;
         }
         __syncthreads();
-        each([&](int i, const Vec<F16> &v) {
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const unsigned b = bucket_of(v.x[e]);
-                if (b >= BUCKETS || (restricted && !stays(key_of(v.x[e]), i + e))) continue;
-                if (by_mass) atomicAdd(&sh.hist[b], weigh(v.x[e]));
-                else atomicAdd((unsigned *) &sh.hist[b], 1u);
-            }
-        });
-        __syncthreads();
     };
     // sh.bucket, sh.above: the first bucket at whose end `need` is reached, and what lies before it; BUCKETS when it never is.
     // Masses: `need` is mass_wanted of all. Returns `need`.
     auto find_bucket = [&](bool by_mass, mass_t need) {
+        __syncthreads();
         // a thread takes two neighbouring buckets
         const mass_t a = sh.hist[2 * threadIdx.x], both = a + sh.hist[2 * threadIdx.x + 1];
         const mass_t sums = block_scan(both, sh.wave_mass), before = sums - both;
@@ -320,20 +347,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         __syncthreads();
         return need;
     };
-    // the tokens of the buckets from..to among what stays, as far as they fit
-    auto gather = [&](unsigned from, unsigned to) {
-        each([&](int i, const Vec<F16> &v) {
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const unsigned b = bucket_of(v.x[e]);
-                if (b < from || b > to) continue;
-                const unsigned key = key_of(v.x[e]);
-                if (restricted && !stays(key, i + e)) continue;
-                const int c = atomicAdd(&sh.list_count, 1);
-                if (c < LISTED) sh.list[c] = (mass_t) key << 32 | ~(unsigned) (i + e);
-            }
-        });
-        __syncthreads();
+    auto append = [&](unsigned key, int i) {
+        const int c = atomicAdd(&sh.list_count, 1);
+        if (c < LISTED) sh.list[c] = (mass_t) key << 32 | ~(unsigned) i;
     };
     auto mass_of_entry = [&](mass_t entry) { return weigh(logit_of((unsigned) (entry >> 32))); };
 
@@ -351,13 +367,13 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
                 counts[threadIdx.x] = 0;
             }
             __syncthreads();
-            each([&](int i, const Vec<F16> &v) {
+            each([&](int i, const Group &g) {
 #pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const unsigned key = key_of(v.x[e]);
-                    if (v.x[e] == -INFINITY || !stays(key, i + e) || (shift < 24 && (key >> (shift + 8)) != prefix)) continue;
+                for (int e = 0; e < GROUP; e++) {
+                    const unsigned key = key_of(g.x[e]);
+                    if (g.x[e] == -INFINITY || !stays(key, i + e) || (shift < 24 && (key >> (shift + 8)) != prefix)) continue;
                     atomicAdd(&counts[(key >> shift) & 255], 1u);
-                    if (by_mass) atomicAdd(&masses[(key >> shift) & 255], weigh(v.x[e]));
+                    if (by_mass) atomicAdd(&masses[(key >> shift) & 255], weigh(g.x[e]));
                 }
             });
             __syncthreads();
@@ -394,9 +410,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
             else few = middle + 1;
         }
         int mine = 0;
-        each([&](int i, const Vec<F16> &v) {
+        each([&](int i, const Group &g) {
 #pragma unroll
-            for (int e = 0; e < N; e++) mine += key_of(v.x[e]) == prefix && stays(prefix, i + e);
+            for (int e = 0; e < GROUP; e++) mine += key_of(g.x[e]) == prefix && stays(prefix, i + e);
         });
         __syncthreads();
         mine = (int) wave_sum((mass_t) mine);
@@ -406,9 +422,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         int before = 0;
         for (int w = 0; w < wave; w++) before += (int) sh.wave_mass[w];
         if (before < (int) most && (int) most <= before + mine) {  // in this wave's part
-            for (int i0 = begin * N; i0 < end * N; i0 += 64) {
+            for (int i0 = begin * GROUP; i0 < end * GROUP; i0 += 64) {
                 const int i = i0 + lane;
-                const bool hit = i < min(end * N, p.vocab) && key_of(load_one<F16>(row, i)) == prefix && stays(prefix, i);
+                const bool hit = i < min(end * GROUP, p.vocab) && key_of(load_one<F16>(row, i)) == prefix && stays(prefix, i);
                 const unsigned long long hits = __ballot(hit);
                 if (before + __popcll(hits) >= (int) most) {
                     if (hit && before + __popcll(hits & ((2ull << lane) - 1)) == (int) most) sh.last_index = i;
@@ -419,7 +435,73 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         }
         __syncthreads();
     };
-    // ---- the filters, counts and then masses (one loop, so that each piece of code is there once)
+
+    // ---- top_k from the group maxima: a list, in falling order for the filters, in the order of the indices for the draw
+    const bool few = k > 0 && k < p.vocab && k <= LISTED / 2;
+    if (few && spread && has_maxima) {
+        for (int n = threadIdx.x; n < groups; n += THREADS) {
+            const unsigned b = bucket_of((float) maxima[n]);
+            if (b < BUCKETS) atomicAdd((unsigned *) &sh.hist[b], 1u);
+        }
+        find_bucket(false, (mass_t) k);
+        // (fewer groups than k: the bucket behind the last, what lies there has no weight)
+        const unsigned bucket = min(sh.bucket, BUCKETS - 1);
+        for (int n = threadIdx.x; n < groups; n += THREADS) {
+            if (bucket_of((float) maxima[n]) > bucket) continue;
+            const Group g = unpack<F16>(group_at(n));
+#pragma unroll
+            for (int e = 0; e < GROUP; e++)
+                if (bucket_of(g.x[e]) <= bucket) append(key_of(g.x[e]), n * GROUP + e);
+        }
+        __syncthreads();
+        const int count = sh.list_count, most = min(k, count);
+        if (count <= LISTED) {
+            sort_list(sh.list, count, false);
+            mass_t entry[2], w[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int i = 2 * (int) threadIdx.x + e;
+                entry[e] = i < most ? sh.list[i] : 0;
+                w[e] = i < most ? mass_of_entry(entry[e]) : 0;
+            }
+            mass_t with = block_scan(w[0] + w[1], sh.wave_mass), all = 0;
+            for (int i = 0; i < NWAVES; i++) all += sh.wave_mass[i];
+            mass_t before = with - w[0] - w[1];
+            const mass_t need = top_p < 1.0f ? max((mass_t) __builtin_ceil(mass_wanted * (double) all), 1ull) : ~0ull;
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int i = 2 * (int) threadIdx.x + e;
+                const float x = logit_of((unsigned) (entry[e] >> 32));
+                const bool kept = i < most && before < need && (x == top || weigh.real(x) >= min_w);
+                before += w[e];
+                // index first now; what does not stay goes to the end
+                if (i < count) sh.list[i] = kept ? (mass_t) ~(unsigned) entry[e] << 32 | (entry[e] >> 32) : ~0ull;
+            }
+            sort_list(sh.list, count, true);
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int i = 2 * (int) threadIdx.x + e;
+                entry[e] = i < count ? sh.list[i] : ~0ull;
+                w[e] = entry[e] == ~0ull ? 0 : weigh(logit_of((unsigned) entry[e]));
+            }
+            with = block_scan(w[0] + w[1], sh.wave_mass);
+            mass_t total = 0;
+            for (int i = 0; i < NWAVES; i++) total += sh.wave_mass[i];
+            const mass_t target = target_of(p.uniform[r], total);
+            before = with - w[0] - w[1];
+            if (before <= target && target < with) {
+                const int e = target < before + w[0] ? 0 : 1;
+                p.tokens[r] = (int) ((e ? entry[1] : entry[0]) >> 32);
+                if (p.probabilities) p.probabilities[r] = (float) ((double) (e ? w[1] : w[0]) / (double) total);
+            }
+            return;
+        }
+    }
+
+    // ---- otherwise: counts and then masses (one loop, so that each piece of code is there once), each a threshold
+    if (threadIdx.x < NWAVES) sh.part_mass[threadIdx.x] = 0;
+    bool masses_known = false;  // whether sh.part_mass holds the masses of the waves' parts
 #pragma unroll 1
     for (int filter = 0; filter < 2; filter++) {
         const bool by_mass = filter == 1;
@@ -427,57 +509,64 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         mass_t need = (mass_t) k;
         bool found = false;
         if (spread) {
-            fill_hist(by_mass);
+            clear_hist();
+            each([&](int i, const Group &g) {
+#pragma unroll
+                for (int e = 0; e < GROUP; e++) {
+                    const unsigned b = bucket_of(g.x[e]);
+                    if (b >= BUCKETS || (restricted && !stays(key_of(g.x[e]), i + e))) continue;
+                    if (by_mass) atomicAdd(&sh.hist[b], weigh.near(g.x[e]));
+                    else atomicAdd((unsigned *) &sh.hist[b], 1u);
+                }
+            });
             need = find_bucket(by_mass, need);
-            const int bucket = sh.bucket;
+            const unsigned bucket = sh.bucket;
             const mass_t above = sh.above;
             if (bucket == BUCKETS) continue;  // everything that weighs anything stays
-            if (!by_mass && above + sh.hist[bucket] <= LISTED) {
-                // ---- few tokens: a list, in falling order for the filters, in the order of the indices for the draw
-                gather(0, (unsigned) bucket);
-                const int count = sh.list_count, most = min(k, count);
-                sort_list(sh.list, count, false);
-                mass_t entry[2], w[2];
+            // the tokens of the bucket into the list; with masses, the masses of what lies above it into the parts' (queued in
+            // LDS until there are 64: a wave would otherwise weigh 64 for the sake of some)
+            mass_t mass = 0;
+            int queued = 0;
+            float *queue = sh.queue[wave];
+            auto kept = [&](float x) -> mass_t {
+                const double w = weigh.near_real(x);
+                return w >= min_w || x == top ? Weigher::whole(w) : 0;
+            };
+            for (int n0 = begin; n0 < end; n0 += 64) {
+                const int n = n0 + lane;
+                const bool live = n < end && (!has_maxima || bucket_of((float) maxima[n]) <= bucket);
+                if (!__any(live)) continue;
+                Group g;
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int i = 2 * (int) threadIdx.x + e;
-                    entry[e] = i < most ? sh.list[i] : 0;
-                    w[e] = i < most ? mass_of_entry(entry[e]) : 0;
-                }
-                mass_t with = block_scan(w[0] + w[1], sh.wave_mass), all = 0;
-                for (int i = 0; i < NWAVES; i++) all += sh.wave_mass[i];
-                mass_t before = with - w[0] - w[1];
-                const mass_t need = top_p < 1.0f ? max((mass_t) __builtin_ceil(mass_wanted * (double) all), 1ull) : ~0ull;
-                __syncthreads();
+                for (int e = 0; e < GROUP; e++) g.x[e] = -INFINITY;
+                if (live) g = unpack<F16>(group_at(n));
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int i = 2 * (int) threadIdx.x + e;
-                    const float x = logit_of((unsigned) (entry[e] >> 32));
-                    const bool kept = i < most && before < need && (x == top || weigh.real(x) >= min_w);
-                    before += w[e];
-                    // index first now; what does not stay goes to the end
-                    if (i < count) sh.list[i] = kept ? (mass_t) ~(unsigned) entry[e] << 32 | (entry[e] >> 32) : ~0ull;
+                for (int e = 0; e < GROUP; e++) {
+                    const unsigned b = bucket_of(g.x[e]);
+                    const bool inside = b <= bucket && (!restricted || stays(key_of(g.x[e]), n * GROUP + e));
+                    if (inside && b == bucket) append(key_of(g.x[e]), n * GROUP + e);
+                    if (!by_mass) continue;
+                    const bool hit = inside && b < bucket;
+                    const unsigned long long hits = __ballot(hit);
+                    if (hit) queue[queued + __popcll(hits & ((1ull << lane) - 1))] = g.x[e];
+                    queued += __popcll(hits);
+                    if (queued >= 64) {
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        mass += kept(queue[lane]);
+                        const float rest = queue[64 + lane];
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        queue[lane] = rest;
+                        queued -= 64;
+                    }
                 }
-                sort_list(sh.list, count, true);
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int i = 2 * (int) threadIdx.x + e;
-                    entry[e] = i < count ? sh.list[i] : ~0ull;
-                    w[e] = entry[e] == ~0ull ? 0 : weigh(logit_of((unsigned) entry[e]));
-                }
-                with = block_scan(w[0] + w[1], sh.wave_mass);
-                mass_t total = 0;
-                for (int i = 0; i < NWAVES; i++) total += sh.wave_mass[i];
-                const mass_t target = target_of(p.uniform[r], total);
-                before = with - w[0] - w[1];
-                if (before <= target && target < with) {
-                    const int e = target < before + w[0] ? 0 : 1;
-                    p.tokens[r] = (int) ((e ? entry[1] : entry[0]) >> 32);
-                    if (p.probabilities) p.probabilities[r] = (float) ((double) (e ? w[1] : w[0]) / (double) total);
-                }
-                return;
             }
-            gather((unsigned) bucket, (unsigned) bucket);
+            if (by_mass) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                if (lane < queued) mass += kept(queue[lane]);
+                mass = wave_sum(mass);
+                if (lane == 0) atomicAdd(&sh.part_mass[wave], mass);
+            }
+            __syncthreads();
             const int count = sh.list_count;
             if (count <= LISTED) {
                 found = true;
@@ -489,20 +578,32 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
                     entry[e] = i < count ? sh.list[i] : 0;
                     w[e] = i >= count ? 0 : by_mass ? mass_of_entry(entry[e]) : 1;
                 }
-                const mass_t with = above + block_scan(w[0] + w[1], sh.wave_mass), before = with - w[0] - w[1];
-                if (before < need && need <= with) {
-                    const mass_t last = need <= before + w[0] ? entry[0] : entry[1];
-                    sh.last_key = (unsigned) (last >> 32);
-                    sh.last_index = (int) ~(unsigned) last;
+                const mass_t with = above + block_scan(w[0] + w[1], sh.wave_mass);
+                mass_t before = with - w[0] - w[1];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    if (before < need) {  // stays
+                        if (by_mass && 2 * (int) threadIdx.x + e < count) {
+                            const int i = (int) ~(unsigned) entry[e];
+                            const mass_t own = kept(logit_of((unsigned) (entry[e] >> 32)));
+                            if (own) atomicAdd(&sh.part_mass[i / (part * GROUP)], own);
+                        }
+                        if (need <= before + w[e]) {
+                            sh.last_key = (unsigned) (entry[e] >> 32);
+                            sh.last_index = (int) ~(unsigned) entry[e];
+                        }
+                    }
+                    before += w[e];
                 }
+                masses_known = by_mass;
                 __syncthreads();
             }
         } else if (by_mass) {
             mass_t mass = 0;
-            each([&](int i, const Vec<F16> &v) {
+            each([&](int i, const Group &g) {
 #pragma unroll
-                for (int e = 0; e < N; e++)
-                    if (stays(key_of(v.x[e]), i + e)) mass += weigh(v.x[e]);
+                for (int e = 0; e < GROUP; e++)
+                    if (stays(key_of(g.x[e]), i + e)) mass += weigh(g.x[e]);
             });
             mass = wave_sum(mass);
             __syncthreads();
@@ -518,55 +619,30 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         restricted = true;
     }
 
-    auto part_masses = [&] {  // sh.wave_mass: the masses of the waves' parts
-        // The tokens that stay are queued in LDS until there are 64 of them: where few of them stay, a wave would
-        // otherwise weigh 64 for the sake of some.
-        mass_t mass = 0;
-        int queued = 0;
-        float *queue = sh.queue[wave];
-        auto kept = [&](float x) -> mass_t {
-            const double w = weigh.real(x);
-            return w >= min_w || x == top ? Weigher::whole(w) : 0;
-        };
-        each_in_step([&](int i, const Vec<F16> &v, bool live) {
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const bool hit = live && v.x[e] > -INFINITY && (!restricted || stays(key_of(v.x[e]), i + e));
-                const unsigned long long hits = __ballot(hit);
-                if (hit) queue[queued + __popcll(hits & ((1ull << lane) - 1))] = v.x[e];
-                queued += __popcll(hits);
-                if (queued >= 64) {
-                    __builtin_amdgcn_wave_barrier();
-                    mass += kept(queue[lane]);
-                    const float rest = queue[64 + lane];
-                    __builtin_amdgcn_wave_barrier();
-                    queue[lane] = rest;
-                    queued -= 64;
-                }
-            }
-        });
-        __builtin_amdgcn_wave_barrier();
-        if (lane < queued) mass += kept(queue[lane]);
-        mass = wave_sum(mass);
-        __syncthreads();
-        if (lane == 0) sh.wave_mass[wave] = mass;
-        __syncthreads();
-    };
-    // ---- the draw
-    part_masses();
-    mass_t total = 0;
-    for (int w = 0; w < NWAVES; w++) total += sh.wave_mass[w];
-    const mass_t target = target_of(p.uniform[r], total);
-    int chosen = 0;
-    mass_t before = 0;
-    while (chosen < NWAVES - 1 && before + sh.wave_mass[chosen] <= target) before += sh.wave_mass[chosen++];
-    // the part that holds the target, shared by all threads
+    // ---- the draw: the wave whose part holds the target, then the place in that part
     auto weight_of = [&](float x, int i) -> mass_t {
         if (x == -INFINITY || !stays(key_of(x), i)) return 0;
         const double w = weigh.real(x);
         return w >= min_w || x == top ? Weigher::whole(w) : 0;
     };
-    const int from = chosen * part * N, to = min(from + part * N, p.vocab), per = (to - from + THREADS - 1) / THREADS;
+    if (!masses_known) {
+        mass_t mass = 0;
+        each([&](int i, const Group &g) {
+#pragma unroll
+            for (int e = 0; e < GROUP; e++) mass += weight_of(g.x[e], i + e);
+        });
+        mass = wave_sum(mass);
+        __syncthreads();
+        if (lane == 0) sh.part_mass[wave] = mass;
+    }
+    __syncthreads();
+    mass_t total = 0;
+    for (int w = 0; w < NWAVES; w++) total += sh.part_mass[w];
+    const mass_t target = target_of(p.uniform[r], total);
+    int chosen = 0;
+    mass_t before = 0;
+    while (chosen < NWAVES - 1 && before + sh.part_mass[chosen] <= target) before += sh.part_mass[chosen++];
+    const int from = chosen * part * GROUP, to = min(from + part * GROUP, p.vocab), per = (to - from + THREADS - 1) / THREADS;
     const int mine = min(from + (int) threadIdx.x * per, to), mine_end = min(mine + per, to);
     mass_t mass = 0;
     for (int i = mine; i < mine_end; i++) mass += weight_of(load_one<F16>(row, i), i);
