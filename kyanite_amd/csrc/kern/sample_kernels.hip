@@ -6,7 +6,7 @@
 //
 // A row belongs to one workgroup of 16 waves, each of which owns a contiguous part of it. What bounds a row is the arithmetic
 // per logit of one compute unit, and the fetch rate of one (about 40 GB/s) for rows that do not fit LDS. So a row is read
-// once where it fits (f16: 53000 logits), and the maxima of its groups of 8 logits are kept beside it, so that later passes
+// once where it fits (f16: 51200 logits), and the maxima of its groups of 8 logits are kept beside it, so that later passes
 // touch only groups that can matter. The filters end in one threshold, the last token that stays in the order of falling
 // logits (ties: rising index):
 //   top_k   the group maxima go into a histogram over the distance to the largest. The bucket that holds the k-th largest of
@@ -30,7 +30,7 @@ namespace {
 
 constexpr int THREADS = 1024, NWAVES = THREADS / 64;
 constexpr int BUCKETS = 2 * THREADS, LISTED = 2 * THREADS;
-constexpr int CACHE_BYTES = 104 * 1024, CACHED_MAXIMA_BYTES = CACHE_BYTES / 8, MAXIMA_BYTES = 112 * 1024;
+constexpr int CACHE_BYTES = 100 * 1024, CACHED_MAXIMA_BYTES = CACHE_BYTES / 8, MAXIMA_BYTES = 108 * 1024;
 
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 typedef _Float16 halfx8_any __attribute__((ext_vector_type(8), aligned(2)));
@@ -143,7 +143,8 @@ struct Shared {
     double roots[64];
     mass_t wave_mass[NWAVES], part_mass[NWAVES];
     float wave_top[NWAVES];
-    int list_count, bucket;
+    int list_count, bucket, place;
+    unsigned short places[LISTED];
     mass_t above;
     unsigned last_key;  // the threshold: the last token that stays
     int last_index;
@@ -327,13 +328,13 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         __syncthreads();
     };
     // sh.bucket, sh.above: the first bucket at whose end `need` is reached, and what lies before it; BUCKETS when it never is.
-    // Masses: `need` is mass_wanted of all. Returns `need`.
-    auto find_bucket = [&](bool by_mass, mass_t need) {
+    // With `share`, `need` is mass_wanted of all. Returns `need`.
+    auto find_bucket = [&](bool share, mass_t need) {
         __syncthreads();
         // a thread takes two neighbouring buckets
         const mass_t a = sh.hist[2 * threadIdx.x], both = a + sh.hist[2 * threadIdx.x + 1];
         const mass_t sums = block_scan(both, sh.wave_mass), before = sums - both;
-        if (by_mass) {
+        if (share) {
             mass_t all = 0;
             for (int w = 0; w < NWAVES; w++) all += sh.wave_mass[w];
             need = (mass_t) __builtin_ceil(mass_wanted * (double) all);
@@ -454,48 +455,79 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
                 if (bucket_of(g.x[e]) <= bucket) append(key_of(g.x[e]), n * GROUP + e);
         }
         __syncthreads();
-        const int count = sh.list_count, most = min(k, count);
+        const int count = sh.list_count;
         if (count <= LISTED) {
-            sort_list(sh.list, count, false);
-            mass_t entry[2], w[2];
+            // A thread keeps two entries. Three times a histogram of what stays of the list finds the entry at which something is
+            // reached: top_k tokens and top_p of the mass in the order of the logits, the target of the draw in the order of
+            // the indices. The entries of the bucket where that is are compared with each other.
+            mass_t entry[2], w[2], total = 0;
+            bool kept[2];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const int i = 2 * (int) threadIdx.x + e;
-                entry[e] = i < most ? sh.list[i] : 0;
-                w[e] = i < most ? mass_of_entry(entry[e]) : 0;
+                const int i = (int) threadIdx.x + THREADS * e;
+                kept[e] = i < count;
+                entry[e] = kept[e] ? sh.list[i] : 0;
+                w[e] = kept[e] ? mass_of_entry(entry[e]) : 0;
             }
-            mass_t with = block_scan(w[0] + w[1], sh.wave_mass), all = 0;
-            for (int i = 0; i < NWAVES; i++) all += sh.wave_mass[i];
-            mass_t before = with - w[0] - w[1];
-            const mass_t need = top_p < 1.0f ? max((mass_t) __builtin_ceil(mass_wanted * (double) all), 1ull) : ~0ull;
-            __syncthreads();
+            int shift = 0;
+            while ((p.vocab >> shift) >= BUCKETS) shift++;
+#pragma unroll 1
+            for (int what = 0; what < 3; what++) {
+                if (what == 0 ? count <= k : what == 1 ? !(top_p < 1.0f) : false) continue;
+                mass_t need = (mass_t) k;
+                if (what == 2) {
+                    mass_t mine = 0;
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int i = 2 * (int) threadIdx.x + e;
-                const float x = logit_of((unsigned) (entry[e] >> 32));
-                const bool kept = i < most && before < need && (x == top || weigh.real(x) >= min_w);
-                before += w[e];
-                // index first now; what does not stay goes to the end
-                if (i < count) sh.list[i] = kept ? (mass_t) ~(unsigned) entry[e] << 32 | (entry[e] >> 32) : ~0ull;
-            }
-            sort_list(sh.list, count, true);
+                    for (int e = 0; e < 2; e++) {
+                        const float x = logit_of((unsigned) (entry[e] >> 32));
+                        kept[e] = kept[e] && (x == top || weigh.real(x) >= min_w);
+                        if (kept[e]) mine += w[e];
+                    }
+                    (void) block_scan(mine, sh.wave_mass);
+                    for (int i = 0; i < NWAVES; i++) total += sh.wave_mass[i];
+                    need = target_of(p.uniform[r], total) + 1;
+                }
+                clear_hist();
+                unsigned b[2];
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int i = 2 * (int) threadIdx.x + e;
-                entry[e] = i < count ? sh.list[i] : ~0ull;
-                w[e] = entry[e] == ~0ull ? 0 : weigh(logit_of((unsigned) entry[e]));
+                for (int e = 0; e < 2; e++) {
+                    b[e] = what == 2 ? ~(unsigned) entry[e] >> shift : min(bucket_of(logit_of((unsigned) (entry[e] >> 32))), BUCKETS - 1u);
+                    if (kept[e]) atomicAdd(&sh.hist[b[e]], what == 0 ? 1ull : w[e]);
+                }
+                need = find_bucket(what == 1, need);
+                const unsigned bucket = sh.bucket;
+                const mass_t above = sh.above;
+                // (the histogram has been read: its room holds what the bucket's entries count)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (kept[e] && b[e] == bucket) {
+                        const int c = atomicAdd(&sh.list_count, 1);
+                        sh.places[c] = (unsigned short) (threadIdx.x + THREADS * e);
+                        sh.hist[c] = what == 0 ? 1ull : w[e];
+                    }
+                __syncthreads();
+                const int inside = sh.list_count;
+                for (int c = threadIdx.x; c < inside; c += THREADS) {
+                    const mass_t own = sh.list[sh.places[c]];
+                    mass_t before = above;
+                    for (int o = 0; o < inside; o++) {
+                        const mass_t other = sh.list[sh.places[o]];
+                        if (what == 2 ? ~(unsigned) other < ~(unsigned) own : other > own) before += sh.hist[o];
+                    }
+                    if (before < need && need <= before + sh.hist[c]) sh.place = sh.places[c];
+                }
+                __syncthreads();
+                const mass_t last = sh.list[sh.place];
+                if (what == 2) {
+                    if (threadIdx.x == 0) {
+                        p.tokens[r] = (int) ~(unsigned) last;
+                        if (p.probabilities) p.probabilities[r] = (float) ((double) mass_of_entry(last) / (double) total);
+                    }
+                    return;
+                }
+#pragma unroll
+                for (int e = 0; e < 2; e++) kept[e] = kept[e] && entry[e] >= last;
             }
-            with = block_scan(w[0] + w[1], sh.wave_mass);
-            mass_t total = 0;
-            for (int i = 0; i < NWAVES; i++) total += sh.wave_mass[i];
-            const mass_t target = target_of(p.uniform[r], total);
-            before = with - w[0] - w[1];
-            if (before <= target && target < with) {
-                const int e = target < before + w[0] ? 0 : 1;
-                p.tokens[r] = (int) ((e ? entry[1] : entry[0]) >> 32);
-                if (p.probabilities) p.probabilities[r] = (float) ((double) (e ? w[1] : w[0]) / (double) total);
-            }
-            return;
         }
     }
 
@@ -510,13 +542,28 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         bool found = false;
         if (spread) {
             clear_hist();
+            // (all weights first, then the atomics: branches in between would leave the reads of the table waiting one by one)
             each([&](int i, const Group &g) {
+                unsigned b[GROUP];
 #pragma unroll
                 for (int e = 0; e < GROUP; e++) {
-                    const unsigned b = bucket_of(g.x[e]);
-                    if (b >= BUCKETS || (restricted && !stays(key_of(g.x[e]), i + e))) continue;
-                    if (by_mass) atomicAdd(&sh.hist[b], weigh.near(g.x[e]));
-                    else atomicAdd((unsigned *) &sh.hist[b], 1u);
+                    b[e] = bucket_of(g.x[e]);
+                    if (restricted && !stays(key_of(g.x[e]), i + e)) b[e] = BUCKETS;
+                }
+                if (by_mass) {
+#pragma unroll
+                    for (int half = 0; half < GROUP; half += 4) {
+                        mass_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) w[e] = weigh.near(g.x[half + e]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (b[half + e] < BUCKETS) atomicAdd(&sh.hist[b[half + e]], w[e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < GROUP; e++)
+                        if (b[e] < BUCKETS) atomicAdd((unsigned *) &sh.hist[b[e]], 1u);
                 }
             });
             need = find_bucket(by_mass, need);
