@@ -6,7 +6,7 @@
 //
 // A row belongs to one workgroup of 16 waves, each of which owns a contiguous part of it. What bounds a row is the arithmetic
 // per logit of one compute unit, and the fetch rate of one (about 40 GB/s) for rows that do not fit LDS. So a row is read
-// once where it fits (f16: 51200 logits), and the maxima of its groups of 8 logits are kept beside it, so that later passes
+// once where it fits (f16: 53000 logits), and the maxima of its groups of 8 logits are kept beside it, so that later passes
 // touch only groups that can matter. The filters end in one threshold, the last token that stays in the order of falling
 // logits (ties: rising index):
 //   top_k   the group maxima go into a histogram over the distance to the largest. The bucket that holds the k-th largest of
@@ -30,7 +30,7 @@ namespace {
 
 constexpr int THREADS = 1024, NWAVES = THREADS / 64;
 constexpr int BUCKETS = 2 * THREADS, LISTED = 2 * THREADS;
-constexpr int CACHE_BYTES = 100 * 1024, CACHED_MAXIMA_BYTES = CACHE_BYTES / 8, MAXIMA_BYTES = 108 * 1024;
+constexpr int CACHE_BYTES = 104 * 1024, CACHED_MAXIMA_BYTES = CACHE_BYTES / 8, MAXIMA_BYTES = 112 * 1024;
 
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 typedef _Float16 halfx8_any __attribute__((ext_vector_type(8), aligned(2)));
@@ -105,24 +105,27 @@ __device__ __forceinline__ Raw<F16> load_group(const void *row, int n, int vocab
     return raw;
 }
 
-// exp((x - top) / T) 2^bits for x <= top. 2^(n / 64 + r / 64) with |r| <= 1/2: a table of 64 roots of two, and the series of
-// exp(r ln2 / 64) up to the 5th power, whose rest is below 4e-17.
+// exp((x - top) / T) 2^bits for x <= top. 2^(n / 256 + y / 256) with |y| <= 1/2: a table of 256 roots of two, and the series of
+// exp(y ln2 / 256) up to the 4th power, whose rest is below 4e-17.
+constexpr int ROOTS = 256;
 struct Weigher {
     float top;
-    double per;  // 64 log2(e) / T
+    double per;  // 256 log2(e) / T
     int bits;
     const double *roots;
-    // (exact at x = top: the argument is zero)
+    // (exact at x = top: the argument is zero; far below, the result is 0 or a positive number below 1 / 4)
     __device__ __forceinline__ double core(double t) const {
-        constexpr double L = 0.010830424696249145;  // ln(2) / 64
-        const double n = __builtin_rint(t), y = t - n;
-        const int i = (int) n;
-        const double s = __builtin_fma(y, __builtin_fma(y, __builtin_fma(y, __builtin_fma(y, __builtin_fma(y, L * L * L * L * L / 120, L * L * L * L / 24), L * L * L / 6), L * L / 2), L), 1.0);
-        return __builtin_ldexp(roots[i & 63] * s, (i >> 6) + bits);
+        constexpr double L = 0.6931471805599453 / ROOTS, MAGIC = 0x1.8p52;
+        // adding 1.5 2^52 rounds to a whole number and leaves it in the low bits
+        const double m = t + MAGIC, y = t - (m - MAGIC);
+        const int i = (int) __builtin_bit_cast(mass_t, m);
+        const double s = __builtin_fma(y, __builtin_fma(y, __builtin_fma(y, __builtin_fma(y, L * L * L * L / 24, L * L * L / 6), L * L / 2), L), 1.0);
+        const mass_t w = __builtin_bit_cast(mass_t, roots[i & (ROOTS - 1)] * s);
+        return __builtin_bit_cast(double, w + ((mass_t) (unsigned) ((i >> 8) + bits) << 52));  // (times a power of two: normal numbers)
     }
     __device__ __forceinline__ double real(float x) const {
         if (top == INFINITY || x == -INFINITY) return x == top ? __builtin_ldexp(1.0, bits) : 0.0;
-        return core(fmax(((double) x - (double) top) * per, -64.0 * 1000));
+        return core(fmax(((double) x - (double) top) * per, -ROOTS * 200.0));
     }
     // (bits <= 51: adding 2^52 rounds to a whole number and leaves it in the low bits)
     static __device__ __forceinline__ mass_t whole(double w) { return __builtin_bit_cast(mass_t, w + 0x1p52) & ((1ull << 52) - 1); }
@@ -139,8 +142,7 @@ __device__ __forceinline__ float logit_of(unsigned key) {
 struct Shared {
     mass_t hist[BUCKETS];
     mass_t list[LISTED];  // key and, below it, the complement of the index: falling order is the order of the filters
-    float queue[NWAVES][128];
-    double roots[64];
+    double roots[ROOTS];
     mass_t wave_mass[NWAVES], part_mass[NWAVES];
     float wave_top[NWAVES];
     int list_count, bucket, place;
@@ -178,13 +180,23 @@ __device__ __forceinline__ mass_t block_scan(mass_t v, mass_t *shared) {
     return v;
 }
 
-// The first `count` entries of the list into falling (or rising) order: a bitonic network, a thread per pair. Steps of 64 and
+// a place in a list for every lane that asks for one: one addition per wave
+__device__ __forceinline__ int take_places(bool live, int *count) {
+    const unsigned long long lanes = __ballot(live);
+    if (lanes == 0) return 0;
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    if (lane == 0) base = atomicAdd(count, __popcll(lanes));
+    return __builtin_amdgcn_readfirstlane(base) + __popcll(lanes & ((1ull << lane) - 1));
+}
+
+// The first `count` entries of the list into falling order: a bitonic network, a thread per pair. Steps of 64 and
 // less stay inside the 128 entries of a wave and need no barrier.
-__device__ __forceinline__ void sort_list(mass_t *list, int count, bool rising) {
+__device__ __forceinline__ void sort_list(mass_t *list, int count) {
     int size = 2;
     while (size < count) size *= 2;
     __syncthreads();
-    for (int i = count + (int) threadIdx.x; i < size; i += THREADS) list[i] = rising ? ~0ull : 0;
+    for (int i = count + (int) threadIdx.x; i < size; i += THREADS) list[i] = 0;
     __syncthreads();
     bool shared = false;  // whether other waves have written since the last barrier
     for (int run = 2; run <= size; run *= 2)
@@ -195,7 +207,7 @@ __device__ __forceinline__ void sort_list(mass_t *list, int count, bool rising) 
             if ((int) threadIdx.x < size / 2) {
                 const int i = 2 * (int) threadIdx.x - ((int) threadIdx.x & (step - 1)), j = i + step;
                 const mass_t a = list[i], b = list[j];
-                const bool up = rising == ((i & run) == 0);
+                const bool up = (i & run) != 0;
                 if (up ? a > b : a < b) {
                     list[i] = b;
                     list[j] = a;
@@ -222,6 +234,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     const int groups = (p.vocab + GROUP - 1) / GROUP, part = (groups + NWAVES - 1) / NWAVES;
     const int begin = min(wave * part, groups), end = min(begin + part, groups);  // of this wave, in groups
     const bool has_maxima = CACHED || groups <= MAXIMA;
+    auto logit_at = [&](int i) { return CACHED ? load_one<F16>(cache, i) : load_one<F16>(row, i); };
     auto group_at = [&](int n) { return CACHED ? cache[n] : load_group<F16>(row, n, p.vocab); };
 
     // f(first index, logits) for the groups of this wave
@@ -263,7 +276,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
         if (lane == 0) sh.wave_top[wave] = top;
-        if (threadIdx.x < 64) sh.roots[threadIdx.x] = exp2(threadIdx.x * (1.0 / 64));
+        if (threadIdx.x < ROOTS) sh.roots[threadIdx.x] = exp2(threadIdx.x * (1.0 / ROOTS));
         for (int b = threadIdx.x; b < BUCKETS; b += THREADS) sh.hist[b] = 0;
         if (threadIdx.x == 0) {
             sh.list_count = 0;
@@ -303,7 +316,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         }
         return;
     }
-    const Weigher weigh{top, 92.332482616893656877 / (double) t, p.bits, sh.roots};
+    const Weigher weigh{top, 369.32993046757462751 / (double) t, p.bits, sh.roots};
     const int k = p.top_k ? p.top_k[r] : 0;
     const float top_p = p.top_p ? p.top_p[r] : 1.0f;
     const double min_w = p.min_p ? __builtin_ldexp((double) p.min_p[r], p.bits) : 0.0;
@@ -447,15 +460,27 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         find_bucket(false, (mass_t) k);
         // (fewer groups than k: the bucket behind the last, what lies there has no weight)
         const unsigned bucket = min(sh.bucket, BUCKETS - 1);
-        for (int n = threadIdx.x; n < groups; n += THREADS) {
-            if (bucket_of((float) maxima[n]) > bucket) continue;
-            const Group g = unpack<F16>(group_at(n));
-#pragma unroll
-            for (int e = 0; e < GROUP; e++)
-                if (bucket_of(g.x[e]) <= bucket) append(key_of(g.x[e]), n * GROUP + e);
+        // the groups that reach it, then, a thread per logit, their logits; places in the lists are taken by whole waves
+        for (int n0 = 0; n0 < groups; n0 += THREADS) {
+            const int n = n0 + (int) threadIdx.x;
+            const bool live = n < groups && bucket_of((float) maxima[n]) <= bucket;
+            const int c = take_places(live, &sh.list_count);
+            if (live && c < LISTED) sh.places[c] = (unsigned short) n;
+        }
+        if (threadIdx.x == 0) sh.place = 0;
+        __syncthreads();
+        const int reaching = sh.list_count;
+        if (reaching <= LISTED) {
+            for (int n0 = 0; n0 < reaching * GROUP; n0 += THREADS) {
+                const int n = n0 + (int) threadIdx.x, i = n < reaching * GROUP ? sh.places[n / GROUP] * GROUP + n % GROUP : p.vocab;
+                const float x = i < p.vocab ? logit_at(i) : -INFINITY;
+                const bool live = bucket_of(x) <= bucket;
+                const int c = take_places(live, &sh.place);
+                if (live && c < LISTED) sh.list[c] = (mass_t) key_of(x) << 32 | ~(unsigned) i;
+            }
         }
         __syncthreads();
-        const int count = sh.list_count;
+        const int count = reaching <= LISTED ? sh.place : LISTED + 1;
         if (count <= LISTED) {
             // A thread keeps two entries. Three times a histogram of what stays of the list finds the entry at which something is
             // reached: top_k tokens and top_p of the mass in the order of the logits, the target of the draw in the order of
@@ -570,18 +595,32 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
             const unsigned bucket = sh.bucket;
             const mass_t above = sh.above;
             if (bucket == BUCKETS) continue;  // everything that weighs anything stays
-            // the tokens of the bucket into the list; with masses, the masses of what lies above it into the parts' (queued in
-            // LDS until there are 64: a wave would otherwise weigh 64 for the sake of some)
+            // The tokens of the bucket go into the list; with masses, the masses of what lies above it into the parts'. Where few
+            // tokens lie so high, a wave would weigh 64 for the sake of some: they are queued until there are 64 of them, in
+            // the room of the histogram, which has been read.
             mass_t mass = 0;
             int queued = 0;
-            float *queue = sh.queue[wave];
+            mass_t *queue = sh.hist + 128 * wave;
             auto kept = [&](float x) -> mass_t {
                 const double w = weigh.near_real(x);
                 return w >= min_w || x == top ? Weigher::whole(w) : 0;
             };
+            auto settle = [&](mass_t item) {
+                const float x = __builtin_bit_cast(float, (unsigned) (item >> 32));
+                const int i = (int) (unsigned) item;
+                const unsigned b = bucket_of(x);
+                if (b > bucket || (restricted && !stays(key_of(x), i))) return;
+                if (b < bucket) {
+                    if (by_mass) mass += kept(x);
+                } else {
+                    append(key_of(x), i);
+                }
+            };
+            // (one comparison per logit: buckets are a little wider here)
+            const float lowest = top - ((float) bucket + 2.0f) / per_bucket;
             for (int n0 = begin; n0 < end; n0 += 64) {
                 const int n = n0 + lane;
-                const bool live = n < end && (!has_maxima || bucket_of((float) maxima[n]) <= bucket);
+                const bool live = n < end && (!has_maxima || (float) maxima[n] >= lowest);
                 if (!__any(live)) continue;
                 Group g;
 #pragma unroll
@@ -589,27 +628,23 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
                 if (live) g = unpack<F16>(group_at(n));
 #pragma unroll
                 for (int e = 0; e < GROUP; e++) {
-                    const unsigned b = bucket_of(g.x[e]);
-                    const bool inside = b <= bucket && (!restricted || stays(key_of(g.x[e]), n * GROUP + e));
-                    if (inside && b == bucket) append(key_of(g.x[e]), n * GROUP + e);
-                    if (!by_mass) continue;
-                    const bool hit = inside && b < bucket;
+                    const bool hit = live && g.x[e] >= lowest;
                     const unsigned long long hits = __ballot(hit);
-                    if (hit) queue[queued + __popcll(hits & ((1ull << lane) - 1))] = g.x[e];
+                    if (hit) queue[queued + __popcll(hits & ((1ull << lane) - 1))] = (mass_t) __builtin_bit_cast(unsigned, g.x[e]) << 32 | (unsigned) (n * GROUP + e);
                     queued += __popcll(hits);
                     if (queued >= 64) {
                         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                        mass += kept(queue[lane]);
-                        const float rest = queue[64 + lane];
+                        settle(queue[lane]);
+                        const mass_t rest = queue[64 + lane];
                         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                         queue[lane] = rest;
                         queued -= 64;
                     }
                 }
             }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (lane < queued) settle(queue[lane]);
             if (by_mass) {
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                if (lane < queued) mass += kept(queue[lane]);
                 mass = wave_sum(mass);
                 if (lane == 0) atomicAdd(&sh.part_mass[wave], mass);
             }
@@ -617,7 +652,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
             const int count = sh.list_count;
             if (count <= LISTED) {
                 found = true;
-                sort_list(sh.list, count, false);
+                sort_list(sh.list, count);
                 mass_t entry[2], w[2];
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
@@ -625,19 +660,19 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
                     entry[e] = i < count ? sh.list[i] : 0;
                     w[e] = i >= count ? 0 : by_mass ? mass_of_entry(entry[e]) : 1;
                 }
-                const mass_t with = above + block_scan(w[0] + w[1], sh.wave_mass);
-                mass_t before = with - w[0] - w[1];
+                // what of the bucket stays: the threshold is the last token before which less than `need` lies
+                mass_t before = above + block_scan(w[0] + w[1], sh.wave_mass) - w[0] - w[1];
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    if (before < need) {  // stays
-                        if (by_mass && 2 * (int) threadIdx.x + e < count) {
-                            const int i = (int) ~(unsigned) entry[e];
+                    const int i = (int) ~(unsigned) entry[e];
+                    if (before < need && 2 * (int) threadIdx.x + e < count) {
+                        if (by_mass) {
                             const mass_t own = kept(logit_of((unsigned) (entry[e] >> 32)));
                             if (own) atomicAdd(&sh.part_mass[i / (part * GROUP)], own);
                         }
                         if (need <= before + w[e]) {
                             sh.last_key = (unsigned) (entry[e] >> 32);
-                            sh.last_index = (int) ~(unsigned) entry[e];
+                            sh.last_index = i;
                         }
                     }
                     before += w[e];
