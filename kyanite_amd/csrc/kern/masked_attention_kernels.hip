@@ -1065,11 +1065,11 @@ __global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))
 // ---- parts -> results ----------------------------------------------------------------------------------------------
 
 // A wave per row of the result. WP / 4 lanes take a part's row, 16 bytes each, so that a wave reads 2 (4) parts at a time; up
-// to 32 parts are in flight together, requested before their weights are known. Bound by the parts: they come out of the
-// caches of other XCDs.
-template <int WP>
+// to PARTS (8 or 32) are in flight together, requested before their weights are known. Bound by the parts: they come out of the
+// caches of other XCDs. (32 in flight where there are two parts: 59 us instead of 43 for a prompt of 1024 tokens.)
+template <int WP, int PARTS>
 __global__ __launch_bounds__(64 * WAVES) void join_attention_kernel(ServingAttentionParams p) {
-    constexpr int LANES = WP / 4, SIDE = 64 / LANES, AHEAD = 32 / SIDE;
+    constexpr int LANES = WP / 4, SIDE = 64 / LANES, AHEAD = PARTS / SIDE;
     const int lane = threadIdx.x & 63, side = lane / LANES, d = 4 * (lane % LANES);
     const unsigned row = __builtin_amdgcn_readfirstlane(blockIdx.x * WAVES + (threadIdx.x >> 6));
     if (row >= (unsigned) p.batch * p.queries * p.heads) return;
@@ -1106,8 +1106,8 @@ __global__ __launch_bounds__(64 * WAVES) void join_attention_kernel(ServingAtten
     floatx4 x = {0, 0, 0, 0};
 #pragma unroll
     for (int s = 0; s < 2; s++)
-        for (int i0 = 0; i0 < count[s]; i0 += 32) {
-            const int n = min(32, count[s] - i0);
+        for (int i0 = 0; i0 < count[s]; i0 += PARTS) {
+            const int n = min(PARTS, count[s] - i0);
             floatx4 part[AHEAD];
 #pragma unroll
             for (int a = 0; a < AHEAD; a++) {
@@ -1159,12 +1159,25 @@ struct Plan {
     int wp;
 };
 
-// Keys are shared by several workgroups while tiles alone leave compute units idle (two workgroups fit each), down to
-// parts of four blocks: below, a part costs more to write and to join than it saves.
-int splits_for(long long workgroups, long long keys, int waves) {
-    const long long WANTED = 2048 / waves;
-    if (workgroups >= WANTED || workgroups == 0) return 1;
-    return (int) std::max(1ll, std::min((WANTED + workgroups - 1) / workgroups, keys / 256));
+// How many workgroups share the keys of a tile, by what that costs in the time of one block of keys (1.5 us with four waves on
+// a compute unit, 2.6 with eight). `longest` and `mean`: keys of a tile. The longest tile is a chain of blocks, all of
+// them together are work for 256 compute units. A part is written and read again: 5900 rows of parts cost as much as a
+// block of four waves, and the launch of the join two blocks. (One prompt of 1024 tokens and 32 heads: 33 us whole, 43
+// in two parts; of 8 heads: 32 us whole, 24 in four.)
+int splits_for(long long workgroups, long long rows, long long longest, long long mean, int waves, bool join_anyway) {
+    const long long blocks = std::max(1ll, (longest + 63) / 64);
+    int best = 1;
+    double least = 0.0;
+    for (long long s = 1; s <= blocks && (s == 1 || workgroups * s <= 512); s++) {
+        const double chain = (double) ((blocks + s - 1) / s), share = (double) mean / (double) std::max(1ll, longest);
+        const double reading = chain * std::max(1.0, share * (double) ((workgroups * s + 255) / 256));
+        const double joining = s == 1 && !join_anyway ? 0.0 : 2.0 + (double) (rows * s) * WAVES / (5900.0 * waves);
+        if (s == 1 || reading + joining < least) {
+            least = reading + joining;
+            best = (int) s;
+        }
+    }
+    return best;
 }
 
 Plan plan_for(const ServingAttentionParams &p) {
@@ -1176,15 +1189,18 @@ Plan plan_for(const ServingAttentionParams &p) {
     l.own_in_rows = p.paged && l.own_rows <= 32;
     l.prefix_in_rows = p.prefix_tokens > 0 && l.prefix_rows <= 32;
     const long long pairs = (long long) p.batch * p.kv_heads;
-    const int tile_rows = 32 * tile_waves(l.wp, p.k_scales != nullptr);
+    const int waves = tile_waves(l.wp, p.k_scales != nullptr), tile_rows = 32 * waves;
     if (!l.own_in_rows) {
         l.own_tiles = (l.own_rows + tile_rows - 1) / tile_rows;
-        l.own_splits = splits_for(l.own_tiles * pairs, p.paged ? p.table_tokens : p.keys, tile_waves(l.wp, p.k_scales != nullptr));
+        const long long keys = p.paged ? p.table_tokens : p.keys, tile_tokens = tile_rows / (p.heads / p.kv_heads) + 2;
+        const long long longest = p.window > 0 ? std::min(keys, p.window + tile_tokens) : keys;
+        const long long mean = p.paged || p.causal ? std::min(longest, std::max(keys - p.queries / 2, 1ll)) : longest;
+        l.own_splits = splits_for(l.own_tiles * pairs, pairs * l.own_rows, longest, mean, waves, p.prefix_tokens > 0);
         l.own_parts = l.own_splits * pairs * l.own_rows;
     }
     if (p.prefix_tokens > 0 && !l.prefix_in_rows) {
         l.prefix_tiles = (l.prefix_rows + tile_rows - 1) / tile_rows;
-        l.prefix_splits = splits_for(l.prefix_tiles * p.kv_heads, p.prefix_tokens, tile_waves(l.wp, p.k_scales != nullptr));
+        l.prefix_splits = splits_for(l.prefix_tiles * p.kv_heads, p.kv_heads * l.prefix_rows, p.prefix_tokens, p.prefix_tokens, waves, true);
         l.prefix_parts = (long long) l.prefix_splits * p.kv_heads * l.prefix_rows;
     }
     if (l.own_in_rows) {
@@ -1236,6 +1252,13 @@ int launch_rows_for(const ServingAttentionParams &p, unsigned workgroups, bool t
     return two_tiles ? launch_rows<WP, 2, false>(p, workgroups, with_prefix, stream) : launch_rows<WP, 1, false>(p, workgroups, with_prefix, stream);
 }
 
+template <int WP, int PARTS>
+int launch_join(const ServingAttentionParams &p, hipStream_t stream) {
+    const unsigned workgroups = (unsigned) (((long long) p.batch * p.queries * p.heads + WAVES - 1) / WAVES);
+    hipLaunchKernelGGL((join_attention_kernel<WP, PARTS>), dim3(workgroups), dim3(64 * WAVES), 0, stream, p);
+    return (int) hipGetLastError();
+}
+
 }  // namespace
 
 // partial values, then their references and sums, then the items of the row kernel
@@ -1285,10 +1308,10 @@ int launch_serving_attention(const ServingAttentionParams &given, void *workspac
     if (l.join) {
         p.part_values = values;
         p.part_stats = stats;
-        const unsigned workgroups = (unsigned) (((long long) p.batch * p.queries * p.heads + WAVES - 1) / WAVES);
-        if (l.wp == 64) hipLaunchKernelGGL(join_attention_kernel<64>, dim3(workgroups), dim3(64 * WAVES), 0, stream, p);
-        else hipLaunchKernelGGL(join_attention_kernel<128>, dim3(workgroups), dim3(64 * WAVES), 0, stream, p);
-        return (int) hipGetLastError();
+        // (which count decides only how many loads are in flight at a time: any number of parts comes out right)
+        const bool few = !l.own_in_rows && l.own_splits <= 8 && l.prefix_splits <= 8;
+        return l.wp == 64 ? few ? launch_join<64, 8>(p, stream) : launch_join<64, 32>(p, stream)
+                          : few ? launch_join<128, 8>(p, stream) : launch_join<128, 32>(p, stream);
     }
     return 0;
 }
