@@ -508,7 +508,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         if (__any(top > ref + SLACK)) {
             top = fmaxf(top, __shfl_xor(top, 32));
             const float new_ref = fmaxf(ref, top);
-            const float alpha = __builtin_amdgcn_exp2f(ref - (new_ref == -INFINITY ? 0.0f : new_ref));
+            const float alpha = ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - new_ref);  // (what is not finite may have been added)
             ref = new_ref;
             sum *= alpha;
 #pragma unroll

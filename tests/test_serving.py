@@ -167,6 +167,11 @@ def _cached_case(device, c, seed=0):
     fill(slots(prefix_table, P))
     for b, n in enumerate(lengths):
         fill(slots(tables[b], min(max(n, 0), table_pages * page)))
+    if "infinite" in c:  # (key, element) of the first sequence
+        at, d = c["infinite"]
+        k, v = cache.held(slots(tables[0], at + 1)[-1:])
+        v[..., d] = -np.inf
+        cache.put(slots(tables[0], at + 1)[-1:], k.astype(np.float16), v.astype(np.float16))
     poisoned = c.get("poison", False)  # the last token of every sequence: only its own query sees it
     if poisoned:
         for b, n in enumerate(lengths):
@@ -330,6 +335,15 @@ PROMPT_CASES = {
 }
 
 
+# (key, element, value): +inf or -inf among the values, which makes that element of all that see the key infinite
+PROMPT_INFINITE = {
+    "first_block": dict(queries=50, heads=2, kv=1, width=64, causal=True, infinite=[(0, 5, 1), (20, 9, -1), (49, 63, 1)]),
+    "later_blocks": dict(queries=300, heads=2, kv=2, width=128, causal=True, window=150, infinite=[(63, 0, 1), (64, 127, -1), (200, 64, 1)]),
+    "whole_blocks": dict(queries=64, keys=128, heads=1, kv=1, width=64, infinite=[(10, 3, 1), (100, 4, -1)]),
+    "in_parts": dict(queries=100, keys=1500, heads=1, kv=1, width=64, causal=True, infinite=[(3, 1, 1), (700, 2, -1), (1450, 3, 1)]),
+}
+
+
 def _prompt_case(device, c, seed=0):
     rng = np.random.default_rng(seed + 7)
     B, S, H, N, W = c.get("batch", 1), c["queries"], c["heads"], c["kv"], c["width"]
@@ -365,6 +379,9 @@ def _prompt_case(device, c, seed=0):
         k_mem[:, c["poison_from"]:], v_mem[:, c["poison_from"]:] = np.inf, np.nan
     if "poison_to" in c:
         k_mem[:, :c["poison_to"]], v_mem[:, :c["poison_to"]] = np.nan, -np.inf
+    for key, d, sign in c.get("infinite", ()):
+        v_mem[:, key, :, 5 + d] = sign * np.inf
+        clean_v[:, key, :, 5 + d] = 0
     slopes = np.array([2.0 ** -(1 + h % 8) for h in range(H)], np.float32) if c.get("slopes") else None
     out_mem = np.full((H, B, S, W + 3), GUARD, np.float16)
     prefix = np.array(c.get("prefix", [0]), np.int32)
@@ -394,7 +411,10 @@ def _prompt_case(device, c, seed=0):
                 out[h, b], bound[h, b] = attend(q_mem[b, h, :, :W].astype(np.float64), k, v, at, places, seen, scale, cap, slopes[h] if slopes is not None else 0.0)
         return out, bound
 
-    return dict(args=args, dev=dev, out_mem=out_mem, expected=expected, W=W, compared=compared)
+    infinite = np.zeros((H, B, S, W))
+    for key, d, sign in c.get("infinite", ()):
+        infinite[..., d] = np.where(visible[None, :, :, key], sign, 0)
+    return dict(args=args, dev=dev, out_mem=out_mem, expected=expected, W=W, compared=compared, infinite=infinite)
 
 
 @pytest.mark.gpu
@@ -411,6 +431,42 @@ def test_attention_of_prompts(name, hip_device):
         got = c["dev"][3].to_array(np.float16, c["out_mem"].shape)
         got[..., :c["W"]][:, ~c["compared"]] = 0
         _check(got, out, bound, c["W"], f"{name}, call {round_}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", PROMPT_INFINITE)
+def test_attention_of_prompts_keeps_infinities(name, hip_device):
+    c = _prompt_case(hip_device, PROMPT_INFINITE[name])
+    stream = kn.HipStream(hip_device)
+    need = kn.attention_workspace_bytes(c["args"])
+    workspace = kn.DeviceBuffer(hip_device, need) if need else None
+    out, bound = c["expected"]()
+    kn.attention(hip_device, stream, c["args"], workspace)
+    stream.synchronize()
+    got = c["dev"][3].to_array(np.float16, c["out_mem"].shape)
+    values, there = got[..., :c["W"]], c["infinite"] != 0
+    assert (values[there] == np.copysign(np.inf, c["infinite"][there])).all(), name
+    values[there] = out[there]
+    _check(got, out, bound, c["W"], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("queries,length,key", [(40, 50, 12), (40, 50, 0), (40, 300, 270), (1, 40, 39), (3, 100, 98), (3, 2500, 1200)])
+def test_cached_attention_keeps_infinities(queries, length, key, hip_device):
+    """an infinity among the values of a key: the same element of every query that sees it"""
+    c = dict(dtype=DType.F16, kv=1, group=2, width=64, page=16, lengths=[length], queries=queries)
+    finite, with_one = _cached_case(hip_device, c), _cached_case(hip_device, dict(c, infinite=(key, 7)))
+    stream = kn.HipStream(hip_device)
+    got = []
+    for case in (finite, with_one):
+        need = kn.cached_attention_workspace_bytes(case["args"])
+        kn.cached_attention(hip_device, stream, case["args"], kn.DeviceBuffer(hip_device, need) if need else None)
+        stream.synchronize()
+        got.append(case["dev"][1].to_array(np.float16, case["out_mem"].shape))
+    sees = length - queries + np.arange(queries) >= key
+    assert (got[1][:, :, sees, 7] == -np.inf).all()
+    got[1][:, :, sees, 7] = got[0][:, :, sees, 7]
+    assert np.array_equal(got[0], got[1])
 
 
 # ---- sampling ------------------------------------------------------------------------------------------------------
