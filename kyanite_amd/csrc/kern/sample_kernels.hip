@@ -29,6 +29,7 @@ namespace kn {
 namespace {
 
 constexpr int THREADS = 1024, NWAVES = THREADS / 64;
+static_assert(NWAVES == 16, "a row of lanes adds up the waves");
 constexpr int BUCKETS = 2 * THREADS, LISTED = 2 * THREADS;
 constexpr int CACHE_BYTES = 104 * 1024, CACHED_MAXIMA_BYTES = CACHE_BYTES / 8, MAXIMA_BYTES = 112 * 1024;
 
@@ -154,30 +155,49 @@ struct Shared {
     unsigned search_prefix, search_count;
 };
 
-__device__ __forceinline__ mass_t wave_scan(mass_t v, int lane) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const mass_t other = __shfl_up(v, m);
-        if (lane >= m) v += other;
-    }
-    return v;
+// v of another lane by the pattern CTRL, 0 where it has none and in rows of 16 lanes outside the mask
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ mass_t from_lane(mass_t v) {
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int) v, CTRL, ROWS, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int) (v >> 32), CTRL, ROWS, 0xf, false);
+    return (mass_t) hi << 32 | lo;
 }
 
-__device__ __forceinline__ mass_t wave_sum(mass_t v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
-    return v;
+__device__ __forceinline__ mass_t lane_of(mass_t v, int lane) {
+    return (mass_t) (unsigned) __builtin_amdgcn_readlane((int) (v >> 32), lane) << 32 | (unsigned) __builtin_amdgcn_readlane((int) v, lane);
 }
 
-// sums over the threads of the workgroup up to and with this one; `shared`: a place per wave
-__device__ __forceinline__ mass_t block_scan(mass_t v, mass_t *shared) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    v = wave_scan(v, lane);
+// sums over the lanes up to and with this one, in a row of 16 lanes and in the wave, without LDS
+__device__ __forceinline__ mass_t row_scan(mass_t v) {
+    v += from_lane<0x111>(v);  // one lane down
+    v += from_lane<0x112>(v);
+    v += from_lane<0x114>(v);
+    return v + from_lane<0x118>(v);
+}
+
+__device__ __forceinline__ mass_t wave_scan(mass_t v) {
+    v = row_scan(v);
+    v += from_lane<0x142, 0xa>(v);         // the last lane of rows 0 and 2 to rows 1 and 3
+    return v + from_lane<0x143, 0xc>(v);  // the last lane of row 1 to rows 2 and 3
+}
+
+__device__ __forceinline__ mass_t wave_sum(mass_t v) { return lane_of(wave_scan(v), 63); }
+
+// sums over the first places, one per wave, of an array in LDS
+__device__ __forceinline__ mass_t scan_of_waves(const mass_t *shared) {
+    const int lane = threadIdx.x & 63;
+    return row_scan(lane < NWAVES ? shared[lane] : 0);
+}
+
+// sums over the threads of the workgroup up to and with this one, and over all; `shared`: a place per wave
+__device__ __forceinline__ mass_t block_scan(mass_t v, mass_t *shared, mass_t *all = nullptr) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    v = wave_scan(v);
     __syncthreads();
     if (lane == 63) shared[wave] = v;
     __syncthreads();
-    for (int w = 0; w < wave; w++) v += shared[w];
-    return v;
+    const mass_t waves = scan_of_waves(shared);
+    if (all) *all = lane_of(waves, NWAVES - 1);
+    return wave ? v + lane_of(waves, wave - 1) : v;
 }
 
 // a place in a list for every lane that asks for one: one addition per wave
@@ -346,10 +366,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         __syncthreads();
         // a thread takes two neighbouring buckets
         const mass_t a = sh.hist[2 * threadIdx.x], both = a + sh.hist[2 * threadIdx.x + 1];
-        const mass_t sums = block_scan(both, sh.wave_mass), before = sums - both;
+        mass_t all;
+        const mass_t sums = block_scan(both, sh.wave_mass, &all), before = sums - both;
         if (share) {
-            mass_t all = 0;
-            for (int w = 0; w < NWAVES; w++) all += sh.wave_mass[w];
             need = (mass_t) __builtin_ceil(mass_wanted * (double) all);
             if (need == 0) need = 1;  // (the most probable token stays)
         }
@@ -508,8 +527,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
                         kept[e] = kept[e] && (x == top || weigh.real(x) >= min_w);
                         if (kept[e]) mine += w[e];
                     }
-                    (void) block_scan(mine, sh.wave_mass);
-                    for (int i = 0; i < NWAVES; i++) total += sh.wave_mass[i];
+                    (void) block_scan(mine, sh.wave_mass, &total);
                     need = target_of(p.uniform[r], total) + 1;
                 }
                 clear_hist();
@@ -691,8 +709,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
             __syncthreads();
             if (lane == 0) sh.wave_mass[wave] = mass;
             __syncthreads();
-            mass_t all = 0;
-            for (int w = 0; w < NWAVES; w++) all += sh.wave_mass[w];
+            const mass_t all = lane_of(scan_of_waves(sh.wave_mass), NWAVES - 1);
             need = max((mass_t) __builtin_ceil(mass_wanted * (double) all), 1ull);
         }
         if (!found) search(by_mass, need);
@@ -718,12 +735,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         if (lane == 0) sh.part_mass[wave] = mass;
     }
     __syncthreads();
-    mass_t total = 0;
-    for (int w = 0; w < NWAVES; w++) total += sh.part_mass[w];
-    const mass_t target = target_of(p.uniform[r], total);
-    int chosen = 0;
-    mass_t before = 0;
-    while (chosen < NWAVES - 1 && before + sh.part_mass[chosen] <= target) before += sh.part_mass[chosen++];
+    const mass_t parts = scan_of_waves(sh.part_mass), total = lane_of(parts, NWAVES - 1), target = target_of(p.uniform[r], total);
+    const int chosen = min((int) __popcll(__ballot(lane < NWAVES && parts <= target)), NWAVES - 1);
+    mass_t before = chosen ? lane_of(parts, chosen - 1) : 0;
     const int from = chosen * part * GROUP, to = min(from + part * GROUP, p.vocab), per = (to - from + THREADS - 1) / THREADS;
     const int mine = min(from + (int) threadIdx.x * per, to), mine_end = min(mine + per, to);
     mass_t mass = 0;
