@@ -10,14 +10,17 @@
 // touch only groups that can matter. The filters end in one threshold, the last token that stays in the order of falling
 // logits (ties: rising index):
 //   top_k   the group maxima go into a histogram over the distance to the largest. The bucket that holds the k-th largest of
-//           them bounds the k-th largest logit from below: the groups that reach it, little more than k, are listed and
-//           sorted, and the other filters and the draw work on that list alone.
+//           them bounds the k-th largest logit from below: the logits of the groups that reach it, little more than k, are
+//           listed, and the filters and the draw work on that list alone.
 //   top_p   (and top_k beyond what the list holds) all logits go into the histogram, masses (counts) instead of ones; the
-//           tokens of the bucket where the mass is reached, usually a hundred, are sorted.
+//           tokens of the bucket where the mass is reached, usually a few hundred, are sorted.
 // The 2048 buckets span the distances at which w is not zero. (Buckets on the bits of x would put most of a row into two dozen
 // of them: the atomics of a wave would queue. Over the distance a normal distribution fills hundreds.) A bucket with more
 // than 2048 tokens (flat rows) is searched by the bits of x, 8 at a time. Without a list the token is found in two steps: the
 // wave whose part holds the target, and the place inside that part.
+// Measured: 8.4 us for one f16 row of 32000 (the best 40), of which reading is a third and the rest a chain of steps between
+// barriers; 29 us for 64 f32 rows of 128001 (the best 1000), reading 8 us at 3.9 TB/s; 41 us for 256 f16 rows of 50001 by mass
+// alone, half of it the f64 arithmetic of 50001 weights on one compute unit.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -533,17 +536,18 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         __syncthreads();
         const int count = __builtin_amdgcn_readfirstlane(reaching <= LISTED ? sh.place : LISTED + 1);
         if (count <= 64) {
-            // One wave does the rest, an entry per lane, without a barrier (12.6 -> X us for the best 40 of 32000 logits): all
+            // One wave does the rest, an entry per lane, without a barrier (12.6 -> 8.4 us for the best 40 of 32000 logits): all
             // entries are compared with all others, then put into the order of the logits and that of the indices.
             if (wave != 0) return;
             const mass_t entry = lane < count ? sh.list[lane] : 0;
             int rank = 0, place = 0;
-#pragma unroll 4
-            for (int o = 0; o < count; o++) {
-                const mass_t other = lane_of(entry, o);
-                rank += other > entry;
-                place += ~(unsigned) other < ~(unsigned) entry;
-            }
+            for (int o0 = 0; o0 < count; o0 += 8)  // (what lies behind the list comes last in both)
+#pragma unroll
+                for (int o = o0; o < o0 + 8; o++) {
+                    const mass_t other = lane_of(entry, o);
+                    rank += other > entry;
+                    place += ~(unsigned) other < ~(unsigned) entry;
+                }
             const bool listed = lane < count;
             auto sums_in_order = [&](mass_t v, int at) {  // lane n: the sum of the first n + 1 in an order
                 sh.hist[lane] = 0;
@@ -607,24 +611,25 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
                 need = find_bucket(what == 1, need);
                 const unsigned bucket = sh.bucket;
                 const mass_t above = sh.above;
-                // (the histogram has been read: its room holds what the bucket's entries count)
+                // (the histogram has been read and the list is in registers: their rooms hold the bucket's entries and what they count)
 #pragma unroll
                 for (int e = 0; e < 2; e++)
                     if (kept[e] && b[e] == bucket) {
                         const int c = atomicAdd(&sh.list_count, 1);
-                        sh.places[c] = (unsigned short) (threadIdx.x + THREADS * e);
+                        sh.list[c] = entry[e];
                         sh.hist[c] = what == 0 ? 1ull : w[e];
                     }
                 __syncthreads();
                 const int inside = sh.list_count;
                 for (int c = threadIdx.x; c < inside; c += THREADS) {
-                    const mass_t own = sh.list[sh.places[c]];
+                    const mass_t own = sh.list[c];
                     mass_t before = above;
+#pragma unroll 4
                     for (int o = 0; o < inside; o++) {
-                        const mass_t other = sh.list[sh.places[o]];
-                        if (what == 2 ? ~(unsigned) other < ~(unsigned) own : other > own) before += sh.hist[o];
+                        const mass_t other = sh.list[o], counts = sh.hist[o];
+                        if (what == 2 ? ~(unsigned) other < ~(unsigned) own : other > own) before += counts;
                     }
-                    if (before < need && need <= before + sh.hist[c]) sh.place = sh.places[c];
+                    if (before < need && need <= before + sh.hist[c]) sh.place = c;
                 }
                 __syncthreads();
                 const mass_t last = sh.list[sh.place];
