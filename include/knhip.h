@@ -191,7 +191,8 @@ void knhip_kernel_free(knhip_kernel *kernel);
  * work may overlap need one each, and so do two captured graphs that may). They can be captured into a HIP graph.
  * Addresses are device addresses with the alignment of their element; strides are in elements, may be zero or negative
  * in operands that are only read, and the axis along a row's `width` is contiguous. Sizes, codes and addresses are checked
- * on the host before anything is launched. Lengths, slots and page numbers are device data and cannot be: entries out of
+ * on the host before anything is launched; rows that are written are refused where their strides let two of them share
+ * memory. Lengths, slots and page numbers are device data and cannot be: entries out of
  * range are skipped, as the operators say, and never reach outside the buffers. */
 
 /* Keys and values of past tokens in pages of `page_tokens` tokens: key (page, head, token, i) is element
@@ -200,7 +201,7 @@ void knhip_kernel_free(knhip_kernel *kernel);
  * page per sequence). KNHIP_F16 keeps the rows as they are. KNHIP_I8 keeps a row x as whole numbers q and one f32 scale:
  * scale = max |x| / 127, q = x / scale rounded to the nearest, ties to even (all zeros where the scale is zero), standing
  * for q * scale; the scales are dense arrays [pages, heads, page_tokens]. `width` is a multiple of 16 up to 256, `k` and `v`
- * are 16 byte aligned and so are the strides in bytes. pages * page_tokens stays below 2^31. */
+ * are 16 byte aligned and so are the strides in bytes; no two rows share memory. pages * page_tokens stays below 2^31. */
 typedef struct {
     int dtype; /* KNHIP_I8 or KNHIP_F16 */
     int pages, heads, page_tokens, width;

@@ -5,6 +5,8 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstdint>
+#include <cstdlib>
 
 #include "../../include/knhip.h"
 #include "executor.h"
@@ -49,6 +51,24 @@ void check_workspace(const char *what, size_t need, const void *workspace, size_
     require_aligned(what, "the workspace", workspace, 256);
 }
 
+// Whether rows of `width` elements at these strides may share memory: going from the smallest stride to the largest, each has to
+// step over all that lies below it.
+template <size_t N>
+bool rows_overlap(const int64_t (&strides)[N], const int (&counts)[N], int width) {
+    size_t order[N], axes = 0;
+    for (size_t i = 0; i < N; i++)
+        if (counts[i] > 1) order[axes++] = i;
+    std::sort(order, order + axes, [&](size_t a, size_t b) { return std::llabs(strides[a]) < std::llabs(strides[b]); });
+    int64_t reach = width;
+    for (size_t i = 0; i < axes; i++) {
+        const int64_t stride = std::llabs(strides[order[i]]);
+        if (stride < reach) return true;
+        if (stride > INT64_MAX / 4 / counts[order[i]]) return false;  // (no memory is that large)
+        reach += stride * (counts[order[i]] - 1);
+    }
+    return false;
+}
+
 // (sizes first: an empty cache or call has no addresses to check)
 void check_cache_sizes(const char *what, const knhip_kv_cache &c) {
     if (c.dtype != KNHIP_F16 && c.dtype != KNHIP_I8) fail(what, ": a cache holds f16 or i8, got dtype code ", c.dtype);
@@ -71,6 +91,7 @@ void check_cache_addresses(const char *what, const knhip_kv_cache &c) {
         if (strides[i] * elem % 16 != 0) fail(what, ": the cache's ", names[i], " stride must be a multiple of 16 bytes, got ", strides[i], " elements");
         if (strides[i] > (int64_t) 1 << 46) fail(what, ": the cache's ", names[i], " stride is out of range");
     }
+    if (rows_overlap(strides, counts, c.width)) fail(what, ": rows of the cache may not overlap, got strides of ", strides[0], ", ", strides[1], ", ", strides[2]);
     if (c.dtype == KNHIP_I8) {
         require_address(what, "k_scales", c.k_scales, 4);
         require_address(what, "v_scales", c.v_scales, 4);
@@ -91,10 +112,11 @@ bool check_rows(const char *what, const knhip_kv_cache *cache, const knhip_cache
     require_address(what, "the rows' v", rows->v, elem);
     require_address(what, "slots", rows->slots, 4);
     if (!write) {
-        const int64_t strides[4] = {rows->k_token_stride, rows->v_token_stride, rows->k_head_stride, rows->v_head_stride};
-        for (int i = 0; i < 4; i++)
-            if ((i < 2 ? rows->tokens : cache->heads) > 1 && std::llabs(strides[i]) < cache->width)
-                fail(what, ": rows that are written may not overlap, got a stride of ", strides[i], " for rows of ", cache->width);
+        const int64_t k_strides[2] = {rows->k_token_stride, rows->k_head_stride}, v_strides[2] = {rows->v_token_stride, rows->v_head_stride};
+        const int counts[2] = {rows->tokens, cache->heads};
+        if (rows_overlap(k_strides, counts, cache->width) || rows_overlap(v_strides, counts, cache->width))
+            fail(what, ": rows that are written may not overlap, got strides of ", k_strides[0], ", ", k_strides[1], " and ", v_strides[0], ", ", v_strides[1],
+                 " for rows of ", cache->width);
     }
     p.quantised = cache->dtype == KNHIP_I8;
     p.k = cache->k;
@@ -131,8 +153,8 @@ void check_scores(const char *what, float scale, float cap, int window, const fl
 void check_result_strides(const char *what, int64_t batch_stride, int64_t token_stride, int64_t head_stride, int batch, int tokens, int heads, int width) {
     const int64_t strides[3] = {batch_stride, token_stride, head_stride};
     const int counts[3] = {batch, tokens, heads};
-    for (int i = 0; i < 3; i++)
-        if (counts[i] > 1 && std::llabs(strides[i]) < width) fail(what, ": rows of out may not overlap, got a stride of ", strides[i], " for rows of ", width);
+    if (rows_overlap(strides, counts, width))
+        fail(what, ": rows of out may not overlap, got strides of ", strides[0], ", ", strides[1], ", ", strides[2], " for rows of ", width);
 }
 
 // true when there is nothing to do

@@ -571,6 +571,30 @@ def test_sample(case, hip_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(30))
+def test_sample_random(seed, hip_device):
+    """sizes and filters anywhere in their ranges, every row with its own"""
+    rng = np.random.default_rng(100 + seed)
+    rows, vocab = int(rng.integers(1, 9)), int(np.exp(rng.uniform(0, np.log(400000))))
+    dtype, kind = [(DType.F16, DType.F32)[seed % 2], ("normal", "normal", "few values", "peaked", "wide", "flat")[seed % 6]]
+    with np.errstate(over="ignore"):
+        logits = _logits(rng, kind, rows, vocab).astype(NP[dtype])
+    filters = dict(temperature=rng.choice([0.3, 0.7, 1.0, 1.0, 2.0, 20.0], rows).astype(np.float32),
+                   top_k=rng.choice([0, 1, 2, 7, 40, 63, 64, 65, 300, 1024, 1025, 20000], rows).astype(np.int32),
+                   top_p=rng.choice([1.0, 0.999, 0.95, 0.9, 0.5, 0.01], rows).astype(np.float32), min_p=rng.choice([0.0, 0.0, 1e-4, 0.05, 0.5], rows).astype(np.float32))
+    filters = {n: a for n, a in filters.items() if rng.random() < 0.8}
+    uniform = rng.random(rows).astype(np.float32)
+    args, dev, workspace = _sample_call(hip_device, logits, dtype, uniform, pad=int(rng.integers(0, 4)), **filters)
+    stream = kn.HipStream(hip_device)
+    kn.sample(hip_device, stream, args, workspace)
+    stream.synchronize()
+    tokens, chance = sample(logits, uniform, **filters)
+    got, p = dev["tokens"].to_array(np.int32, rows), dev["probabilities"].to_array(np.float32, rows)
+    assert np.array_equal(got, tokens), (vocab, dtype, kind, filters)
+    assert (np.abs(p - chance) <= chance * 2.0 ** -23 + vocab * 2.0 ** -42).all()
+
+
+@pytest.mark.gpu
 def test_sampling_follows_the_probabilities(hip_device):
     """evenly spaced random numbers draw every token as often as its probability says"""
     rng = np.random.default_rng(2)
@@ -664,6 +688,191 @@ def test_a_decoding_step_captured_and_replayed(hip_device):
         assert np.array_equal(tokens, expected)
 
 
+# ---- large offsets, many rows, other streams, graphs ---------------------------------------------------------------
+
+def _h2d(device, ptr, array):
+    from ctypes import c_void_p
+    array = np.ascontiguousarray(array)
+    kn._lib.check(kn._lib.lib.knhip_memcpy_h2d(device.index, c_void_p(ptr), array.ctypes.data, array.nbytes))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,queries", [(DType.I8, 1), (DType.I8, 40), (DType.F16, 1), (DType.F16, 40)], ids=lambda x: str(getattr(x, "name", x)))
+def test_cache_offsets_beyond_32_bits(dtype, queries, hip_device):
+    """a cache whose pages lie 2^27 bytes apart gives the results of a dense one, bit for bit"""
+    rng = np.random.default_rng(3)
+    pages, N, page, W, G, n = 40, 2, 16, 64, 3, 300
+    size = NP[dtype]().nbytes
+    apart = (1 << 27) // size
+    stream = kn.HipStream(hip_device)
+    # the tokens fill the last pages, in any order; a prefix of 40 in the first ones
+    prefix_table, table = np.array([0, 39, 1], np.int32), (20 + rng.permutation(19)).astype(np.int32)
+    slots = np.concatenate([prefix_table[np.arange(40) // page] * page + np.arange(40) % page, table[np.arange(n) // page] * page + np.arange(n) % page])
+    rows_k, rows_v = (upload(hip_device, rng.standard_normal((len(slots), N, W)).astype(np.float16)) for _ in range(2))
+    dev = [upload(hip_device, a) for a in (slots.astype(np.int32), np.array([n], np.int32), table, prefix_table, rng.standard_normal((1, queries, N * G, W)).astype(np.float16))]
+    outs, backs = [], []
+    for page_stride in (N * page * W, apart):
+        mem = [kn.DeviceBuffer(hip_device, ((pages - 1) * page_stride + N * page * W) * size) for _ in range(2)]
+        scales = [kn.DeviceBuffer(hip_device, pages * N * page * 4) for _ in range(2)]
+        cache = kn.kv_cache(dtype, pages, N, page, W, mem[0].ptr, mem[1].ptr, *([s.ptr for s in scales] if dtype == DType.I8 else [0, 0]),
+                            strides=(page_stride, page * W, W))
+        kn.cache_write(hip_device, stream, cache, kn.cache_rows(DType.F16, len(slots), rows_k.ptr, (N * W, W), rows_v.ptr, (N * W, W), dev[0].ptr))
+        back = [kn.DeviceBuffer(hip_device, len(slots) * N * W * 4) for _ in range(2)]
+        kn.cache_read(hip_device, stream, cache, kn.cache_rows(DType.F32, len(slots), back[0].ptr, (N * W, W), back[1].ptr, (N * W, W), dev[0].ptr))
+        out = kn.DeviceBuffer(hip_device, queries * N * G * W * 2)
+        args = kn.cached_attention_args(1, queries, N * G, cache, dev[4].ptr, (0, N * G * W, W), out.ptr, (0, N * G * W, W), dev[1].ptr, dev[2].ptr, len(table),
+                                        len(table), prefix_tokens=40, prefix_table=dev[3].ptr)
+        need = kn.cached_attention_workspace_bytes(args)
+        workspace = kn.DeviceBuffer(hip_device, max(need, 1))
+        kn.cached_attention(hip_device, stream, args, workspace)
+        stream.synchronize()
+        outs.append(out.to_array(np.uint16, queries * N * G * W))
+        backs.append([b.to_array(np.uint32, len(slots) * N * W) for b in back])
+    assert np.array_equal(outs[0], outs[1]) and outs[0].any()
+    assert np.array_equal(backs[0][0], backs[1][0]) and np.array_equal(backs[0][1], backs[1][1])
+
+
+@pytest.mark.gpu
+def test_prompt_and_logit_offsets_beyond_32_bits(hip_device):
+    rng = np.random.default_rng(4)
+    S, N, W, apart = 100, 2, 64, 1 << 25
+    stream = kn.HipStream(hip_device)
+    k, v, q = (rng.standard_normal((S, N, W)).astype(np.float16) for _ in range(3))
+    dense = [upload(hip_device, a) for a in (k, v, q)]
+    far = [kn.DeviceBuffer(hip_device, ((S - 1) * apart + N * W) * 2) for _ in range(2)]
+    for t in range(S):
+        for buf, a in zip(far, (k, v)):
+            _h2d(hip_device, buf.ptr + t * apart * 2, a[t])
+    outs = []
+    for ks, stride in ((dense, N * W), (far, apart)):
+        out = kn.DeviceBuffer(hip_device, S * N * W * 2)
+        args = kn.attention_args(1, S, S, N, N, W, dense[2].ptr, (0, N * W, W), ks[0].ptr, (0, stride, W), ks[1].ptr, (0, stride, W), out.ptr, (0, N * W, W), causal=True)
+        workspace = kn.DeviceBuffer(hip_device, max(kn.attention_workspace_bytes(args), 1))
+        kn.attention(hip_device, stream, args, workspace)
+        stream.synchronize()
+        outs.append(out.to_array(np.uint16, S * N * W))
+    assert np.array_equal(*outs) and outs[0].any()
+    # rows of logits as far apart
+    rows, vocab = S, 50
+    logits, uniform = rng.standard_normal((rows, vocab)).astype(np.float16), rng.random(rows).astype(np.float32)
+    for t in range(rows):
+        _h2d(hip_device, far[0].ptr + t * apart * 2, logits[t])
+    dev_uniform, tokens = upload(hip_device, uniform), kn.DeviceBuffer(hip_device, rows * 4)
+    kn.sample(hip_device, stream, kn.sample_args(DType.F16, rows, vocab, far[0].ptr, apart, dev_uniform.ptr, tokens.ptr))
+    stream.synchronize()
+    assert np.array_equal(tokens.to_array(np.int32, rows), sample(logits, uniform)[0])
+
+
+@pytest.mark.gpu
+def test_very_many_sequences_and_rows(hip_device):
+    """70000 sequences of no or one token: zeros or that token's values; as many prompts of one token, rows of logits"""
+    rng = np.random.default_rng(6)
+    B, N, G, W = 70000, 1, 2, 16
+    stream = kn.HipStream(hip_device)
+    k, v, q = rng.standard_normal((B, N, W)).astype(np.float16), rng.standard_normal((B, N, W)).astype(np.float16), rng.standard_normal((B, N * G, W)).astype(np.float16)
+    lengths = (np.arange(B) % 3 > 0).astype(np.int32)
+    dev = [upload(hip_device, a) for a in (k, v, q, lengths, np.arange(B, dtype=np.int32))]
+    out = kn.DeviceBuffer(hip_device, B * N * G * W * 2)
+    cache = kn.kv_cache(DType.F16, B, N, 1, W, dev[0].ptr, dev[1].ptr)
+    args = kn.cached_attention_args(B, 1, N * G, cache, dev[2].ptr, (N * G * W, W, W), out.ptr, (N * G * W, N * G * W, W), dev[3].ptr, dev[4].ptr, 1, 1)
+    workspace = kn.DeviceBuffer(hip_device, max(kn.cached_attention_workspace_bytes(args), 1))
+    kn.cached_attention(hip_device, stream, args, workspace)
+    stream.synchronize()
+    expected = np.repeat(v, G, 1) * (lengths[:, None, None] > 0)
+    assert np.array_equal(out.to_array(np.float16, (B, N * G, W)), expected)
+    args = kn.attention_args(B, 1, 1, N * G, N, W, dev[2].ptr, (N * G * W, W, W), dev[0].ptr, (N * W, W, W), dev[1].ptr, (N * W, W, W), out.ptr,
+                             (N * G * W, N * G * W, W), causal=True)
+    workspace = kn.DeviceBuffer(hip_device, max(kn.attention_workspace_bytes(args), 1))
+    kn.attention(hip_device, stream, args, workspace)
+    stream.synchronize()
+    assert np.array_equal(out.to_array(np.float16, (B, N * G, W)), np.repeat(v, G, 1))
+    uniform = rng.random(B).astype(np.float32)
+    dev_uniform, tokens = upload(hip_device, uniform), kn.DeviceBuffer(hip_device, B * 4)
+    kn.sample(hip_device, stream, kn.sample_args(DType.F16, B, W, dev[0].ptr, W, dev_uniform.ptr, tokens.ptr))
+    stream.synchronize()
+    assert np.array_equal(tokens.to_array(np.int32, B), sample(k[:, 0], uniform)[0])
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once(hip_device):
+    """prompts in parts, a shared prefix and draws on two streams, each with its own workspace: the results of calls made alone"""
+    streams = [kn.HipStream(hip_device) for _ in range(2)]
+    prompts = [_prompt_case(hip_device, dict(queries=90, keys=1500, heads=2, kv=1, width=64, causal=True), seed=s) for s in range(2)]
+    cached = [_cached_case(hip_device, dict(dtype=DType.I8, kv=2, group=4, width=128, page=16, lengths=[700 + i for i in range(9)], prefix=900), seed=s) for s in range(2)]
+    rng = np.random.default_rng(8)
+    draws = [_sample_call(hip_device, rng.standard_normal((5, 40000)).astype(np.float32), DType.F32, rng.random(5), top_p=np.full(5, 0.9)) for _ in range(2)]
+    spaces = [[kn.DeviceBuffer(hip_device, max(n, 1)) for n in (kn.attention_workspace_bytes(prompts[i]["args"]), kn.cached_attention_workspace_bytes(cached[i]["args"]))]
+              for i in range(2)]
+
+    def call(i):
+        kn.attention(hip_device, streams[i], prompts[i]["args"], spaces[i][0])
+        kn.cached_attention(hip_device, streams[i], cached[i]["args"], spaces[i][1])
+        kn.sample(hip_device, streams[i], draws[i][0], draws[i][2])
+
+    def results(i):
+        streams[i].synchronize()
+        return (prompts[i]["dev"][3].to_array(np.uint16, prompts[i]["out_mem"].shape), cached[i]["dev"][1].to_array(np.uint16, cached[i]["out_mem"].shape),
+                draws[i][1]["tokens"].to_array(np.int32, 5))
+
+    alone = []
+    for i in range(2):
+        call(i)
+        alone.append(results(i))
+    for _ in range(20):
+        for i in range(2):
+            call(i)
+    for i in range(2):
+        for a, b in zip(alone[i], results(i)):
+            assert np.array_equal(a, b)
+
+
+@pytest.mark.gpu
+def test_prompts_and_reads_captured_and_replayed(hip_device):
+    """a prompt in parts over keys that are read out of a cache, and a draw with every filter, as one graph"""
+    rng = np.random.default_rng(9)
+    S, K, N, W, rows, vocab = 70, 1100, 1, 64, 3, 33000
+    stream = kn.HipStream(hip_device)
+    cache = CacheCase(hip_device, DType.I8, 70, N, 16, W)
+    cache.put(np.arange(70 * 16), *rng.standard_normal((2, 70 * 16, N, W)).astype(np.float16))
+    args_cache = cache.upload()
+    dev = dict(k=kn.DeviceBuffer(hip_device, K * N * W * 2), v=kn.DeviceBuffer(hip_device, K * N * W * 2), q=kn.DeviceBuffer(hip_device, S * N * W * 2),
+               out=kn.DeviceBuffer(hip_device, S * N * W * 2), slots=kn.DeviceBuffer(hip_device, K * 4))
+    read = kn.cache_rows(DType.F16, K, dev["k"].ptr, (N * W, W), dev["v"].ptr, (N * W, W), dev["slots"].ptr)
+    prompt = kn.attention_args(1, S, K, N, N, W, dev["q"].ptr, (0, N * W, W), dev["k"].ptr, (0, N * W, W), dev["v"].ptr, (0, N * W, W), dev["out"].ptr,
+                               (0, N * W, W), causal=True)
+    logits = rng.standard_normal((rows, vocab)).astype(np.float32) * 3
+    draw, parts, _ = _sample_call(hip_device, logits, DType.F32, rng.random(rows), temperature=np.full(rows, 0.8), top_k=np.array([900, 0, 40]),
+                                  top_p=np.full(rows, 0.9), min_p=np.full(rows, 0.001))
+    need = kn.attention_workspace_bytes(prompt)
+    assert need > 0
+    workspace = kn.DeviceBuffer(hip_device, need)
+
+    def step():
+        kn.cache_read(hip_device, stream, args_cache, read)
+        kn.attention(hip_device, stream, prompt, workspace)
+        kn.sample(hip_device, stream, draw)
+
+    def results():
+        stream.synchronize()
+        return dev["out"].to_array(np.uint16, S * N * W), parts["tokens"].to_array(np.int32, rows)
+
+    graph, seen = None, []
+    for _ in range(4):
+        _h2d(hip_device, dev["slots"].ptr, rng.permutation(70 * 16)[:K].astype(np.int32))
+        _h2d(hip_device, dev["q"].ptr, rng.standard_normal((S, N, W)).astype(np.float16))
+        _h2d(hip_device, parts["uniform"].ptr, rng.random(rows).astype(np.float32))
+        if graph is None:
+            with Graph(stream) as graph:
+                step()
+        graph.launch()
+        replayed = results()
+        step()
+        for a, b in zip(replayed, results()):
+            assert np.array_equal(a, b)
+        seen.append(replayed[0])
+    assert not any(np.array_equal(seen[0], other) for other in seen[1:])
+
+
 # ---- what is refused (on the host, before anything is launched) ----------------------------------------------------
 
 def _valid():
@@ -696,7 +905,11 @@ REFUSED = [
     ("cache", "rows.k", 0, "rows' k is null"),
     ("cache", "rows.v", 3, "2 byte aligned"),
     ("cache", "rows.slots", 0, "slots is null"),
+    ("cache", "cache.head_stride", 512, "may not overlap"),
+    ("cache", "cache.page_stride", 1024, "may not overlap"),
     ("read", "rows.k_token_stride", 0, "may not overlap"),
+    ("read", "rows.k_token_stride", 64, "may not overlap"),
+    ("read", "rows.v_token_stride", -127, "may not overlap"),
     ("read", "rows.v_head_stride", 8, "may not overlap"),
     ("cached", "cache.width", 144, "at most 128"),
     ("cached", "cache.heads", 3, "evenly"),
@@ -711,6 +924,7 @@ REFUSED = [
     ("cached", "q", 1, "q must be 2 byte aligned"),
     ("cached", "out", 0, "out is null"),
     ("cached", "out_head_stride", 0, "out may not overlap"),
+    ("cached", "out_batch_stride", 128, "out may not overlap"),
     ("cached", "scale", math.inf, "scale must be finite"),
     ("cached", "cap", -1.0, "cap must be finite"),
     ("cached", "cap", math.nan, "cap must be finite"),
