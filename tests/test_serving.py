@@ -688,6 +688,54 @@ def test_a_decoding_step_captured_and_replayed(hip_device):
         assert np.array_equal(tokens, expected)
 
 
+# ---- shapes, masks and options anywhere in their ranges --------------------------------------------------------------
+
+def _random_scores(rng):
+    return dict(cap=float(rng.choice([0.0, 0.0, 3.0, 30.0])), slopes=bool(rng.random() < 0.3), size=float(rng.choice([1.0, 1.0, 4.0])))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(24))
+def test_cached_attention_random(seed, hip_device):
+    rng = np.random.default_rng(500 + seed)
+    page, batch = int(rng.choice([1, 5, 16, 16, 32, 100])), int(rng.integers(1, 12))
+    longest = int(np.exp(rng.uniform(0, np.log(1800))))
+    c = dict(dtype=[DType.I8, DType.F16][seed % 2], kv=int(rng.integers(1, 4)), group=int(rng.choice([1, 2, 3, 4, 8, 13])), width=16 * int(rng.integers(1, 9)),
+             page=page, lengths=[int(n) for n in rng.integers(-2, longest + 1, batch)], queries=int(rng.choice([1, 1, 1, 2, 5, 33])),
+             prefix=int(rng.choice([0, 0, 1, 70, 700])), window=int(rng.choice([0, 0, 1, 40, 500])), order=str(rng.choice(["dense", "tokens first"])), **_random_scores(rng))
+    case = _cached_case(hip_device, c, seed)
+    stream = kn.HipStream(hip_device)
+    workspace = kn.DeviceBuffer(hip_device, max(kn.cached_attention_workspace_bytes(case["args"]), 1))
+    kn.cached_attention(hip_device, stream, case["args"], workspace)
+    stream.synchronize()
+    out, bound = case["expected"]()
+    _check(case["dev"][1].to_array(np.float16, case["out_mem"].shape), out, bound, case["W"], str(c))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(24))
+def test_attention_of_prompts_random(seed, hip_device):
+    rng = np.random.default_rng(700 + seed)
+    queries, kv, batch = int(np.exp(rng.uniform(0, np.log(700)))), int(rng.integers(1, 4)), int(rng.integers(1, 4))
+    c = dict(batch=batch, queries=queries, heads=kv * int(rng.choice([1, 2, 3, 8])), kv=kv, width=8 * int(rng.integers(1, 17)), causal=bool(rng.random() < 0.7),
+             window=int(rng.choice([0, 0, 1, 33, 200])), **_random_scores(rng))
+    if rng.random() < 0.5:
+        c["keys"] = int(np.exp(rng.uniform(0, np.log(1500))))
+    else:
+        cuts = [sorted({int(x) for x in rng.integers(0, queries, 3)}) for _ in range(batch)]
+        if rng.random() < 0.5:
+            c["spans"] = cuts
+    if c["causal"] and rng.random() < 0.4:
+        c["prefix"] = [int(x) for x in rng.integers(-5, 2 * queries, batch)]
+    case = _prompt_case(hip_device, c, seed)
+    stream = kn.HipStream(hip_device)
+    workspace = kn.DeviceBuffer(hip_device, max(kn.attention_workspace_bytes(case["args"]), 1))
+    kn.attention(hip_device, stream, case["args"], workspace)
+    stream.synchronize()
+    out, bound = case["expected"]()
+    _check(case["dev"][3].to_array(np.float16, case["out_mem"].shape), out, bound, case["W"], str(c))
+
+
 # ---- large offsets, many rows, other streams, graphs ---------------------------------------------------------------
 
 def _h2d(device, ptr, array):
