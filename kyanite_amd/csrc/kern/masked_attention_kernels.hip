@@ -153,13 +153,14 @@ __device__ __forceinline__ halfx8 widen(unsigned a, unsigned b) {
 // ---- 32 rows per wave, 4 or 8 waves per workgroup ------------------------------------------------------------------
 
 // The waves walk all blocks of 64 keys, which they stage together in one of two LDS buffers, one barrier per block: the
-// block after the current one is in flight in registers meanwhile. WP: the width, padded to 64 or 128 with zeros. SHAPED: with
+// block after the current one is in flight in registers meanwhile. KG = 2: twice the waves for the same rows, in two groups that take
+// every other block each and are joined at the end through LDS. WP: the width, padded to 64 or 128 with zeros. SHAPED: with
 // cap or distance bias. I8: keys and values are staged as the whole numbers they are, exact in f16; the scale of a key is
 // applied to its scores, that of a value to its weights, both in f32. The scaled weights keep inside f16 by a power of two
 // that the waves of a workgroup share: it starts from the first block and grows when a scale passes it by 2^6.
-template <int WP, int STRETCH, bool I8, bool SHAPED, int TW>
+template <int WP, int STRETCH, bool I8, bool SHAPED, int TW, int KG>
 __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_attention_kernel(ServingAttentionParams p) {
-    constexpr int BKEYS = 64, THREADS = 64 * TW;
+    constexpr int BKEYS = 64, RW = TW / KG, THREADS = 64 * RW;  // waves for the rows, threads that stage a block
     constexpr int PIECE = I8 ? 16 : 8;        // elements per 128 bit load
     constexpr int C = WP / PIECE;             // loads per row
     constexpr int VECS = BKEYS * C / THREADS;  // of K and of V, per lane and block
@@ -168,15 +169,19 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     constexpr int OS = WP + 8, WAVE_ROWS = 32 * OS;
     constexpr int DT = WP / 32, QC = WP / 8;
     constexpr bool PAGED = STRETCH != PROMPT;
-    constexpr int LDS_HALVES = 2 * STAGE > TW * WAVE_ROWS ? 2 * STAGE : TW * WAVE_ROWS;
+    constexpr int JOIN = KG > 1 ? RW * 64 * (DT * 16 + 2) * 2 : 0;  // the other group's accumulators, in halves
+    constexpr int LDS_HALVES = std::max({2 * KG * STAGE, TW * WAVE_ROWS, JOIN + RW * WAVE_ROWS});
     static_assert(WP != 128 || VECS >= 1, "unsupported shape");
     __shared__ __attribute__((aligned(16))) half_t lds[LDS_HALVES];
     __shared__ __attribute__((aligned(16))) float kscale_s[2][BKEYS], vscale_s[2][BKEYS];
     __shared__ unsigned long long gone_s[2][TW], bad_s[2][TW];
     __shared__ int big_s[2][TW];
     __shared__ int range_s[TW][4];
+    static_assert(!I8 || KG == 1, "groups of waves share the power of two");
 
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, all_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = all_wave % RW, group = all_wave / RW;  // rows of the tile, blocks of keys
+    const int thread = (int) threadIdx.x % THREADS;
     const int c = lane & 31, h = lane >> 5;
     // workgroups of one head of keys are a multiple of the (sequence, head) pairs apart: with 8 pairs or a multiple of them
     // they run on one XCD and share its L2; the last tiles, with the most keys under a causal mask, come first
@@ -186,7 +191,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const unsigned rows = (unsigned) (STRETCH == PREFIX ? p.batch : 1) * p.queries * p.group_div.d;
     const int split = blockIdx.y, splits = gridDim.y;
 
-    const unsigned first_row = (unsigned) tile * (32 * TW) + wave * 32;
+    const unsigned first_row = (unsigned) tile * (32 * RW) + wave * 32;
     const unsigned row = first_row + c, row_c = min(row, rows - 1);
     const Row w = row_of<STRETCH>(p, row_c, b, kv_head);
 
@@ -201,7 +206,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             for (int i = 0; i < 4; i++) a[i] = min(a[i], __shfl_xor(a[i], m));
         if (lane == 0)
 #pragma unroll
-            for (int i = 0; i < 4; i++) range_s[wave][i] = a[i];
+            for (int i = 0; i < 4; i++) range_s[all_wave][i] = a[i];
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -234,7 +239,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         kb += kv_head * p.k_head * ELEM;
         vb += kv_head * p.v_head * ELEM;
     }
-    const int stage_row = (int) threadIdx.x / C, part = (int) threadIdx.x % C;
+    const int stage_row = thread / C, part = thread % C;
     constexpr int ROW_STEP = THREADS / C;  // rows between a lane's loads
     const bool part_live = part * PIECE < p.width;
     const long long k_lane = stage_row * p.k_token * ELEM + 16 * part, v_lane = stage_row * p.v_token * ELEM + 16 * part;  // prompts
@@ -305,7 +310,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const float near_cap = I8 ? 0.35f : uniform(0.35f / to_cap);
     float value_unit = 0x1p60f;  // I8: what the scales of values are multiplied by, a power of two
     auto stage = [&](int buffer, bool masked) {
-        half_t *ks = lds + buffer * STAGE, *vs = ks + BKEYS * KS;
+        half_t *ks = lds + (KG * buffer + group) * STAGE, *vs = ks + BKEYS * KS;
         bool big = false;
 #pragma unroll
         for (int i = 0; i < VECS; i++) {
@@ -326,7 +331,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             }
         }
         // which of the block's rows are not there, and which hold values that a product with a zero weight does not remove
-        if (PAGED || masked) {
+        if (KG > 1 || PAGED || masked) {
             unsigned long long gone_rows = 0, bad_rows = 0;
 #pragma unroll
             for (int i = 0; i < VECS; i++) {
@@ -344,24 +349,25 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             }
             const int any_big = I8 ? __any(big) : 0;
             if (lane == 0) {
-                gone_s[buffer][wave] = gone_rows;
-                bad_s[buffer][wave] = bad_rows;
-                if (I8) big_s[buffer][wave] = any_big;
+                gone_s[buffer][all_wave] = gone_rows;
+                bad_s[buffer][all_wave] = bad_rows;
+                if (I8) big_s[buffer][all_wave] = any_big;
             }
         }
     };
 
-    if (first_block < end_block) {
-        look_up(first_block);
-        fetch(first_block);
-        look_up(min(first_block + 1, end_block - 1));
+    const int start = first_block + group;
+    if (start < end_block) {
+        look_up(start);
+        fetch(start);
+        look_up(min(start + KG, end_block - 1));
     }
 
     // ---- Q: the wave's 32 rows, whole lines at a time, through the wave's part of LDS; lane (query c, half h) holds elements
     // 16 t + 8 h .. + 7 for step t, in the order of the staged keys
     halfx8 qf[WP / 16];
     {
-        half_t *qs = lds + wave * WAVE_ROWS;
+        half_t *qs = lds + all_wave * WAVE_ROWS;
 #pragma unroll
         for (int i = 0; i < 32 * QC / 64; i++) {
             const int e = lane + 64 * i, r = e / QC, d = 8 * (e % QC);
@@ -387,28 +393,36 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const int v_corner = BKEYS * KS + (4 * h + (lane & 15) / 4) * VS + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
     constexpr bool LOG2_UNITS = SHAPED || I8;  // the scores have their factor before the exponential
 
-    for (int block = first_block; block < end_block; block++) {
-        const int buffer = block & 1, key0 = block * BKEYS;
+    for (int turn = 0; first_block + KG * turn < end_block; turn++) {
+        const int block = start + KG * turn, buffer = turn & 1, key0 = block * BKEYS;
+        const bool live = KG == 1 || block < end_block;  // (the last turn may have one block less)
         bool masked = key0 < whole_from || key0 + BKEYS > whole_end;
-        stage(buffer, masked);
-        if (block + 1 < end_block) {
-            fetch(block + 1);
-            look_up(min(block + 2, end_block - 1));
+        if (live) {
+            stage(buffer, masked);
+            if (block + KG < end_block) {
+                fetch(block + KG);
+                look_up(min(block + 2 * KG, end_block - 1));
+            }
+        } else if (lane == 0) {
+            bad_s[buffer][all_wave] = 0;
         }
         __syncthreads();
-        half_t *ks = lds + buffer * STAGE;
+        half_t *ks = lds + (KG * buffer + group) * STAGE;
         unsigned long long gone_rows = 0;
-        if (PAGED || masked) {
-            unsigned long long bad_rows = 0;
+        if (KG > 1 || PAGED || masked) {
+            unsigned long long bad_rows = 0, bad_anywhere = 0;
             int big = 0;
 #pragma unroll
-            for (int i = 0; i < TW; i++) {
-                gone_rows |= gone_s[buffer][i];
-                if (!I8) bad_rows |= bad_s[buffer][i];
+            for (int i = 0; i < RW; i++) {
+                gone_rows |= gone_s[buffer][group * RW + i];
+                if (!I8) bad_rows |= bad_s[buffer][group * RW + i];
                 if (I8) big |= big_s[buffer][i];
             }
+            if (!I8)
+#pragma unroll
+                for (int i = 0; i < TW; i++) bad_anywhere |= bad_s[buffer][i];
             gone_rows = ((unsigned long long) __builtin_amdgcn_readfirstlane((unsigned) (gone_rows >> 32)) << 32) | (unsigned) __builtin_amdgcn_readfirstlane((unsigned) gone_rows);
-            masked |= gone_rows != 0;
+            if (PAGED) masked |= gone_rows != 0;
             if (I8 && __builtin_amdgcn_readfirstlane(big)) {  // (the same for all waves, which take the barriers together)
                 float most = vscale_s[buffer][lane];
 #pragma unroll
@@ -424,7 +438,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
                 __syncthreads();
             }
             bad_rows = ((unsigned long long) __builtin_amdgcn_readfirstlane((unsigned) (bad_rows >> 32)) << 32) | (unsigned) __builtin_amdgcn_readfirstlane((unsigned) bad_rows);
-            if (!I8 && bad_rows != 0) {
+            if (!I8 && (__builtin_amdgcn_readfirstlane((unsigned) (bad_anywhere >> 32)) | __builtin_amdgcn_readfirstlane((unsigned) bad_anywhere)) != 0) {
                 // Infinities or NaN among the values of a block that not every row sees whole: a weight of zero does not remove
                 // them from a product, so they are added here for the queries that see their key, and then taken out.
                 for (unsigned long long left = bad_rows; left; left &= left - 1) {
@@ -440,7 +454,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
                             }
                 }
                 __syncthreads();
-                for (int e = threadIdx.x; e < BKEYS * QC; e += THREADS) {
+                for (int e = thread; e < BKEYS * QC; e += THREADS) {
                     const int r = e / QC;
                     halfx8 *x = (halfx8 *) &ks[BKEYS * KS + r * VS + 8 * (e % QC)];
                     if ((bad_rows >> r) & 1) *x = finite_or_zero(*x);
@@ -449,6 +463,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             }
         }
 
+        if (!live) break;  // (nothing comes behind it)
         floatx16 st[2];
 #pragma unroll
         for (int u = 0; u < 2; u++)
@@ -546,6 +561,34 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         }
     }
 
+    if (KG > 1) {  // the other group's blocks
+        float *other = (float *) lds + wave * 64 * (DT * 16 + 2);
+        __syncthreads();  // (every wave is done with the buffers)
+        if (group == 1) {
+#pragma unroll
+            for (int t = 0; t < DT; t++)
+#pragma unroll
+                for (int a = 0; a < 4; a++)
+                    *(floatx4 *) &other[(4 * t + a) * 256 + 4 * lane] = floatx4{oacc[t][4 * a], oacc[t][4 * a + 1], oacc[t][4 * a + 2], oacc[t][4 * a + 3]};
+            *(float2 *) &other[DT * 16 * 64 + 2 * lane] = float2{ref, sum};
+        }
+        __syncthreads();
+        if (group == 1) return;
+        const float2 stats = *(const float2 *) &other[DT * 16 * 64 + 2 * lane];
+        const float new_ref = fmaxf(ref, stats.x), minus = new_ref == -INFINITY ? 0.0f : new_ref;
+        // (a group that saw nothing adds nothing but what is not finite, see above)
+        const float own = ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - minus), its = stats.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(stats.x - minus);
+        ref = new_ref;
+        sum = sum * own + stats.y * its;
+#pragma unroll
+        for (int t = 0; t < DT; t++)
+#pragma unroll
+            for (int a = 0; a < 4; a++) {
+                const floatx4 x = *(const floatx4 *) &other[(4 * t + a) * 256 + 4 * lane];
+#pragma unroll
+                for (int v = 0; v < 4; v++) oacc[t][4 * a + v] = oacc[t][4 * a + v] * own + x[v] * its;
+            }
+    }
     sum += __shfl_xor(sum, 32);
     const float back = I8 ? 1.0f / value_unit : 1.0f;
     // (dims 32 t + 8 a + 4 h + (0 .. 3) are registers 4 a .. 4 a + 3, the middle two changed over where widen() does)
@@ -568,8 +611,8 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     }
     // ---- the result: normalised, rounded, through the wave's rows of LDS into whole rows
     const float inv = sum > 0.0f || sum != sum ? back / sum : 0.0f;
-    __syncthreads();  // (every wave is done with the buffers)
-    half_t *os = lds + wave * WAVE_ROWS;
+    if (KG == 1) __syncthreads();  // (every wave is done with the buffers)
+    half_t *os = lds + JOIN + wave * WAVE_ROWS;
 #pragma unroll
     for (int t = 0; t < DT; t++)
 #pragma unroll
@@ -1219,20 +1262,32 @@ Plan plan_for(const ServingAttentionParams &p) {
 
 size_t round256(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-template <int WP, int STRETCH, bool I8>
+template <int WP, int STRETCH, bool I8, int KG>
 int launch_tiles(const ServingAttentionParams &p, unsigned workgroups, int splits, hipStream_t stream) {
-    constexpr int TW = tile_waves(WP, I8);
+    constexpr int TW = tile_waves(WP, I8) * KG;
     const dim3 grid(workgroups, (unsigned) splits), block(64 * TW);
-    if (p.cap > 0.0f || p.slopes) hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, true, TW>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, false, TW>), grid, block, 0, stream, p);
+    if (p.cap > 0.0f || p.slopes) hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, true, TW, KG>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, false, TW, KG>), grid, block, 0, stream, p);
     return (int) hipGetLastError();
+}
+
+// Where compute units would have one workgroup of four waves each, a second group of waves takes every other block of keys. (Two
+// workgroups overlap better than two groups, which wait at the same barriers: with 32 heads 1024 tokens, 256 workgroups, take 30
+// us in two groups and 33 without, 1536 tokens, 384 workgroups, 44 and 52, but 3000 tokens, 752 workgroups, 128 and 104.)
+template <int WP, int STRETCH>
+int launch_tiles_of(const ServingAttentionParams &p, unsigned workgroups, int splits, hipStream_t stream) {
+    if constexpr (STRETCH != PROMPT)
+        if (p.k_scales) return launch_tiles<WP, STRETCH, true, 1>(p, workgroups, splits, stream);
+    const int keys = STRETCH == PROMPT ? p.keys : STRETCH == OWN ? p.table_tokens : p.prefix_tokens;  // (one block cannot be shared)
+    return (long long) workgroups * splits <= 384 && keys > 64 ? launch_tiles<WP, STRETCH, false, 2>(p, workgroups, splits, stream)
+                                                               : launch_tiles<WP, STRETCH, false, 1>(p, workgroups, splits, stream);
 }
 
 template <int WP>
 int launch_tiles_for(const ServingAttentionParams &p, int stretch, unsigned workgroups, int splits, hipStream_t stream) {
-    if (stretch == PROMPT) return launch_tiles<WP, PROMPT, false>(p, workgroups, splits, stream);
-    if (stretch == OWN) return p.k_scales ? launch_tiles<WP, OWN, true>(p, workgroups, splits, stream) : launch_tiles<WP, OWN, false>(p, workgroups, splits, stream);
-    return p.k_scales ? launch_tiles<WP, PREFIX, true>(p, workgroups, splits, stream) : launch_tiles<WP, PREFIX, false>(p, workgroups, splits, stream);
+    return stretch == PROMPT ? launch_tiles_of<WP, PROMPT>(p, workgroups, splits, stream)
+         : stretch == OWN    ? launch_tiles_of<WP, OWN>(p, workgroups, splits, stream)
+                             : launch_tiles_of<WP, PREFIX>(p, workgroups, splits, stream);
 }
 
 template <int WP, int NT, bool I8>

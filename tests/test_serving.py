@@ -268,6 +268,8 @@ CACHED_CASES = {
     "many_sequences": dict(dtype=DType.I8, kv=1, group=2, width=64, page=16, lengths=[(13 * i) % 70 for i in range(150)]),
     "long_and_short": dict(dtype=DType.I8, kv=1, group=2, width=64, page=16, lengths=[9000, 5, 0, 2500]),
     "long_f16_wide_rows": dict(dtype=DType.F16, kv=1, group=4, width=128, page=16, lengths=[5000, 40], queries=8),
+    "many_prompts_over_the_cache": dict(dtype=DType.F16, kv=2, group=1, width=128, page=16, lengths=[40 + (9 * i) % 100 for i in range(200)], queries=40, poison=True),
+    "many_prompts_over_the_cache_i8": dict(dtype=DType.I8, kv=2, group=1, width=64, page=16, lengths=[(9 * i) % 120 for i in range(200)], queries=40, prefix=100, cap=9.0),
     "many_heads_of_one": dict(dtype=DType.I8, kv=1, group=71, width=64, page=16, lengths=[300, 4]),
 }
 
@@ -331,6 +333,9 @@ PROMPT_CASES = {
     "padded_batch": dict(batch=3, queries=140, heads=2, kv=2, width=128, causal=True, lengths=[140, 1, 0]),
     "unseen_is_nan": dict(batch=2, queries=260, heads=2, kv=2, width=64, causal=True, lengths=[100, 259], poison=True),
     "future_is_nan": dict(queries=200, keys=200, heads=2, kv=2, width=64, causal=True, poison_from=150),
+    "many_prompts": dict(batch=210, queries=70, heads=2, kv=2, width=128, causal=True, lengths=[(7 * i) % 71 for i in range(210)], poison=True),
+    "many_prompts_everything": dict(batch=200, queries=40, keys=150, heads=4, kv=2, width=64, causal=True, cap=8.0, slopes=True, window=90,
+                                    prefix=[i % 60 for i in range(200)], size=2.0),
     "past_is_nan": dict(queries=200, heads=1, kv=1, width=128, causal=True, window=30, poison_to=71),
 }
 
@@ -340,6 +345,7 @@ PROMPT_INFINITE = {
     "first_block": dict(queries=50, heads=2, kv=1, width=64, causal=True, infinite=[(0, 5, 1), (20, 9, -1), (49, 63, 1)]),
     "later_blocks": dict(queries=300, heads=2, kv=2, width=128, causal=True, window=150, infinite=[(63, 0, 1), (64, 127, -1), (200, 64, 1)]),
     "whole_blocks": dict(queries=64, keys=128, heads=1, kv=1, width=64, infinite=[(10, 3, 1), (100, 4, -1)]),
+    "many": dict(batch=400, queries=35, keys=100, heads=1, kv=1, width=64, causal=True, infinite=[(0, 5, 1), (70, 9, -1), (99, 63, 1)]),
     "in_parts": dict(queries=100, keys=1500, heads=1, kv=1, width=64, causal=True, infinite=[(3, 1, 1), (700, 2, -1), (1450, 3, 1)]),
 }
 
