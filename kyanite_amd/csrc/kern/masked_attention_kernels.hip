@@ -305,9 +305,10 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const float scale2 = uniform(p.scale == 0.0f ? 1.0f : fabsf(p.scale) * LOG2E);
     const bool capped = SHAPED && p.cap > 0.0f;
     const float to_cap = uniform(capped ? scale2 / (LOG2E * p.cap) : 0.0f), cap2 = uniform(p.cap * LOG2E);
-    // the series takes scores (I8: scores over the cap) up to 0.35 of the cap
+    // the series takes scores (I8: scores over the cap) up to 0.35 of the cap; with caps so small that its coefficients would
+    // leave f32 nothing does
     const CapSeries series(cap2, I8 ? 1.0f : to_cap);
-    const float near_cap = I8 ? 0.35f : uniform(0.35f / to_cap);
+    const float near_cap = I8 ? 0.35f : uniform(to_cap < 4096.0f ? 0.35f / to_cap : -1.0f);
     float value_unit = 0x1p60f;  // I8: what the scales of values are multiplied by, a power of two
     auto stage = [&](int buffer, bool masked) {
         half_t *ks = lds + (KG * buffer + group) * STAGE, *vs = ks + BKEYS * KS;

@@ -104,7 +104,7 @@ bool check_rows(const char *what, const knhip_kv_cache *cache, const knhip_cache
     check_cache_sizes(what, *cache);
     if (rows->dtype != KNHIP_F16 && rows->dtype != KNHIP_F32) fail(what, ": rows are f16 or f32, got dtype code ", rows->dtype);
     if (rows->tokens < 0) fail(what, ": negative size");
-    if ((long long) rows->tokens * cache->heads > INT_MAX) fail(what, ": tokens * heads must stay below 2^31");
+    if ((long long) rows->tokens * cache->heads > INT_MAX / 16) fail(what, ": tokens * heads must stay below 2^27");
     if (rows->tokens == 0 || cache->heads == 0) return true;
     if (cache->pages > 0) check_cache_addresses(what, *cache);
     const size_t elem = rows->dtype == KNHIP_F16 ? 2 : 4;
@@ -144,8 +144,10 @@ bool check_rows(const char *what, const knhip_kv_cache *cache, const knhip_cache
 }
 
 void check_scores(const char *what, float scale, float cap, int window, const float *slopes) {
-    if (!std::isfinite(scale)) fail(what, ": the scale must be finite");
-    if (!(cap >= 0.0f) || !std::isfinite(cap)) fail(what, ": the cap must be finite and not negative");
+    // (in units of log2 too)
+    if (!std::isfinite(scale * 1.5f)) fail(what, ": the scale must be finite");
+    if (!(cap >= 0.0f) || !std::isfinite(cap * 1.5f)) fail(what, ": the cap must be finite and not negative");
+    if (cap > 0.0f && !std::isfinite(std::max(std::fabs(scale), 1.0f) * 1.5f / cap)) fail(what, ": the cap is too small for the scale");
     if (window < 0) fail(what, ": the window must not be negative");
     if (slopes != nullptr) require_aligned(what, "slopes", slopes, 4);
 }
@@ -169,6 +171,7 @@ bool plan_cached_attention(const knhip_cached_attention_args *args, ServingAtten
     check_scores(what, a.scale, a.cap, a.window, a.slopes);
     if (a.batch == 0 || a.queries == 0 || a.heads == 0) return true;
     if (c.heads < 1 || a.heads % c.heads != 0) fail(what, ": ", a.heads, " heads cannot share ", c.heads, " heads of the cache evenly");
+    if ((long long) a.batch * c.heads >= 1 << 22) fail(what, ": batch * heads of the cache must stay below 2^22");
     if ((long long) a.batch * a.queries * a.heads > INT_MAX / 128) fail(what, ": batch * queries * heads must stay below 2^24");
     // (pages may occur in several tables, so that the places of a sequence may outnumber the slots of the cache)
     const long long table_tokens = (long long) a.table_pages * c.page_tokens;
@@ -225,6 +228,7 @@ bool plan_attention(const knhip_attention_args *args, ServingAttentionParams &p)
     check_scores(what, a.scale, a.cap, a.window, a.slopes);
     if (a.batch == 0 || a.queries == 0 || a.heads == 0) return true;
     if (a.kv_heads < 1 || a.heads % a.kv_heads != 0) fail(what, ": ", a.heads, " heads cannot share ", a.kv_heads, " heads of keys evenly");
+    if ((long long) a.batch * a.kv_heads >= 1 << 22) fail(what, ": batch * kv_heads must stay below 2^22");
     if ((long long) a.batch * a.queries * a.heads > INT_MAX / 16) fail(what, ": batch * queries * heads must stay below 2^27");
     if (a.keys > INT_MAX / 2 || a.queries > INT_MAX / 2) fail(what, ": queries and keys must stay below 2^30");
     require_address(what, "q", a.q, 2);

@@ -319,6 +319,9 @@ PROMPT_CASES = {
     "no_keys": dict(queries=5, keys=0, heads=2, kv=2, width=64),
     "cross": dict(batch=3, queries=50, keys=77, heads=4, kv=2, width=40),
     "cap": dict(queries=257, heads=2, kv=2, width=128, causal=True, cap=5.0, size=4.0),
+    "tiny_cap": dict(queries=150, heads=2, kv=2, width=128, causal=True, cap=1e-6),
+    "tiny_cap_equal_scores": dict(queries=150, heads=2, kv=2, width=128, causal=True, cap=1e-6, scale=0.0),
+    "huge_cap": dict(queries=150, heads=2, kv=2, width=64, causal=True, cap=1e30),
     "bias": dict(queries=300, heads=4, kv=4, width=64, causal=True, slopes=True),
     "bias_both_sides": dict(queries=150, heads=2, kv=2, width=64, slopes=True),
     "window": dict(queries=400, heads=2, kv=1, width=128, causal=True, window=37),
@@ -955,7 +958,7 @@ REFUSED = [
     ("cache", "cache.page_stride", -2048, "less than a row"),
     ("cache", "rows.dtype", int(DType.I8), "rows are f16 or f32"),
     ("cache", "rows.tokens", -1, "negative size"),
-    ("cache", "rows.tokens", (1 << 31) - 1, "below 2\\^31"),
+    ("cache", "rows.tokens", 1 << 26, "below 2\\^27"),
     ("cache", "rows.k", 0, "rows' k is null"),
     ("cache", "rows.v", 3, "2 byte aligned"),
     ("cache", "rows.slots", 0, "slots is null"),
@@ -970,6 +973,10 @@ REFUSED = [
     ("cached", "heads", 5, "evenly"),
     ("cached", "batch", -1, "negative size"),
     ("cached", "queries", 1 << 24, "below 2\\^24"),
+    ("cached", "batch", 1 << 21, "below 2\\^22"),
+    ("prompt", "batch", 1 << 21, "below 2\\^22"),
+    ("prompt", "cap", 1e-44, "too small"),
+    ("cached", "cap", 3.2e38, "cap must be finite"),
     ("cached", "table_pages", 1 << 27, "below 2\\^30"),
     ("cached", "prefix_tokens", 1 << 30, "below 2\\^30"),
     ("cached", "prefix_table", 0, "prefix_table is null"),
