@@ -241,7 +241,7 @@ int knhip_cache_read(int device, void *stream, const knhip_kv_cache *cache, cons
  *     out = sum_j softmax(z)_j v_j, or zeros where nothing is seen
  * A query that would stand before the sequence's own first token (lengths[b] < queries: a padded batch) gives zeros.
  * Lengths beyond table_pages * page_tokens count as that, negative ones as 0; the keys of a page number outside the cache
- * are not seen. q and out are f16; the shared tokens are read once for all sequences. Sums and statistics are f32, the
+ * are not seen. q and out are f16; many shared tokens are read once for all sequences. Sums and statistics are f32, the
  * weights enter the second product as f16. width: a multiple of 16 up to 128. */
 typedef struct {
     int batch, queries, heads;

@@ -9,7 +9,8 @@
 // that a block of keys is fetched once for them. Three kernels:
 //   tile_attention_kernel   32 rows per wave, 128 or 256 per workgroup: prompts, prompts over a cache, and the shared prefix of a batch, whose
 //                           rows are the queries of ALL sequences
-//   row_attention_kernel    up to 16 or 32 rows per workgroup: the few queries of one sequence over its own keys
+//   row_attention_kernel    up to 16 or 32 rows per workgroup: the few queries of one sequence over its own keys, and over a
+//                           prefix that is short
 //   join_attention_kernel   the softmax of parts: keys are split between workgroups where rows are few, and a sequence with
 //                           a prefix has its own part and the prefix's
 // Scores are computed transposed, S^T = K Q^T, so that a lane owns a query and the accumulators of S^T are the operands of
@@ -74,7 +75,7 @@ __device__ __forceinline__ Row row_of(const ServingAttentionParams &p, unsigned 
         w.hi = p.keys;
         if (p.causal) w.hi = min(w.hi, max(w.at + 1, p.prefix ? p.prefix[w.b] : 0));
     } else {
-        const int own = (STRETCH == OWN && length >= 0 ? length : own_length(p, w.b)) - p.queries + w.t;  // below 0: a query of padding
+        const int own = (length >= 0 ? length : own_length(p, w.b)) - p.queries + w.t;  // below 0: a query of padding
         w.at = STRETCH == OWN ? own : p.prefix_tokens + own;
         w.hi = own < 0 ? 0 : STRETCH == OWN ? own + 1 : p.prefix_tokens;
     }
@@ -654,7 +655,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 constexpr int ROW_ITEMS = 512, ROW_MIN_KEYS = 1024, ROW_WAVES = 8, ROW_THREADS = 64 * ROW_WAVES;
 
 struct Item {
-    int seg, length, from, end, items;
+    int seg, length, from, end, nth, items;
 };
 
 // segments -1 (the prefix, when `with_prefix`) and 0 .. batch - 1; false when there is no such item. Every wave works it out
@@ -703,6 +704,7 @@ __device__ __forceinline__ bool find_item(const ServingAttentionParams &p, int w
             out.seg = s0 + l - with_prefix;
             out.length = __builtin_amdgcn_readlane(r.x, l);
             const int per = 32 * ((__builtin_amdgcn_readlane(own_steps, l) + out.items - 1) / out.items);
+            out.nth = nth;
             out.from = min(begin + nth * per, out.length);
             out.end = min(begin + nth * per + per, out.length);
             if (nth == 0 && threadIdx.x == 0) ((int2 *) p.part_items)[out.seg + 1] = int2{item, out.items};
@@ -732,7 +734,7 @@ __device__ __forceinline__ void load_words(const char *from, unsigned (&to)[WORD
 
 // PAGE16: pages are multiples of 16 tokens and a tile of 16 keys spans less than 2 GiB, so that a tile lies in one page, whose
 // number and address the whole wave shares, and lanes differ by 32 bit offsets
-template <int WP, int NT, bool I8, bool SHAPED, bool PAGE16>
+template <int WP, int NT, bool I8, bool SHAPED, bool PAGE16, bool INSIDE>
 // (at least two waves per SIMD: with more registers than that leaves, the results of matrix instructions would lie in AGPRs, and
 // the compiler reads such a result too early behind a branch)
 __global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))) void row_attention_kernel(ServingAttentionParams p, int with_prefix) {
@@ -750,41 +752,18 @@ __global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))
     Item item;
     if (!find_item(p, with_prefix, global_item, item)) return;
     const bool is_prefix = item.seg < 0;
-    const int b = is_prefix ? 0 : item.seg, count = item.length;
+    const int b = is_prefix ? 0 : item.seg;
     const int rows = (is_prefix ? p.batch : 1) * p.queries * (int) p.group_div.d;
-    const int *table = is_prefix ? p.prefix_table : p.tables + b * p.table_stride;
-
-    int pages[2] = {0, 0};
-    auto look_up = [&](int key0) {  // the pages of a step's tiles, ahead of their loads; behind the last key: none
-        if (PAGE16)
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int j = key0 + 16 * u;
-                pages[u] = j < item.end ? table[p.page_tokens.div((unsigned) j)] : -1;
-            }
-    };
     constexpr int STRIDE = 32 * ROW_WAVES;
-    if (item.from < item.end) look_up(item.from + 32 * wave);
 
     // ---- the rows: lane i of a tile of 16 owns row 16 n + i
     halfx8 qf[NT][STEPS];
-    int at[NT], lo[NT], hi[NT];
     float slope2[NT];
-    int whole_from = 0, whole_end = INT_MAX, any_from = INT_MAX, any_end = 0;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const int r = 16 * n + i;
-        const Row w = is_prefix ? row_of<PREFIX>(p, min(r, rows - 1), 0, kv_head) : row_of<OWN>(p, min(r, rows - 1), b, kv_head, count);
-        at[n] = w.at;
-        lo[n] = w.lo;
-        hi[n] = w.hi;
+        const Row w = is_prefix ? row_of<PREFIX>(p, min(r, rows - 1), 0, kv_head) : row_of<OWN>(p, min(r, rows - 1), b, kv_head, item.length);
         slope2[n] = SHAPED && p.slopes ? p.slopes[w.head] * LOG2E : 0.0f;
-        whole_from = max(whole_from, w.lo);
-        whole_end = min(whole_end, w.hi);
-        if (w.hi > w.lo) {
-            any_from = min(any_from, w.lo);
-            any_end = max(any_end, w.hi);
-        }
         const half_t *q = (const half_t *) p.q + (w.b * p.q_batch + w.t * p.q_token + w.head * p.q_head);
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
@@ -794,20 +773,6 @@ __global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))
             qf[n][s] = I8 ? halfx8{x[0], x[2], x[1], x[3], x[4], x[6], x[5], x[7]} : x;
         }
     }
-#pragma unroll
-    for (int m = 1; m < 16; m <<= 1) {
-        whole_from = max(whole_from, __shfl_xor(whole_from, m));
-        whole_end = min(whole_end, __shfl_xor(whole_end, m));
-        any_from = min(any_from, __shfl_xor(any_from, m));
-        any_end = max(any_end, __shfl_xor(any_end, m));
-    }
-    whole_from = __builtin_amdgcn_readfirstlane(whole_from);
-    whole_end = __builtin_amdgcn_readfirstlane(whole_end);
-    any_from = __builtin_amdgcn_readfirstlane(any_from);
-    any_end = __builtin_amdgcn_readfirstlane(any_end);
-    int from = max(item.from, any_from & ~31), end = min(item.end, any_end);
-    if (from >= end) from = end = 0;  // (nothing to see: any_from may be INT_MAX, nothing may be added to it)
-
     floatx4 oacc[NT][DPL];
     float ref[NT], sum[NT];
 #pragma unroll
@@ -823,242 +788,294 @@ __global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))
     const char *kb = (const char *) p.k + kv_head * p.k_head * ELEM, *vb = (const char *) p.v + kv_head * p.v_head * ELEM;
     const bool v_live = i * DPL < p.width, k_whole = p.width == WP;
 
-    uint4 kreg[2][KP];
-    unsigned vreg[8][VW];
-    floatx4 kscale[2], vscale[2];
+    // INSIDE: two stretches one after the other, the sequence's first item begins with the prefix. (An instantiation of its own: the
+    // loop costs the others a tenth of their time.)
+    int taken = 0;  // steps of the stretch before, so that the waves go on in turn
+#pragma unroll 1
+    for (int stretch = INSIDE && item.nth == 0 ? 0 : 1; stretch < 2; stretch++) {
+        const bool shared = is_prefix || stretch == 0;
+        const int count = stretch == 0 ? p.prefix_tokens : item.length, item_from = stretch == 0 ? 0 : item.from, item_end = stretch == 0 ? count : item.end;
+        const int *table = shared ? p.prefix_table : p.tables + b * p.table_stride;
+        int pages[2] = {0, 0};
+        auto look_up = [&](int key0) {  // the pages of a step's tiles, ahead of their loads; behind the last key: none
+            if (PAGE16)
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
-        kscale[u] = vscale[u] = floatx4{1, 1, 1, 1};
-#pragma unroll
-        for (int c = 0; c < KP; c++) kreg[u][c] = uint4{0, 0, 0, 0};
-    }
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-#pragma unroll
-        for (int x = 0; x < VW; x++) vreg[e][x] = 0;
-    unsigned gone = 0, gone_next = 0;  // keys of the lane's 8 (4 u + e: key 16 u + 4 g + e) that are not there
-    const unsigned k_lane = PAGE16 ? (unsigned) (i * (int) p.k_token * ELEM + 16 * g) : 0;
-    const unsigned v_lane = PAGE16 ? (unsigned) ((4 * g * (int) p.v_token + i * DPL) * ELEM) : 0;
-
-    // the places of a step's tiles: page and token inside it (PAGE16)
-    int page_next[2] = {-1, -1};
-    unsigned in_next[2] = {0, 0};
-    auto place = [&](int key0) {
-        if (PAGE16) {
-            gone_next = 0;
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const unsigned j = (unsigned) (key0 + 16 * u);
-                page_next[u] = __builtin_amdgcn_readfirstlane(pages[u]);
-                in_next[u] = j - p.page_tokens.div(j) * p.page_tokens.d;
-                if ((unsigned) page_next[u] >= (unsigned) p.pages) gone_next |= 15u << (4 * u);
-            }
-        }
-    };
-    auto load_k = [&](int key0) {
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            if (PAGE16) {
-                if ((gone_next >> (4 * u)) & 1) continue;
-                const char *base = kb + (page_next[u] * p.k_page + in_next[u] * p.k_token) * ELEM;
-#pragma unroll
-                for (int c = 0; c < KP; c++)
-                    if (k_whole || 64 * c + 16 * g < p.width * ELEM) kreg[u][c] = *(const uint4 *) (base + (k_lane + 64 * c));
-            } else {
-                const int j = key0 + 16 * u + i, pg = j < count ? table[p.page_tokens.div((unsigned) j)] : -1;
-                const unsigned at_j = (unsigned) j - p.page_tokens.div((unsigned) j) * p.page_tokens.d;
-                const char *base = kb + (pg * p.k_page + at_j * p.k_token) * ELEM;
-                if ((unsigned) pg < (unsigned) p.pages)
-#pragma unroll
-                    for (int c = 0; c < KP; c++)
-                        if (64 * c + 16 * g < p.width * ELEM) kreg[u][c] = *(const uint4 *) (base + 64 * c + 16 * g);
-            }
-        }
-    };
-    auto load_scales = [&](int key0) {
-        if (!I8) return;
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            if (PAGE16) {
-                if ((gone_next >> (4 * u)) & 1) continue;
-                const long long s = ((long long) page_next[u] * p.kv_heads + kv_head) * p.page_tokens.d + in_next[u];
-                kscale[u] = *(const floatx4_any *) ((const char *) (p.k_scales + s) + (unsigned) (16 * g));
-                vscale[u] = *(const floatx4_any *) ((const char *) (p.v_scales + s) + (unsigned) (16 * g));
-            }
-        }
-    };
-    auto load_v = [&](int key0) {
-        if (!PAGE16) gone_next = 0;
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            if (PAGE16) {
-                if ((gone_next >> (4 * u)) & 1) continue;
-                const char *base = vb + (page_next[u] * p.v_page + in_next[u] * p.v_token) * ELEM;
-                if (v_live)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) load_words(base + (long long) e * p.v_token * ELEM + v_lane, vreg[4 * u + e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int j = key0 + 16 * u + 4 * g + e, pg = j < count ? table[p.page_tokens.div((unsigned) j)] : -1;
-                    const unsigned at_j = (unsigned) j - p.page_tokens.div((unsigned) j) * p.page_tokens.d;
-                    if ((unsigned) pg < (unsigned) p.pages) {
-                        if (v_live) load_words(vb + (pg * p.v_page + at_j * p.v_token + i * DPL) * ELEM, vreg[4 * u + e]);
-                        if (I8) {
-                            const long long s = ((long long) pg * p.kv_heads + kv_head) * p.page_tokens.d + at_j;
-                            kscale[u][e] = p.k_scales[s];
-                            vscale[u][e] = p.v_scales[s];
-                        }
-                    } else {
-                        gone_next |= 1u << (4 * u + e);
-                    }
+                for (int u = 0; u < 2; u++) {
+                    const int j = key0 + 16 * u;
+                    pages[u] = j < item_end ? table[p.page_tokens.div((unsigned) j)] : -1;
                 }
-            }
-        }
-    };
+        };
+        const int first_key = 32 * ((wave - taken) & (ROW_WAVES - 1));
+        if (item_from < item_end) look_up(item_from + first_key);
 
-    int key0 = from + 32 * wave;
-    if (key0 < end) {
-        if (from != item.from) look_up(key0);
-        place(key0);
-        load_k(key0);
-        load_scales(key0);
-        load_v(key0);
-        look_up(key0 + STRIDE);
-    }
-    while (key0 < end) {
-        gone = gone_next;
-        const int next = key0 + STRIDE;
-        const bool more = next < end;
-        if (more) place(next);
-        const bool masked = key0 < whole_from || key0 + 32 > min(whole_end, end) || __any(gone != 0);
-        floatx4 st[NT][2];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            halfx8 a[STEPS];
-#pragma unroll
-            for (int s = 0; s < STEPS; s++) {
-                if (I8) {
-                    const uint4 x = kreg[u][s / 2];
-                    a[s] = s % 2 ? widen(x.z, x.w) : widen(x.x, x.y);
-                } else {
-                    a[s] = __builtin_bit_cast(halfx8, kreg[u][I8 ? 0 : s]);
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                st[n][u] = floatx4{0, 0, 0, 0};
-#pragma unroll
-                for (int s = 0; s < STEPS; s++) st[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[s], qf[n][s], st[n][u], 0, 0, 0);
-            }
-        }
-        if (more) load_k(next);
-        float value_log[8];
-        if (I8)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                vscale[e / 4][e % 4] = fmaxf(vscale[e / 4][e % 4], 0x1p-40f);  // (values below 2^-33 are zeros of an f16 result)
-                value_log[e] = __builtin_amdgcn_logf(vscale[e / 4][e % 4]);
-            }
-        halfx8 weights[NT];
+        int at[NT], lo[NT], hi[NT];
+        int whole_from = 0, whole_end = INT_MAX, any_from = INT_MAX, any_end = 0;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            float top = -INFINITY, s2[8];
+            const int r = min(16 * n + i, rows - 1);
+            const Row w = !shared ? row_of<OWN>(p, r, b, kv_head, item.length) : row_of<PREFIX>(p, b * rows + r, 0, kv_head, is_prefix ? -1 : item.length);
+            at[n] = w.at;
+            lo[n] = w.lo;
+            hi[n] = w.hi;
+            whole_from = max(whole_from, w.lo);
+            whole_end = min(whole_end, w.hi);
+            if (w.hi > w.lo) {
+                any_from = min(any_from, w.lo);
+                any_end = max(any_end, w.hi);
+            }
+        }
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int key = key0 + 16 * (e / 4) + 4 * g + e % 4;
-                float x = st[n][e / 4][e % 4];
-                if (I8) x *= kscale[e / 4][e % 4];
-                if (SHAPED) {
-                    x = capped ? cap2 * tanh_fast(x * to_cap) : x * scale2;
-                    x = __builtin_fmaf(-slope2[n], fabsf((float) (at[n] - key)), x);
+        for (int m = 1; m < 16; m <<= 1) {
+            whole_from = max(whole_from, __shfl_xor(whole_from, m));
+            whole_end = min(whole_end, __shfl_xor(whole_end, m));
+            any_from = min(any_from, __shfl_xor(any_from, m));
+            any_end = max(any_end, __shfl_xor(any_end, m));
+        }
+        whole_from = __builtin_amdgcn_readfirstlane(whole_from);
+        whole_end = __builtin_amdgcn_readfirstlane(whole_end);
+        any_from = __builtin_amdgcn_readfirstlane(any_from);
+        any_end = __builtin_amdgcn_readfirstlane(any_end);
+        int from = max(item_from, any_from & ~31), end = min(item_end, any_end);
+        if (from >= end) from = end = 0;  // (nothing to see: any_from may be INT_MAX, nothing may be added to it)
+
+        uint4 kreg[2][KP];
+        unsigned vreg[8][VW];
+        floatx4 kscale[2], vscale[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            kscale[u] = vscale[u] = floatx4{1, 1, 1, 1};
+#pragma unroll
+            for (int c = 0; c < KP; c++) kreg[u][c] = uint4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+#pragma unroll
+            for (int x = 0; x < VW; x++) vreg[e][x] = 0;
+        unsigned gone = 0, gone_next = 0;  // keys of the lane's 8 (4 u + e: key 16 u + 4 g + e) that are not there
+        const unsigned k_lane = PAGE16 ? (unsigned) (i * (int) p.k_token * ELEM + 16 * g) : 0;
+        const unsigned v_lane = PAGE16 ? (unsigned) ((4 * g * (int) p.v_token + i * DPL) * ELEM) : 0;
+
+        // the places of a step's tiles: page and token inside it (PAGE16)
+        int page_next[2] = {-1, -1};
+        unsigned in_next[2] = {0, 0};
+        auto place = [&](int key0) {
+            if (PAGE16) {
+                gone_next = 0;
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const unsigned j = (unsigned) (key0 + 16 * u);
+                    page_next[u] = __builtin_amdgcn_readfirstlane(pages[u]);
+                    in_next[u] = j - p.page_tokens.div(j) * p.page_tokens.d;
+                    if ((unsigned) page_next[u] >= (unsigned) p.pages) gone_next |= 15u << (4 * u);
+                }
+            }
+        };
+        auto load_k = [&](int key0) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                if (PAGE16) {
+                    if ((gone_next >> (4 * u)) & 1) continue;
+                    const char *base = kb + (page_next[u] * p.k_page + in_next[u] * p.k_token) * ELEM;
+#pragma unroll
+                    for (int c = 0; c < KP; c++)
+                        if (k_whole || 64 * c + 16 * g < p.width * ELEM) kreg[u][c] = *(const uint4 *) (base + (k_lane + 64 * c));
                 } else {
-                    x *= scale2;
+                    const int j = key0 + 16 * u + i, pg = j < count ? table[p.page_tokens.div((unsigned) j)] : -1;
+                    const unsigned at_j = (unsigned) j - p.page_tokens.div((unsigned) j) * p.page_tokens.d;
+                    const char *base = kb + (pg * p.k_page + at_j * p.k_token) * ELEM;
+                    if ((unsigned) pg < (unsigned) p.pages)
+#pragma unroll
+                        for (int c = 0; c < KP; c++)
+                            if (64 * c + 16 * g < p.width * ELEM) kreg[u][c] = *(const uint4 *) (base + 64 * c + 16 * g);
                 }
-                if (masked && ((unsigned) (key - lo[n]) >= (unsigned) (hi[n] - lo[n]) || key >= end || ((gone >> e) & 1))) x = -INFINITY;
-                s2[e] = x;
-                top = fmaxf(top, I8 ? x + value_log[e] : x);
             }
-            if (__any(top > ref[n] + SLACK)) {
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float new_ref = fmaxf(ref[n], top);
-                const float alpha = __builtin_amdgcn_exp2f(ref[n] - (new_ref == -INFINITY ? 0.0f : new_ref));
-                ref[n] = new_ref;
-                sum[n] *= alpha;
+        };
+        auto load_scales = [&](int key0) {
+            if (!I8) return;
 #pragma unroll
-                for (int d = 0; d < DPL; d++) oacc[n][d] *= alpha;
-            }
-            const float minus = ref[n] == -INFINITY ? 0.0f : ref[n];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float x = __builtin_amdgcn_exp2f(s2[e] - minus);
-                sum[n] += x;
-                weights[n][e] = (half_t) (I8 ? x * vscale[e / 4][e % 4] : x);
-            }
-        }
-        if (more && PAGE16) load_scales(next);
-        unsigned bad = 0;  // keys of the lane's 8 whose values hold an infinity or NaN, where not every row sees every key
-        if (!I8 && masked) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const bool there = key0 + 16 * (e / 4) + 4 * g + e % 4 < count && !((gone >> e) & 1);
-                bool any = false;
-#pragma unroll
-                for (int x = 0; x < VW; x++) {
-                    if (!there) vreg[e][x] = 0;
-                    any |= (vreg[e][x] & 0x7c00u) == 0x7c00u || (vreg[e][x] & 0x7c000000u) == 0x7c000000u;
+            for (int u = 0; u < 2; u++) {
+                if (PAGE16) {
+                    if ((gone_next >> (4 * u)) & 1) continue;
+                    const long long s = ((long long) page_next[u] * p.kv_heads + kv_head) * p.page_tokens.d + in_next[u];
+                    kscale[u] = *(const floatx4_any *) ((const char *) (p.k_scales + s) + (unsigned) (16 * g));
+                    vscale[u] = *(const floatx4_any *) ((const char *) (p.v_scales + s) + (unsigned) (16 * g));
                 }
-                // (of the 16 lanes of a group)
-                if ((__ballot(any) >> (16 * g)) & 0xffffu) bad |= 1u << e;
             }
-        }
-        const bool any_bad = !I8 && __any(bad != 0);
+        };
+        auto load_v = [&](int key0) {
+            if (!PAGE16) gone_next = 0;
 #pragma unroll
-        for (int d = 0; d < DPL; d++) {
-            unsigned pair[4];
+            for (int u = 0; u < 2; u++) {
+                if (PAGE16) {
+                    if ((gone_next >> (4 * u)) & 1) continue;
+                    const char *base = vb + (page_next[u] * p.v_page + in_next[u] * p.v_token) * ELEM;
+                    if (v_live)
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if (I8) {
-                    const unsigned sel = (unsigned) (d % 4) | 0x0c00u | (unsigned) (4 + d % 4) << 16 | 0x0c000000u;
-                    pair[k] = pk_sub_1152(__builtin_amdgcn_perm(vreg[2 * k + 1][d / 4] ^ 0x80808080u, vreg[2 * k][d / 4] ^ 0x80808080u, sel) | 0x64006400u);
+                        for (int e = 0; e < 4; e++) load_words(base + (long long) e * p.v_token * ELEM + v_lane, vreg[4 * u + e]);
                 } else {
-                    pair[k] = __builtin_amdgcn_perm(vreg[2 * k + 1][I8 ? 0 : d / 2], vreg[2 * k][I8 ? 0 : d / 2], d % 2 ? 0x07060302u : 0x05040100u);
-                }
-            }
-            const halfx8 a = __builtin_bit_cast(halfx8, uint4{pair[0], pair[1], pair[2], pair[3]});
-            const halfx8 good = any_bad ? finite_or_zero(a) : a;
 #pragma unroll
-            for (int n = 0; n < NT; n++) oacc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(good, weights[n], oacc[n][d], 0, 0, 0);
-        }
-        if (any_bad) {
-            // (as in the kernel above: what is not finite is added for the queries that see its key)
-#pragma unroll 1
-            for (int key = 0; key < 32; key++) {
-                const int group = (key % 16) / 4, nth = 4 * (key / 16) + key % 4;
-                if (!__any(g == group && ((bad >> nth) & 1))) continue;
-#pragma unroll
-                for (int d = 0; d < DPL; d++)
-#pragma unroll
-                    for (int v = 0; v < 4; v++) {
-                        // register v of product d: dim (4 g + v) DPL + d, which lane (4 g + v, group) holds
-                        unsigned word = 0;
-#pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            if (e == nth) word = vreg[e][I8 ? 0 : d / 2];
-                        const unsigned got = __shfl(word, 16 * group + 4 * g + v);
-                        const float x = (float) __builtin_bit_cast(half_t, (unsigned short) (d % 2 ? got >> 16 : got));
-#pragma unroll
-                        for (int n = 0; n < NT; n++)
-                            if ((unsigned) (key0 + key - lo[n]) < (unsigned) (hi[n] - lo[n])) oacc[n][d][v] += x - x == 0.0f ? 0.0f : x;
+                    for (int e = 0; e < 4; e++) {
+                        const int j = key0 + 16 * u + 4 * g + e, pg = j < count ? table[p.page_tokens.div((unsigned) j)] : -1;
+                        const unsigned at_j = (unsigned) j - p.page_tokens.div((unsigned) j) * p.page_tokens.d;
+                        if ((unsigned) pg < (unsigned) p.pages) {
+                            if (v_live) load_words(vb + (pg * p.v_page + at_j * p.v_token + i * DPL) * ELEM, vreg[4 * u + e]);
+                            if (I8) {
+                                const long long s = ((long long) pg * p.kv_heads + kv_head) * p.page_tokens.d + at_j;
+                                kscale[u][e] = p.k_scales[s];
+                                vscale[u][e] = p.v_scales[s];
+                            }
+                        } else {
+                            gone_next |= 1u << (4 * u + e);
+                        }
                     }
+                }
             }
+        };
+
+        int key0 = from + first_key;
+        if (key0 < end) {
+            if (from != item_from) look_up(key0);
+            place(key0);
+            load_k(key0);
+            load_scales(key0);
+            load_v(key0);
+            look_up(key0 + STRIDE);
         }
-        if (more) {
-            load_v(next);
-            look_up(next + STRIDE);
+        while (key0 < end) {
+            gone = gone_next;
+            const int next = key0 + STRIDE;
+            const bool more = next < end;
+            if (more) place(next);
+            const bool masked = key0 < whole_from || key0 + 32 > min(whole_end, end) || __any(gone != 0);
+            floatx4 st[NT][2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                halfx8 a[STEPS];
+#pragma unroll
+                for (int s = 0; s < STEPS; s++) {
+                    if (I8) {
+                        const uint4 x = kreg[u][s / 2];
+                        a[s] = s % 2 ? widen(x.z, x.w) : widen(x.x, x.y);
+                    } else {
+                        a[s] = __builtin_bit_cast(halfx8, kreg[u][I8 ? 0 : s]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    st[n][u] = floatx4{0, 0, 0, 0};
+#pragma unroll
+                    for (int s = 0; s < STEPS; s++) st[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[s], qf[n][s], st[n][u], 0, 0, 0);
+                }
+            }
+            if (more) load_k(next);
+            float value_log[8];
+            if (I8)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    vscale[e / 4][e % 4] = fmaxf(vscale[e / 4][e % 4], 0x1p-40f);  // (values below 2^-33 are zeros of an f16 result)
+                    value_log[e] = __builtin_amdgcn_logf(vscale[e / 4][e % 4]);
+                }
+            halfx8 weights[NT];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                float top = -INFINITY, s2[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int key = key0 + 16 * (e / 4) + 4 * g + e % 4;
+                    float x = st[n][e / 4][e % 4];
+                    if (I8) x *= kscale[e / 4][e % 4];
+                    if (SHAPED) {
+                        x = capped ? cap2 * tanh_fast(x * to_cap) : x * scale2;
+                        x = __builtin_fmaf(-slope2[n], fabsf((float) (at[n] - key)), x);
+                    } else {
+                        x *= scale2;
+                    }
+                    if (masked && ((unsigned) (key - lo[n]) >= (unsigned) (hi[n] - lo[n]) || key >= end || ((gone >> e) & 1))) x = -INFINITY;
+                    s2[e] = x;
+                    top = fmaxf(top, I8 ? x + value_log[e] : x);
+                }
+                if (__any(top > ref[n] + SLACK)) {
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const float new_ref = fmaxf(ref[n], top);
+                    const float alpha = __builtin_amdgcn_exp2f(ref[n] - (new_ref == -INFINITY ? 0.0f : new_ref));
+                    ref[n] = new_ref;
+                    sum[n] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < DPL; d++) oacc[n][d] *= alpha;
+                }
+                const float minus = ref[n] == -INFINITY ? 0.0f : ref[n];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float x = __builtin_amdgcn_exp2f(s2[e] - minus);
+                    sum[n] += x;
+                    weights[n][e] = (half_t) (I8 ? x * vscale[e / 4][e % 4] : x);
+                }
+            }
+            if (more && PAGE16) load_scales(next);
+            unsigned bad = 0;  // keys of the lane's 8 whose values hold an infinity or NaN, where not every row sees every key
+            if (!I8 && masked) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const bool there = key0 + 16 * (e / 4) + 4 * g + e % 4 < count && !((gone >> e) & 1);
+                    bool any = false;
+#pragma unroll
+                    for (int x = 0; x < VW; x++) {
+                        if (!there) vreg[e][x] = 0;
+                        any |= (vreg[e][x] & 0x7c00u) == 0x7c00u || (vreg[e][x] & 0x7c000000u) == 0x7c000000u;
+                    }
+                    // (of the 16 lanes of a group)
+                    if ((__ballot(any) >> (16 * g)) & 0xffffu) bad |= 1u << e;
+                }
+            }
+            const bool any_bad = !I8 && __any(bad != 0);
+#pragma unroll
+            for (int d = 0; d < DPL; d++) {
+                unsigned pair[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    if (I8) {
+                        const unsigned sel = (unsigned) (d % 4) | 0x0c00u | (unsigned) (4 + d % 4) << 16 | 0x0c000000u;
+                        pair[k] = pk_sub_1152(__builtin_amdgcn_perm(vreg[2 * k + 1][d / 4] ^ 0x80808080u, vreg[2 * k][d / 4] ^ 0x80808080u, sel) | 0x64006400u);
+                    } else {
+                        pair[k] = __builtin_amdgcn_perm(vreg[2 * k + 1][I8 ? 0 : d / 2], vreg[2 * k][I8 ? 0 : d / 2], d % 2 ? 0x07060302u : 0x05040100u);
+                    }
+                }
+                const halfx8 a = __builtin_bit_cast(halfx8, uint4{pair[0], pair[1], pair[2], pair[3]});
+                const halfx8 good = any_bad ? finite_or_zero(a) : a;
+#pragma unroll
+                for (int n = 0; n < NT; n++) oacc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(good, weights[n], oacc[n][d], 0, 0, 0);
+            }
+            if (any_bad) {
+                // (as in the kernel above: what is not finite is added for the queries that see its key)
+#pragma unroll 1
+                for (int key = 0; key < 32; key++) {
+                    const int group = (key % 16) / 4, nth = 4 * (key / 16) + key % 4;
+                    if (!__any(g == group && ((bad >> nth) & 1))) continue;
+#pragma unroll
+                    for (int d = 0; d < DPL; d++)
+#pragma unroll
+                        for (int v = 0; v < 4; v++) {
+                            // register v of product d: dim (4 g + v) DPL + d, which lane (4 g + v, group) holds
+                            unsigned word = 0;
+#pragma unroll
+                            for (int e = 0; e < 8; e++)
+                                if (e == nth) word = vreg[e][I8 ? 0 : d / 2];
+                            const unsigned got = __shfl(word, 16 * group + 4 * g + v);
+                            const float x = (float) __builtin_bit_cast(half_t, (unsigned short) (d % 2 ? got >> 16 : got));
+#pragma unroll
+                            for (int n = 0; n < NT; n++)
+                                if ((unsigned) (key0 + key - lo[n]) < (unsigned) (hi[n] - lo[n])) oacc[n][d][v] += x - x == 0.0f ? 0.0f : x;
+                        }
+                }
+            }
+            if (more) {
+                load_v(next);
+                look_up(next + STRIDE);
+            }
+            key0 = next;
         }
-        key0 = next;
+        taken = (end - from + 31) / 32;
     }
 
     // ---- the waves' parts into one
@@ -1078,7 +1095,7 @@ __global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))
                 *(floatx4 *) &os[wave][16 * n + i][(4 * g + v) * DPL + d] = floatx4{oacc[n][d][v], oacc[n][d + 1][v], oacc[n][d + 2][v], oacc[n][d + 3][v]};
     }
     __syncthreads();
-    const bool direct = !is_prefix && p.prefix_tokens == 0 && item.items == 1;
+    const bool direct = !is_prefix && (p.prefix_tokens == 0 || INSIDE) && item.items == 1;
     for (int e = threadIdx.x; e < rows * (WP / 4); e += ROW_THREADS) {
         const int r = e / (WP / 4), d = 4 * (e % (WP / 4));
         float top = -INFINITY, total = 0.0f;
@@ -1093,7 +1110,7 @@ __global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))
         }
         if (direct) {
             const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
-            const Row w = row_of<OWN>(p, r, b, kv_head, count);
+            const Row w = row_of<OWN>(p, r, b, kv_head, item.length);
             if (d < p.width)
                 *(halfx4_any *) ((half_t *) p.out + (w.b * p.o_batch + w.t * p.o_token + w.head * p.o_head + d)) =
                     halfx4{(half_t) (x[0] * inv), (half_t) (x[1] * inv), (half_t) (x[2] * inv), (half_t) (x[3] * inv)};
@@ -1129,7 +1146,7 @@ __global__ __launch_bounds__(64 * WAVES) void join_attention_kernel(ServingAtten
         at[0] = (long long) kv_head * p.prefix_splits * prefix_rows + prefix_row;
         apart[0] = prefix_rows;
         count[0] = p.prefix_splits;
-    } else if (p.prefix_tokens > 0) {
+    } else if (p.prefix_tokens > 0 && !p.prefix_inside) {
         const int2 items = ((const int2 *) p.part_items)[0];
         at[0] = p.row_prefix_part + ((long long) items.x * p.kv_heads + kv_head) * prefix_rows + prefix_row;
         apart[0] = p.kv_heads * prefix_rows;
@@ -1141,7 +1158,7 @@ __global__ __launch_bounds__(64 * WAVES) void join_attention_kernel(ServingAtten
         count[1] = p.own_splits;
     } else {
         const int2 items = ((const int2 *) p.part_items)[b + 1];
-        if (p.prefix_tokens == 0 && items.y == 1) return;  // (written where it was computed)
+        if ((p.prefix_tokens == 0 || p.prefix_inside) && items.y == 1) return;  // (written where it was computed)
         at[1] = p.row_own_part + ((long long) items.x * p.kv_heads + kv_head) * own_rows + own_row;
         apart[1] = p.kv_heads * own_rows;
         count[1] = items.y;
@@ -1195,6 +1212,7 @@ struct Plan {
     int own_rows;             // per sequence and head of keys
     long long prefix_rows;
     bool own_in_rows, prefix_in_rows;  // which kernel
+    bool prefix_inside;                // of every sequence's own rows, see row_attention_kernel
     long long own_tiles, prefix_tiles;
     int own_splits, prefix_splits;     // of the tile kernel
     long long items;                   // of the row kernel, at most
@@ -1231,18 +1249,25 @@ Plan plan_for(const ServingAttentionParams &p) {
     l.prefix_rows = (long long) p.batch * l.own_rows;
     // a tile of 16 or 32 rows keeps the keys streaming; more rows are worth staging them for
     l.own_in_rows = p.paged && l.own_rows <= 32;
-    l.prefix_in_rows = p.prefix_tokens > 0 && l.prefix_rows <= 32;
     const long long pairs = (long long) p.batch * p.kv_heads;
+    // A short prefix is read again for every sequence, which takes a workgroup, one per compute unit at a time, about a
+    // microsecond for 128 keys, and saves the launch of the tiles and the join, or only the join where all rows of the batch fit this
+    // kernel. (64 sequences of up to 700 tokens, 8 heads of keys, two rounds of workgroups: 18 shared tokens 27 us against
+    // 45, 512 37 against 46, 1024 48 against 49, 2048 70 against 51. One sequence: 18 14 against 19, 1024 23 against 21.)
+    const bool few_rows = l.prefix_rows <= 32;
+    l.prefix_inside = l.own_in_rows && l.own_rows <= 16 && p.prefix_tokens > 0 && p.prefix_tokens * ((pairs + 255) / 256) <= (few_rows ? 768 : 1792);
+    l.prefix_in_rows = !l.prefix_inside && p.prefix_tokens > 0 && few_rows;
+    const bool prefix_apart = !l.prefix_inside && p.prefix_tokens > 0;
     const int waves = tile_waves(l.wp, p.k_scales != nullptr), tile_rows = 32 * waves;
     if (!l.own_in_rows) {
         l.own_tiles = (l.own_rows + tile_rows - 1) / tile_rows;
         const long long keys = p.paged ? p.table_tokens : p.keys, tile_tokens = tile_rows / (p.heads / p.kv_heads) + 2;
         const long long longest = p.window > 0 ? std::min(keys, p.window + tile_tokens) : keys;
         const long long mean = p.paged || p.causal ? std::min(longest, std::max(keys - p.queries / 2, 1ll)) : longest;
-        l.own_splits = splits_for(l.own_tiles * pairs, pairs * l.own_rows, longest, mean, waves, p.prefix_tokens > 0);
+        l.own_splits = splits_for(l.own_tiles * pairs, pairs * l.own_rows, longest, mean, waves, prefix_apart);
         l.own_parts = l.own_splits * pairs * l.own_rows;
     }
-    if (p.prefix_tokens > 0 && !l.prefix_in_rows) {
+    if (prefix_apart && !l.prefix_in_rows) {
         l.prefix_tiles = (l.prefix_rows + tile_rows - 1) / tile_rows;
         l.prefix_splits = splits_for(l.prefix_tiles * p.kv_heads, p.kv_heads * l.prefix_rows, p.prefix_tokens, p.prefix_tokens, waves, true);
         l.prefix_parts = (long long) l.prefix_splits * p.kv_heads * l.prefix_rows;
@@ -1256,7 +1281,7 @@ Plan plan_for(const ServingAttentionParams &p) {
         l.own_parts = l.items * p.kv_heads * l.own_rows;
         if (l.prefix_in_rows) l.prefix_parts = l.items * p.kv_heads * l.prefix_rows;
     }
-    l.join = p.prefix_tokens > 0 || (l.own_in_rows ? l.items > p.batch : l.own_splits > 1);
+    l.join = prefix_apart || (l.own_in_rows ? l.items > p.batch : l.own_splits > 1);
     if (!l.join) l.own_parts = 0;
     return l;
 }
@@ -1291,21 +1316,27 @@ int launch_tiles_for(const ServingAttentionParams &p, int stretch, unsigned work
                              : launch_tiles_of<WP, PREFIX>(p, workgroups, splits, stream);
 }
 
-template <int WP, int NT, bool I8>
+template <int WP, int NT, bool I8, bool INSIDE>
 int launch_rows(const ServingAttentionParams &p, unsigned workgroups, int with_prefix, hipStream_t stream) {
     const bool shaped = p.cap > 0.0f || p.slopes, page16 = p.page_tokens.d % 16 == 0 && p.k_token <= 1 << 25;
     const dim3 grid(workgroups), block(ROW_THREADS);
-    if (shaped && page16) hipLaunchKernelGGL((row_attention_kernel<WP, NT, I8, true, true>), grid, block, 0, stream, p, with_prefix);
-    else if (shaped) hipLaunchKernelGGL((row_attention_kernel<WP, NT, I8, true, false>), grid, block, 0, stream, p, with_prefix);
-    else if (page16) hipLaunchKernelGGL((row_attention_kernel<WP, NT, I8, false, true>), grid, block, 0, stream, p, with_prefix);
-    else hipLaunchKernelGGL((row_attention_kernel<WP, NT, I8, false, false>), grid, block, 0, stream, p, with_prefix);
+    if (shaped && page16) hipLaunchKernelGGL((row_attention_kernel<WP, NT, I8, true, true, INSIDE>), grid, block, 0, stream, p, with_prefix);
+    else if (shaped) hipLaunchKernelGGL((row_attention_kernel<WP, NT, I8, true, false, INSIDE>), grid, block, 0, stream, p, with_prefix);
+    else if (page16) hipLaunchKernelGGL((row_attention_kernel<WP, NT, I8, false, true, INSIDE>), grid, block, 0, stream, p, with_prefix);
+    else hipLaunchKernelGGL((row_attention_kernel<WP, NT, I8, false, false, INSIDE>), grid, block, 0, stream, p, with_prefix);
     return (int) hipGetLastError();
+}
+
+template <int WP, bool I8>
+int launch_rows_of(const ServingAttentionParams &p, unsigned workgroups, bool two_tiles, int with_prefix, hipStream_t stream) {
+    if (p.prefix_inside) return launch_rows<WP, 1, I8, true>(p, workgroups, with_prefix, stream);
+    return two_tiles ? launch_rows<WP, 2, I8, false>(p, workgroups, with_prefix, stream) : launch_rows<WP, 1, I8, false>(p, workgroups, with_prefix, stream);
 }
 
 template <int WP>
 int launch_rows_for(const ServingAttentionParams &p, unsigned workgroups, bool two_tiles, int with_prefix, hipStream_t stream) {
-    if (p.k_scales) return two_tiles ? launch_rows<WP, 2, true>(p, workgroups, with_prefix, stream) : launch_rows<WP, 1, true>(p, workgroups, with_prefix, stream);
-    return two_tiles ? launch_rows<WP, 2, false>(p, workgroups, with_prefix, stream) : launch_rows<WP, 1, false>(p, workgroups, with_prefix, stream);
+    return p.k_scales ? launch_rows_of<WP, true>(p, workgroups, two_tiles, with_prefix, stream)
+                      : launch_rows_of<WP, false>(p, workgroups, two_tiles, with_prefix, stream);
 }
 
 template <int WP, int PARTS>
@@ -1336,6 +1367,7 @@ int launch_serving_attention(const ServingAttentionParams &given, void *workspac
     p.part_items = l.own_in_rows ? (int32_t *) ((char *) stats + round256(parts * 8)) : nullptr;
     p.row_prefix_part = 0;
     p.row_own_part = l.prefix_parts;
+    p.prefix_inside = l.prefix_inside;
     p.prefix_splits = l.prefix_splits;
     p.own_splits = l.own_splits;
     const long long pairs = (long long) p.batch * p.kv_heads;

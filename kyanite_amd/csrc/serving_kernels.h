@@ -71,6 +71,7 @@ struct ServingAttentionParams {
     int32_t *part_items;  // [stretch][first item, items], the prefix first
     long long row_prefix_part, row_own_part;
     int prefix_splits, own_splits;
+    int prefix_inside;  // the workgroups of a sequence's own keys take the prefix as well
 };
 int launch_serving_attention(const ServingAttentionParams &p, void *workspace, ihipStream_t *stream);
 size_t serving_attention_workspace(const ServingAttentionParams &p);

@@ -268,6 +268,12 @@ CACHED_CASES = {
     "many_sequences": dict(dtype=DType.I8, kv=1, group=2, width=64, page=16, lengths=[(13 * i) % 70 for i in range(150)]),
     "long_and_short": dict(dtype=DType.I8, kv=1, group=2, width=64, page=16, lengths=[9000, 5, 0, 2500]),
     "long_f16_wide_rows": dict(dtype=DType.F16, kv=1, group=4, width=128, page=16, lengths=[5000, 40], queries=8),
+    "prefix_apart": dict(dtype=DType.I8, kv=2, group=4, width=128, page=16, lengths=[(7 * i) % 60 for i in range(40)], prefix=1801, lost=[(-1, 3), (2, 0)]),
+    "prefix_apart_f16": dict(dtype=DType.F16, kv=1, group=4, width=64, page=48, lengths=[(7 * i) % 60 for i in range(20)], prefix=1999, cap=9.0, slopes=True, window=1900),
+    "prefix_apart_few_rows": dict(dtype=DType.I8, kv=2, group=4, width=128, page=16, lengths=[50, 0, 1300], prefix=1000, queries=2),
+    "prefix_inside_several_items": dict(dtype=DType.I8, kv=2, group=4, width=128, page=16, lengths=[3000, 0, 5, 1300], prefix=333, queries=3),
+    "prefix_inside_window": dict(dtype=DType.F16, kv=1, group=8, width=96, page=16, lengths=[30, 400, 5], prefix=200, window=100, queries=2, slopes=True),
+    "prefix_inside_lost": dict(dtype=DType.F16, kv=1, group=4, width=128, page=7, lengths=[20, 3, 0], queries=3, prefix=50, lost=[(-1, 0), (-1, 6), (0, 1)], poison=True),
     "many_prompts_over_the_cache": dict(dtype=DType.F16, kv=2, group=1, width=128, page=16, lengths=[40 + (9 * i) % 100 for i in range(200)], queries=40, poison=True),
     "many_prompts_over_the_cache_i8": dict(dtype=DType.I8, kv=2, group=1, width=64, page=16, lengths=[(9 * i) % 120 for i in range(200)], queries=40, prefix=100, cap=9.0),
     "many_heads_of_one": dict(dtype=DType.I8, kv=1, group=71, width=64, page=16, lengths=[300, 4]),
