@@ -1203,10 +1203,12 @@ __global__ __launch_bounds__(64 * WAVES) void join_attention_kernel(ServingAtten
 
 // ---- plans ---------------------------------------------------------------------------------------------------------
 
-// Whole numbers are widened as they are staged, work that eight waves share better than four (16384 shared keys of width 128
-// for 256 rows of 8 heads: 51.6 -> 44.1 us); f16 only passes through, and smaller workgroups wait less for each other (8192
-// tokens of 32 heads: 884 us against 915).
-constexpr int tile_waves(int wp, bool i8) { return wp == 128 && i8 ? 8 : 4; }
+// Waves for the rows of a tile, 32 rows each. Whole numbers are widened as they are staged, work that eight waves share better
+// than four (16384 shared keys of width 128 for 256 rows of 8 heads, and what goes with them: 76 us against 99). f16 only
+// passes through; eight waves still stage once for twice the rows, which pays where that leaves tiles enough to even out
+// their lengths (32 heads: 8192 tokens 627 us against 663, 4096 tokens 175 against 190, but 2048 tokens 96 against 74). `rows`:
+// of a sequence and head of keys, `pairs` of which there are.
+int tile_waves(int wp, bool i8, long long rows, long long pairs) { return wp == 128 && (i8 || (rows >= 1024 && rows * pairs >= 1024 * 128)) ? 8 : 4; }
 
 struct Plan {
     int own_rows;             // per sequence and head of keys
@@ -1215,6 +1217,7 @@ struct Plan {
     bool prefix_inside;                // of every sequence's own rows, see row_attention_kernel
     long long own_tiles, prefix_tiles;
     int own_splits, prefix_splits;     // of the tile kernel
+    int own_waves, prefix_waves;       // for the rows of a tile
     long long items;                   // of the row kernel, at most
     bool join;
     long long prefix_parts, own_parts;  // rows of partial results
@@ -1258,18 +1261,21 @@ Plan plan_for(const ServingAttentionParams &p) {
     l.prefix_inside = l.own_in_rows && l.own_rows <= 16 && p.prefix_tokens > 0 && p.prefix_tokens * ((pairs + 255) / 256) <= (few_rows ? 768 : 1792);
     l.prefix_in_rows = !l.prefix_inside && p.prefix_tokens > 0 && few_rows;
     const bool prefix_apart = !l.prefix_inside && p.prefix_tokens > 0;
-    const int waves = tile_waves(l.wp, p.k_scales != nullptr), tile_rows = 32 * waves;
+    const bool i8 = p.k_scales != nullptr;
     if (!l.own_in_rows) {
+        l.own_waves = tile_waves(l.wp, i8, l.own_rows, pairs);
+        const int tile_rows = 32 * l.own_waves;
         l.own_tiles = (l.own_rows + tile_rows - 1) / tile_rows;
         const long long keys = p.paged ? p.table_tokens : p.keys, tile_tokens = tile_rows / (p.heads / p.kv_heads) + 2;
         const long long longest = p.window > 0 ? std::min(keys, p.window + tile_tokens) : keys;
         const long long mean = p.paged || p.causal ? std::min(longest, std::max(keys - p.queries / 2, 1ll)) : longest;
-        l.own_splits = splits_for(l.own_tiles * pairs, pairs * l.own_rows, longest, mean, waves, prefix_apart);
+        l.own_splits = splits_for(l.own_tiles * pairs, pairs * l.own_rows, longest, mean, l.own_waves, prefix_apart);
         l.own_parts = l.own_splits * pairs * l.own_rows;
     }
     if (prefix_apart && !l.prefix_in_rows) {
-        l.prefix_tiles = (l.prefix_rows + tile_rows - 1) / tile_rows;
-        l.prefix_splits = splits_for(l.prefix_tiles * p.kv_heads, p.kv_heads * l.prefix_rows, p.prefix_tokens, p.prefix_tokens, waves, true);
+        l.prefix_waves = tile_waves(l.wp, i8, l.prefix_rows, p.kv_heads);
+        l.prefix_tiles = (l.prefix_rows + 32 * l.prefix_waves - 1) / (32 * l.prefix_waves);
+        l.prefix_splits = splits_for(l.prefix_tiles * p.kv_heads, p.kv_heads * l.prefix_rows, p.prefix_tokens, p.prefix_tokens, l.prefix_waves, true);
         l.prefix_parts = (long long) l.prefix_splits * p.kv_heads * l.prefix_rows;
     }
     if (l.own_in_rows) {
@@ -1288,9 +1294,9 @@ Plan plan_for(const ServingAttentionParams &p) {
 
 size_t round256(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-template <int WP, int STRETCH, bool I8, int KG>
+template <int WP, int STRETCH, bool I8, int RW, int KG>
 int launch_tiles(const ServingAttentionParams &p, unsigned workgroups, int splits, hipStream_t stream) {
-    constexpr int TW = tile_waves(WP, I8) * KG;
+    constexpr int TW = RW * KG;
     const dim3 grid(workgroups, (unsigned) splits), block(64 * TW);
     if (p.cap > 0.0f || p.slopes) hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, true, TW, KG>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, false, TW, KG>), grid, block, 0, stream, p);
@@ -1301,19 +1307,21 @@ int launch_tiles(const ServingAttentionParams &p, unsigned workgroups, int split
 // workgroups overlap better than two groups, which wait at the same barriers: with 32 heads 1024 tokens, 256 workgroups, take 30
 // us in two groups and 33 without, 1536 tokens, 384 workgroups, 44 and 52, but 3000 tokens, 752 workgroups, 128 and 104.)
 template <int WP, int STRETCH>
-int launch_tiles_of(const ServingAttentionParams &p, unsigned workgroups, int splits, hipStream_t stream) {
+int launch_tiles_of(const ServingAttentionParams &p, int waves, unsigned workgroups, int splits, hipStream_t stream) {
     if constexpr (STRETCH != PROMPT)
-        if (p.k_scales) return launch_tiles<WP, STRETCH, true, 1>(p, workgroups, splits, stream);
+        if (p.k_scales) return launch_tiles<WP, STRETCH, true, WP == 128 ? 8 : 4, 1>(p, workgroups, splits, stream);
+    if constexpr (WP == 128)
+        if (waves == 8) return launch_tiles<WP, STRETCH, false, 8, 1>(p, workgroups, splits, stream);
     const int keys = STRETCH == PROMPT ? p.keys : STRETCH == OWN ? p.table_tokens : p.prefix_tokens;  // (one block cannot be shared)
-    return (long long) workgroups * splits <= 384 && keys > 64 ? launch_tiles<WP, STRETCH, false, 2>(p, workgroups, splits, stream)
-                                                               : launch_tiles<WP, STRETCH, false, 1>(p, workgroups, splits, stream);
+    return (long long) workgroups * splits <= 384 && keys > 64 ? launch_tiles<WP, STRETCH, false, 4, 2>(p, workgroups, splits, stream)
+                                                               : launch_tiles<WP, STRETCH, false, 4, 1>(p, workgroups, splits, stream);
 }
 
 template <int WP>
-int launch_tiles_for(const ServingAttentionParams &p, int stretch, unsigned workgroups, int splits, hipStream_t stream) {
-    return stretch == PROMPT ? launch_tiles_of<WP, PROMPT>(p, workgroups, splits, stream)
-         : stretch == OWN    ? launch_tiles_of<WP, OWN>(p, workgroups, splits, stream)
-                             : launch_tiles_of<WP, PREFIX>(p, workgroups, splits, stream);
+int launch_tiles_for(const ServingAttentionParams &p, int stretch, int waves, unsigned workgroups, int splits, hipStream_t stream) {
+    return stretch == PROMPT ? launch_tiles_of<WP, PROMPT>(p, waves, workgroups, splits, stream)
+         : stretch == OWN    ? launch_tiles_of<WP, OWN>(p, waves, workgroups, splits, stream)
+                             : launch_tiles_of<WP, PREFIX>(p, waves, workgroups, splits, stream);
 }
 
 template <int WP, int NT, bool I8, bool INSIDE>
@@ -1375,7 +1383,7 @@ int launch_serving_attention(const ServingAttentionParams &given, void *workspac
         p.part_values = values;
         p.part_stats = stats;
         const unsigned workgroups = (unsigned) (l.prefix_tiles * p.kv_heads);
-        const int e = l.wp == 64 ? launch_tiles_for<64>(p, PREFIX, workgroups, l.prefix_splits, stream) : launch_tiles_for<128>(p, PREFIX, workgroups, l.prefix_splits, stream);
+        const int e = l.wp == 64 ? launch_tiles_for<64>(p, PREFIX, l.prefix_waves, workgroups, l.prefix_splits, stream) : launch_tiles_for<128>(p, PREFIX, l.prefix_waves, workgroups, l.prefix_splits, stream);
         if (e != 0) return e;
     }
     if (!l.own_in_rows) {
@@ -1383,7 +1391,7 @@ int launch_serving_attention(const ServingAttentionParams &given, void *workspac
         p.part_stats = l.join ? stats + 2 * l.prefix_parts : nullptr;
         const unsigned workgroups = (unsigned) (l.own_tiles * pairs);
         const int stretch = p.paged ? OWN : PROMPT;
-        const int e = l.wp == 64 ? launch_tiles_for<64>(p, stretch, workgroups, l.own_splits, stream) : launch_tiles_for<128>(p, stretch, workgroups, l.own_splits, stream);
+        const int e = l.wp == 64 ? launch_tiles_for<64>(p, stretch, l.own_waves, workgroups, l.own_splits, stream) : launch_tiles_for<128>(p, stretch, l.own_waves, workgroups, l.own_splits, stream);
         if (e != 0) return e;
     } else {
         p.part_values = values;

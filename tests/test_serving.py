@@ -275,6 +275,7 @@ CACHED_CASES = {
     "prefix_inside_window": dict(dtype=DType.F16, kv=1, group=8, width=96, page=16, lengths=[30, 400, 5], prefix=200, window=100, queries=2, slopes=True),
     "prefix_inside_lost": dict(dtype=DType.F16, kv=1, group=4, width=128, page=7, lengths=[20, 3, 0], queries=3, prefix=50, lost=[(-1, 0), (-1, 6), (0, 1)], poison=True),
     "many_prompts_over_the_cache": dict(dtype=DType.F16, kv=2, group=1, width=128, page=16, lengths=[40 + (9 * i) % 100 for i in range(200)], queries=40, poison=True),
+    "many_long_prompts_over_the_cache": dict(dtype=DType.F16, kv=2, group=8, width=128, page=16, lengths=[120 + i for i in range(70)], queries=130, prefix=70),
     "many_prompts_over_the_cache_i8": dict(dtype=DType.I8, kv=2, group=1, width=64, page=16, lengths=[(9 * i) % 120 for i in range(200)], queries=40, prefix=100, cap=9.0),
     "many_heads_of_one": dict(dtype=DType.I8, kv=1, group=71, width=64, page=16, lengths=[300, 4]),
 }
@@ -343,6 +344,8 @@ PROMPT_CASES = {
     "unseen_is_nan": dict(batch=2, queries=260, heads=2, kv=2, width=64, causal=True, lengths=[100, 259], poison=True),
     "future_is_nan": dict(queries=200, keys=200, heads=2, kv=2, width=64, causal=True, poison_from=150),
     "many_prompts": dict(batch=210, queries=70, heads=2, kv=2, width=128, causal=True, lengths=[(7 * i) % 71 for i in range(210)], poison=True),
+    "many_long_prompts": dict(batch=70, queries=130, heads=16, kv=2, width=128, causal=True, lengths=[(7 * i) % 131 for i in range(70)], poison=True),
+    "many_long_prompts_capped": dict(batch=70, queries=130, keys=150, heads=16, kv=2, width=104, causal=True, cap=8.0, slopes=True, window=90, size=2.0),
     "many_prompts_everything": dict(batch=200, queries=40, keys=150, heads=4, kv=2, width=64, causal=True, cap=8.0, slopes=True, window=90,
                                     prefix=[i % 60 for i in range(200)], size=2.0),
     "past_is_nan": dict(queries=200, heads=1, kv=1, width=128, causal=True, window=30, poison_to=71),
