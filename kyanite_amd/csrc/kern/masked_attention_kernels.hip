@@ -151,6 +151,20 @@ __device__ __forceinline__ halfx8 widen(unsigned a, unsigned b) {
                                             pk_sub_1152((b & 0x00ff00ffu) | 0x64006400u), pk_sub_1152(((b >> 8) & 0x00ff00ffu) | 0x64006400u)});
 }
 
+// What the scale of an 8 bit value adds to its score (in units of log2), so that the weight is the softmax's times the scale, and what
+// such a weight is multiplied by in the softmax's own sum. A key that a query does not see has the score -infinity, and with it
+// the weight zero whatever its scale holds: not finite (or absurdly large) scales are NaN to the score and zero to the sum. Scales
+// below 2^-40 count as that: values below 2^-33 are zeros of an f16 result.
+struct ValueScale {
+    float log, inv;
+    __device__ __forceinline__ explicit ValueScale(float scale) {
+        const float held = scale < 0x1p-40f ? 0x1p-40f : scale;
+        const bool good = held <= 0x1p100f;
+        log = good ? __builtin_amdgcn_logf(held) : __builtin_nanf("");
+        inv = good ? __builtin_amdgcn_rcpf(held) : 0.0f;
+    }
+};
+
 // ---- 32 rows per wave, 4 or 8 waves per workgroup ------------------------------------------------------------------
 
 // The waves walk all blocks of 64 keys, which they stage together in one of two LDS buffers, one barrier per block: the
@@ -645,8 +659,8 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 //                    lanes; the order of a row's elements in the product is free, Q is loaded in the same one
 //   O^T += V^T P^T   the accumulators of two tiles of S^T are the operand, keys 4 g + e and 16 + 4 g + e; lane (i, g) reads
 //                    elements i DPL .. + DPL - 1 of those 8 keys and turns them in registers: product dt has dim i DPL + dt
-// The scale of a key is applied to its score, that of a value to its weight, in f32; the reference
-// of the softmax follows score + log2(value scale), which keeps the scaled weights inside the range of f16.
+// The scale of a key is applied to its score, that of a value to its weight, in f32 and ahead of the exponential (ValueScale); the
+// reference of the softmax follows score + log2(value scale), which keeps the scaled weights inside the range of f16.
 
 // Which keys a workgroup takes, decided on the device, where the lengths are: stretches (the prefix when it is done here, then
 // every sequence's own keys) are cut into items of about the same size, ROW_ITEMS of them over all heads, and workgroup x
@@ -968,12 +982,13 @@ __global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))
                 }
             }
             if (more) load_k(next);
-            float value_log[8];
+            float value_log[8], value_inv[8];
             if (I8)
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    vscale[e / 4][e % 4] = fmaxf(vscale[e / 4][e % 4], 0x1p-40f);  // (values below 2^-33 are zeros of an f16 result)
-                    value_log[e] = __builtin_amdgcn_logf(vscale[e / 4][e % 4]);
+                    const ValueScale v(vscale[e / 4][e % 4]);
+                    value_log[e] = v.log;
+                    value_inv[e] = v.inv;
                 }
             halfx8 weights[NT];
 #pragma unroll
@@ -990,9 +1005,10 @@ __global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))
                     } else {
                         x *= scale2;
                     }
+                    if (I8) x += value_log[e];
                     if (masked && ((unsigned) (key - lo[n]) >= (unsigned) (hi[n] - lo[n]) || key >= end || ((gone >> e) & 1))) x = -INFINITY;
                     s2[e] = x;
-                    top = fmaxf(top, I8 ? x + value_log[e] : x);
+                    top = fmaxf(top, x);
                 }
                 if (__any(top > ref[n] + SLACK)) {
                     top = fmaxf(top, __shfl_xor(top, 16));
@@ -1008,8 +1024,8 @@ __global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const float x = __builtin_amdgcn_exp2f(s2[e] - minus);
-                    sum[n] += x;
-                    weights[n][e] = (half_t) (I8 ? x * vscale[e / 4][e % 4] : x);
+                    sum[n] = I8 ? __builtin_fmaf(x, value_inv[e], sum[n]) : sum[n] + x;
+                    weights[n][e] = (half_t) x;
                 }
             }
             if (more && PAGE16) load_scales(next);

@@ -1,0 +1,174 @@
+"""The serving operators where magnitudes are extreme. Bounds are those of the operators' own rounding steps, key by key."""
+import numpy as np
+import pytest
+
+import kyanite_amd as kn
+from kyanite_amd import DType
+from serving_oracle import upload
+
+PAGE = 16
+
+
+def attend(q, k, v, at, places, visible, scale, cap, slope, value_scales=None):
+    """One head in 64 bits: q [rows, width], k, v [keys, width], visible [rows, keys]. (result, bound on its error).
+
+    A score is a sum of `width` products and the few operations behind it, in f32: off by (width + 16) 2^-24 of the sum of
+    its products' sizes. The cap does not enlarge that, and its own formula is off by 16 x 2^-24 of its result (a quotient
+    of 1 - 2 / (1 + e) is known to 2^-22, its result is at least a third of the cap). Factors and the bias in units of log2, the
+    difference to the reference, the power of two and, for 8 bit values, the logarithm of their scale (below 2^5 in size) add
+    roundings of 2^-24 each of what they round: 8 x 2^-24 of score and bias, 64 x 2^-24 of one. An error d of a score moves
+    its term of the result by d times its share. Weights are rounded to f16: half a step of 2^-11, and half of 2^-24 where
+    they are below the normal numbers while the largest of a row is at least 2^7 (8 bit: the largest product of weight and scale,
+    for values of up to 127). Chains of sums over the keys: 2^-24 per matrix instruction. The result is rounded to f16."""
+    rows, keys = visible.shape
+    if keys == 0:
+        return np.zeros((rows, v.shape[1])), np.full((rows, v.shape[1]), 2.0 ** -24)
+    with np.errstate(invalid="ignore"):
+        s = (q @ k.T) * scale
+        off = (np.abs(q) @ np.abs(k).T) * abs(scale) * (q.shape[1] + 16) * 2.0 ** -24
+    z = cap * np.tanh(s / cap) if cap else s
+    bias = slope * np.abs(at[:, None] - places[None, :])
+    off = off + (24 * np.abs(z) + 8 * np.abs(bias) + 64) * 2.0 ** -24
+    z = np.where(visible, z - bias, -np.inf)
+    top = z.max(-1, keepdims=True)
+    e = np.exp(z - np.where(np.isfinite(top), top, 0.0))
+    total = e.sum(-1, keepdims=True)
+    safe = np.where(total > 0, total, 1.0)
+    w, off = e / safe, np.where(visible, off, 0.0)
+    v = np.where(visible.any(0)[:, None], v, 0.0)  # what nobody sees
+    out = w @ v
+    moved = ((w * off) @ np.abs(v) + np.abs(out) * (w * off).sum(-1, keepdims=True)) * 1.1
+    if value_scales is None:
+        below = 2.0 ** -32 * (visible.astype(float) @ np.abs(v)) / safe
+    else:
+        held = np.where(visible.any(0), value_scales, 0.0)  # (scales below 2^-40 count as that)
+        below = 2.0 ** -32 * 127 * visible.sum(-1, keepdims=True) * (e * np.maximum(held, 2.0 ** -40)).max(-1, keepdims=True) / safe + 2.0 ** -33
+    chain = (keys / 16 + 16) * 2.0 ** -24
+    return out, (w @ np.abs(v)) * (2.0 ** -11 + chain) + below + moved + np.abs(out) * 2.0 ** -11 + 2.0 ** -24
+
+
+class Case:
+    """Sequences over a cache whose pages lie one behind the other: the prefix's first, then `table_pages` per sequence. Keys and
+    values are given per place, [place, heads, width] in f64; 8 bit rows are quantised here."""
+
+    def __init__(self, dtype, lengths, kv=1, group=2, width=64, queries=1, prefix=0, page=PAGE, seed=0, **scores):
+        self.rng = np.random.default_rng(seed)
+        self.dtype, self.lengths, self.kv, self.group, self.width, self.queries, self.prefix, self.page = dtype, lengths, kv, group, width, queries, prefix, page
+        self.scores = dict(dict(scale=width ** -0.5, cap=0.0, window=0, slopes=None), **scores)
+        self.table_pages, self.prefix_pages = max(1, -(-max(lengths) // page)), -(-prefix // page)
+        self.pages = self.prefix_pages + len(lengths) * self.table_pages
+        shape = (self.pages * page, kv, width)
+        self.q = self.rng.standard_normal((len(lengths), queries, kv * group, width)).astype(np.float16)
+        self.k, self.v = self.rng.standard_normal(shape), self.rng.standard_normal(shape)
+        self.spoilt = []  # (place, whose scale, value)
+
+    def place(self, b, j):
+        """where key j of sequence b lies (j < prefix: in the prefix)"""
+        return j if j < self.prefix else (self.prefix_pages + b * self.table_pages) * self.page + j - self.prefix
+
+    def held(self):
+        """what the cache holds: (k, v, scales of k, scales of v), [place, heads, ...]"""
+        if self.dtype == DType.F16:
+            return self.k.astype(np.float16), self.v.astype(np.float16), None, None
+        out = []
+        for x in (self.k, self.v):
+            scale = (np.abs(x).max(-1) / 127).astype(np.float32)
+            out.append((np.rint(x / np.where(scale > 0, scale, 1)[..., None]).clip(-127, 127).astype(np.int8), scale))
+        return out[0][0], out[1][0], out[0][1], out[1][1]
+
+    def run(self, device):
+        held = list(self.held())
+        for place, which, value in self.spoilt:
+            held[2 + which][place] = value
+        paged = [None if x is None else np.ascontiguousarray(np.moveaxis(x.reshape((self.pages, self.page) + x.shape[1:]), 1, 2)) for x in held]
+        tables = (self.prefix_pages + np.arange(len(self.lengths) * self.table_pages)).astype(np.int32)
+        mem = [upload(device, x if x is not None else np.zeros(1, np.float32)) for x in paged]
+        B, T, H, W = self.q.shape
+        dev = [upload(device, x) for x in (self.q, np.array(self.lengths, np.int32), tables, np.arange(max(self.prefix_pages, 1), dtype=np.int32),
+                                           np.asarray(self.scores["slopes"] if self.scores["slopes"] is not None else [0], np.float32))]
+        out = kn.DeviceBuffer(device, self.q.nbytes)
+        scales = (mem[2].ptr, mem[3].ptr) if self.dtype == DType.I8 else (0, 0)
+        cache = kn.kv_cache(self.dtype, self.pages, self.kv, self.page, W, mem[0].ptr, mem[1].ptr, *scales)
+        strides = (T * H * W, H * W, W)
+        args = kn.cached_attention_args(B, T, H, cache, dev[0].ptr, strides, out.ptr, strides, dev[1].ptr, dev[2].ptr, self.table_pages, self.table_pages,
+                                        prefix_tokens=self.prefix, prefix_table=dev[3].ptr if self.prefix else 0, scale=self.scores["scale"],
+                                        cap=self.scores["cap"], window=self.scores["window"], slopes=dev[4].ptr if self.scores["slopes"] is not None else 0)
+        stream = kn.HipStream(device)
+        kn.cached_attention(device, stream, args, kn.DeviceBuffer(device, max(kn.cached_attention_workspace_bytes(args), 1)))
+        stream.synchronize()
+        return out.to_array(np.float16, self.q.shape)
+
+    def check(self, got, what=""):
+        k, v, ks, vs = (None if x is None else x.astype(np.float64) for x in self.held())
+        if self.dtype == DType.I8:
+            k, v = k * ks[..., None], v * vs[..., None]
+        T = self.queries
+        for b, n in enumerate(self.lengths):
+            places = np.arange(self.prefix + n)
+            at = self.prefix + n - T + np.arange(T)
+            where = np.array([self.place(b, j) for j in places], np.int64)
+            visible = (places <= at[:, None]) & (at[:, None] >= self.prefix)
+            if self.scores["window"]:
+                visible &= places > at[:, None] - self.scores["window"]
+            for h in range(self.kv * self.group):
+                g = h // self.group
+                slope = 0.0 if self.scores["slopes"] is None else float(self.scores["slopes"][h])
+                out, bound = attend(self.q[b, :, h].astype(np.float64), k[where, g], v[where, g], at, places, visible, float(np.float32(self.scores["scale"])),
+                                    float(np.float32(self.scores["cap"])), slope, None if vs is None else vs[where, g])
+                off = np.abs(got[b, :, h].astype(np.float64) - out)
+                assert (off <= bound).all(), f"{what}: sequence {b} head {h}: {np.max(off / bound):.2f} of the bound, {np.max(off):.3e} off"
+
+
+# (which kernel: few rows, a prefix beside few rows in one launch or in its own, many rows, a prefix for many rows)
+FORMS = {
+    "rows": dict(lengths=[50, 33, 100, 7]),
+    "rows_odd_pages": dict(lengths=[50, 33, 100, 7], page=5),
+    "rows_wide": dict(lengths=[50, 333], width=128, group=4, queries=3),
+    "rows_in_parts": dict(lengths=[2500, 40], width=128),
+    "prefix_inside": dict(lengths=[50, 3], prefix=100, queries=2),
+    "prefix_in_rows": dict(lengths=[50, 3], prefix=1000, width=128),
+    "prefix_of_many": dict(lengths=[50 + i % 7 for i in range(24)], prefix=2100, group=4),
+    "prefix_of_many_wide": dict(lengths=[50 + i % 7 for i in range(24)], prefix=2100, group=4, width=128),
+    "tiles": dict(lengths=[200, 90], queries=40),
+    "tiles_wide": dict(lengths=[300, 90], queries=40, width=128, group=3),
+}
+
+ROW_FORMS = ("rows", "rows_odd_pages", "rows_wide", "rows_in_parts", "prefix_inside", "prefix_in_rows")
+
+
+# ---- scales that nobody sees ---------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf, 3e38, 1e12], ids=str)
+@pytest.mark.parametrize("form", [f for f in FORMS if f in ROW_FORMS])
+def test_scales_of_unseen_slots_change_nothing(form, value, hip_device):
+    """slots behind a sequence's last key, and keys in front of every query's window"""
+    c = dict(FORMS[form])
+    window = c["prefix"] // 2 + max(c["lengths"]) if "prefix" in c else 30 + c.get("queries", 1)
+    case = Case(DType.I8, window=window, **c)
+    clean = case.run(hip_device)
+    case.check(clean, "clean")
+    for b, n in enumerate(case.lengths):
+        first = case.prefix + n - case.queries - window + 1  # the first key that any query sees
+        end = case.place(b, case.prefix) + case.table_pages * case.page
+        unseen = list(range(case.place(b, case.prefix + n - 1) + 1, end)) + [case.place(b, j) for j in range(case.prefix, max(first, case.prefix))]
+        case.spoilt += [(p, which, value) for p in unseen for which in (0, 1)]
+    seen_prefix = min(max(0, case.prefix + n - case.queries - window + 1) for n in case.lengths)
+    case.spoilt += [(p, which, value) for p in range(min(seen_prefix, case.prefix)) for which in (0, 1)]
+    case.spoilt += [(p, which, value) for p in range(case.prefix, case.prefix_pages * case.page) for which in (0, 1)]
+    assert case.spoilt
+    assert np.array_equal(case.run(hip_device).view(np.uint16), clean.view(np.uint16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [np.nan, np.inf, 3e38], ids=str)
+@pytest.mark.parametrize("form", ["rows_wide"])
+def test_scales_that_one_query_sees_leave_the_others_alone(form, value, hip_device):
+    """the newest key's scales: the last query sees them, the queries before do not"""
+    case = Case(DType.I8, **FORMS[form])
+    clean = case.run(hip_device)
+    case.spoilt = [(case.place(b, n - 1), which, value) for b, n in enumerate(case.lengths) for which in (0, 1)]
+    got = case.run(hip_device)
+    assert np.array_equal(got[:, :-1].view(np.uint16), clean[:, :-1].view(np.uint16))
+    if value != 3e38:
+        assert np.isnan(got[:, -1]).all()
