@@ -171,8 +171,9 @@ struct ValueScale {
 // block after the current one is in flight in registers meanwhile. KG = 2: twice the waves for the same rows, in two groups that take
 // every other block each and are joined at the end through LDS. WP: the width, padded to 64 or 128 with zeros. SHAPED: with
 // cap or distance bias. I8: keys and values are staged as the whole numbers they are, exact in f16; the scale of a key is
-// applied to its scores, that of a value to its weights, both in f32. The scaled weights keep inside f16 by a power of two
-// that the waves of a workgroup share: it starts from the first block and grows when a scale passes it by 2^6.
+// applied to its scores, that of a value to its weights, both in f32 and ahead of the exponential (ValueScale). The reference of a
+// query's softmax follows score + log2(value scale), so that what the second product holds in f16 goes by what a key contributes:
+// a large value of little weight takes no bits from the others.
 template <int WP, int STRETCH, bool I8, bool SHAPED, int TW, int KG>
 __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_attention_kernel(ServingAttentionParams p) {
     constexpr int BKEYS = 64, RW = TW / KG, THREADS = 64 * RW;  // waves for the rows, threads that stage a block
@@ -188,11 +189,10 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     constexpr int LDS_HALVES = std::max({2 * KG * STAGE, TW * WAVE_ROWS, JOIN + RW * WAVE_ROWS});
     static_assert(WP != 128 || VECS >= 1, "unsupported shape");
     __shared__ __attribute__((aligned(16))) half_t lds[LDS_HALVES];
-    __shared__ __attribute__((aligned(16))) float kscale_s[2][BKEYS], vscale_s[2][BKEYS];
+    __shared__ __attribute__((aligned(16))) float kscale_s[2][BKEYS], vlog_s[2][BKEYS], vinv_s[2][BKEYS];
     __shared__ unsigned long long gone_s[2][TW], bad_s[2][TW];
-    __shared__ int big_s[2][TW];
     __shared__ int range_s[TW][4];
-    static_assert(!I8 || KG == 1, "groups of waves share the power of two");
+    static_assert(!I8 || KG == 1, "one group of waves stages the scales");
 
     const int lane = threadIdx.x & 63, all_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wave = all_wave % RW, group = all_wave / RW;  // rows of the tile, blocks of keys
@@ -324,10 +324,8 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     // leave f32 nothing does
     const CapSeries series(cap2, I8 ? 1.0f : to_cap);
     const float near_cap = I8 ? 0.35f : uniform(to_cap < 4096.0f ? 0.35f / to_cap : -1.0f);
-    float value_unit = 0x1p60f;  // I8: what the scales of values are multiplied by, a power of two
     auto stage = [&](int buffer, bool masked) {
         half_t *ks = lds + (KG * buffer + group) * STAGE, *vs = ks + BKEYS * KS;
-        bool big = false;
 #pragma unroll
         for (int i = 0; i < VECS; i++) {
             const int r = stage_row + ROW_STEP * i;
@@ -338,8 +336,9 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
                 *(halfx8 *) &vs[r * VS + 16 * part + 8] = widen(vreg[i].z, vreg[i].w);
                 if (part == 0) {
                     kscale_s[buffer][r] = kscale[i] * (capped ? to_cap : scale2);
-                    vscale_s[buffer][r] = vscale[i] * value_unit;
-                    big |= vscale[i] * value_unit > 64.0f;
+                    const ValueScale v(vscale[i]);
+                    vlog_s[buffer][r] = v.log;
+                    vinv_s[buffer][r] = v.inv;
                 }
             } else {
                 *(uint4 *) &ks[r * KS + 8 * part] = kreg[i];
@@ -363,11 +362,9 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
                         if (missing & lanes) gone_rows |= 1ull << r;
                     }
             }
-            const int any_big = I8 ? __any(big) : 0;
             if (lane == 0) {
                 gone_s[buffer][all_wave] = gone_rows;
                 bad_s[buffer][all_wave] = bad_rows;
-                if (I8) big_s[buffer][all_wave] = any_big;
             }
         }
     };
@@ -427,32 +424,16 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         unsigned long long gone_rows = 0;
         if (KG > 1 || PAGED || masked) {
             unsigned long long bad_rows = 0, bad_anywhere = 0;
-            int big = 0;
 #pragma unroll
             for (int i = 0; i < RW; i++) {
                 gone_rows |= gone_s[buffer][group * RW + i];
                 if (!I8) bad_rows |= bad_s[buffer][group * RW + i];
-                if (I8) big |= big_s[buffer][i];
             }
             if (!I8)
 #pragma unroll
                 for (int i = 0; i < TW; i++) bad_anywhere |= bad_s[buffer][i];
             gone_rows = ((unsigned long long) __builtin_amdgcn_readfirstlane((unsigned) (gone_rows >> 32)) << 32) | (unsigned) __builtin_amdgcn_readfirstlane((unsigned) gone_rows);
             if (PAGED) masked |= gone_rows != 0;
-            if (I8 && __builtin_amdgcn_readfirstlane(big)) {  // (the same for all waves, which take the barriers together)
-                float most = vscale_s[buffer][lane];
-#pragma unroll
-                for (int m = 1; m < 64; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
-                const float unit = __builtin_ldexpf(1.0f, -__builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(most)));
-                value_unit *= unit;
-#pragma unroll
-                for (int t = 0; t < DT; t++)
-#pragma unroll
-                    for (int v = 0; v < 16; v++) oacc[t][v] *= unit;
-                __syncthreads();
-                if (threadIdx.x < BKEYS) vscale_s[buffer][threadIdx.x] *= unit;
-                __syncthreads();
-            }
             bad_rows = ((unsigned long long) __builtin_amdgcn_readfirstlane((unsigned) (bad_rows >> 32)) << 32) | (unsigned) __builtin_amdgcn_readfirstlane((unsigned) bad_rows);
             if (!I8 && (__builtin_amdgcn_readfirstlane((unsigned) (bad_anywhere >> 32)) | __builtin_amdgcn_readfirstlane((unsigned) bad_anywhere)) != 0) {
                 // Infinities or NaN among the values of a block that not every row sees whole: a weight of zero does not remove
@@ -500,8 +481,10 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
                 for (int a = 0; a < 4; a++) {
                     const floatx4 f = *(const floatx4 *) &kscale_s[buffer][32 * u + 8 * a + 4 * h];
+                    floatx4 l = {0, 0, 0, 0};
+                    if (!SHAPED) l = *(const floatx4 *) &vlog_s[buffer][32 * u + 8 * a + 4 * h];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) st[u][4 * a + e] *= f[e];
+                    for (int e = 0; e < 4; e++) st[u][4 * a + e] = SHAPED ? st[u][4 * a + e] * f[e] : __builtin_fmaf(st[u][4 * a + e], f[e], l[e]);
                 }
             if (SHAPED && capped) {
                 // (the same choice for the whole wave; most scores lie far below the cap)
@@ -524,6 +507,13 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
                 for (int v = 0; v < 16; v++) st[u][v] = __builtin_fmaf(-slope2, fabsf(away - (float) (8 * (v / 4) + v % 4)), st[u][v]);
             }
+            if (SHAPED && I8)
+#pragma unroll
+                for (int a = 0; a < 4; a++) {
+                    const floatx4 l = *(const floatx4 *) &vlog_s[buffer][32 * u + 8 * a + 4 * h];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) st[u][4 * a + e] += l[e];
+                }
             if (masked) {
                 const unsigned missing = (unsigned) (gone_rows >> (32 * u)) >> (4 * h);
 #pragma unroll
@@ -554,13 +544,13 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
             for (int a = 0; a < 4; a++) {
                 floatx4 f = {1, 1, 1, 1};
-                if (I8) f = *(const floatx4 *) &vscale_s[buffer][32 * u + 8 * a + 4 * h];
+                if (I8) f = *(const floatx4 *) &vinv_s[buffer][32 * u + 8 * a + 4 * h];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int v = 4 * a + i;
                     const float e = __builtin_amdgcn_exp2f(LOG2_UNITS ? st[u][v] - minus : __builtin_fmaf(st[u][v], scale2, -minus));
-                    sum += e;
-                    pv[2 * u + v / 8][v % 8] = (half_t) (I8 ? e * f[i] : e);
+                    sum = I8 ? __builtin_fmaf(e, f[i], sum) : sum + e;
+                    pv[2 * u + v / 8][v % 8] = (half_t) e;
                 }
             }
 #pragma unroll
@@ -606,7 +596,6 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             }
     }
     sum += __shfl_xor(sum, 32);
-    const float back = I8 ? 1.0f / value_unit : 1.0f;
     // (dims 32 t + 8 a + 4 h + (0 .. 3) are registers 4 a .. 4 a + 3, the middle two changed over where widen() does)
     auto dims = [&](int t, int a) {
         return I8 ? floatx4{oacc[t][4 * a], oacc[t][4 * a + 2], oacc[t][4 * a + 1], oacc[t][4 * a + 3]}
@@ -620,13 +609,13 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
             for (int t = 0; t < DT; t++)
 #pragma unroll
-                for (int a = 0; a < 4; a++) *(floatx4 *) (o + 32 * t + 8 * a + 4 * h) = dims(t, a) * back;
+                for (int a = 0; a < 4; a++) *(floatx4 *) (o + 32 * t + 8 * a + 4 * h) = dims(t, a);
             if (h == 0) *(float2 *) (p.part_stats + 2 * at) = float2{ref, sum};
         }
         return;
     }
     // ---- the result: normalised, rounded, through the wave's rows of LDS into whole rows
-    const float inv = sum > 0.0f || sum != sum ? back / sum : 0.0f;
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
     if (KG == 1) __syncthreads();  // (every wave is done with the buffers)
     half_t *os = lds + JOIN + wave * WAVE_ROWS;
 #pragma unroll

@@ -133,14 +133,12 @@ FORMS = {
     "tiles_wide": dict(lengths=[300, 90], queries=40, width=128, group=3),
 }
 
-ROW_FORMS = ("rows", "rows_odd_pages", "rows_wide", "rows_in_parts", "prefix_inside", "prefix_in_rows")
-
 
 # ---- scales that nobody sees ---------------------------------------------------------------------------------------
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf, 3e38, 1e12], ids=str)
-@pytest.mark.parametrize("form", [f for f in FORMS if f in ROW_FORMS])
+@pytest.mark.parametrize("form", FORMS)
 def test_scales_of_unseen_slots_change_nothing(form, value, hip_device):
     """slots behind a sequence's last key, and keys in front of every query's window"""
     c = dict(FORMS[form])
@@ -162,7 +160,7 @@ def test_scales_of_unseen_slots_change_nothing(form, value, hip_device):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("value", [np.nan, np.inf, 3e38], ids=str)
-@pytest.mark.parametrize("form", ["rows_wide"])
+@pytest.mark.parametrize("form", ["rows_wide", "tiles", "tiles_wide"])
 def test_scales_that_one_query_sees_leave_the_others_alone(form, value, hip_device):
     """the newest key's scales: the last query sees them, the queries before do not"""
     case = Case(DType.I8, **FORMS[form])
@@ -172,3 +170,37 @@ def test_scales_that_one_query_sees_leave_the_others_alone(form, value, hip_devi
     assert np.array_equal(got[:, :-1].view(np.uint16), clean[:, :-1].view(np.uint16))
     if value != 3e38:
         assert np.isnan(got[:, -1]).all()
+
+
+# ---- values of different magnitudes --------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [DType.I8, DType.F16], ids=lambda d: d.name)
+@pytest.mark.parametrize("spread", ["from_1e-3_to_6e4", "later_outlier", "dominant_outlier", "rising", "zeros"])
+@pytest.mark.parametrize("form", FORMS)
+def test_values_of_different_magnitudes(form, spread, dtype, hip_device):
+    case = Case(dtype, seed=3, **FORMS[form])
+    rng, n = case.rng, len(case.v)
+    if spread == "from_1e-3_to_6e4":
+        case.v *= np.exp(rng.uniform(np.log(1e-3), np.log(1e4), n))[:, None, None]
+    else:
+        case.v *= 0.05
+    if spread == "rising":
+        case.v *= 4.0 ** (np.arange(n) // 64 % 9)[:, None, None]
+    for b in range(len(case.lengths)):
+        first, last = case.place(b, 0), case.place(b, case.prefix + case.lengths[b] - case.queries)
+        if spread == "zeros":
+            case.v[first] = 0
+            case.k[first] = case.q[b, 0, 0] * 2.0  # most of the weight, for one head
+        for place in (last - 3, (first + last) // 2 if case.prefix == 0 else case.prefix // 2 + 1):
+            if spread == "later_outlier":  # a score far below all others
+                case.v[place] = rng.standard_normal((case.kv, case.width)).clip(-2, 2) * 15000
+                case.k[place] = 0
+                case.q[..., 0] = 30
+                case.k[place, :, 0] = -8
+            if spread == "dominant_outlier":
+                case.v[place] = rng.standard_normal((case.kv, case.width)).clip(-2, 2) * 15000
+                case.k[place] = 0
+                case.q[..., 0] = 20
+                case.k[place, :, 0] = 4
+    case.check(case.run(hip_device), f"{form} {spread}")
