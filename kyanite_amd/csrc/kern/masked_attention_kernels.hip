@@ -97,23 +97,37 @@ __device__ __forceinline__ float tanh_fast(float x) {
 // a number that is the same in all lanes, into a scalar register
 __device__ __forceinline__ float uniform(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); }
 
-// c tanh(f s) for |f s| <= 0.35 as an odd series in s, up to the 9th power: the next term is 1382 / 155925 x^10 of the result,
-// below 2.5e-7. Half the time of the exponential and the reciprocal.
-struct CapSeries {
+// The capped score c tanh(f s) in units of log2, off by a few units of its last place, or by 2^-16 where caps are small. Three forms:
+//   series   |f s| <= 0.35 for a whole wave, the usual case: an odd series in s up to the 9th power; the next term is 1382 / 155925 x^10
+//            of the result, below 2.5e-7. Half the time of the exponential and the reciprocal.
+//   small    c <= SMALL: tanh_fast, whose 2^-22 of the cap are at most 2^-16, which moves a weight by a twentieth of its rounding to f16
+//   any      the series where |f s| <= 0.35, tanh_fast beyond, where its error is small against its result too
+// (8192 tokens whose scores lie around their cap: 1120 us if small caps went the last way, 830 so. All three in one tile kernel
+// cost it registers: a capped prefix of 16384 tokens 96 us instead of 86; so its larger caps are an instantiation of their own.)
+// `factor` is that of a score without a cap, c f: it is not formed from them, so that no cap near the end of f32 loses bits.
+struct Cap {
+    static constexpr float SMALL = 64.0f;
+    static __host__ __device__ __forceinline__ bool large(float cap) { return cap * LOG2E > SMALL; }
+    float c, f, near;  // near: up to which |s|; with caps so small that the coefficients would leave f32 nothing is
     float k[5];
-    __device__ __forceinline__ CapSeries(float c, float f) {
+    __device__ __forceinline__ Cap(float cap, float per_score, float factor) {
+        c = uniform(cap);
+        f = uniform(per_score);
+        near = uniform(fabsf(f) < 4096.0f ? 0.35f / fabsf(f) : -1.0f);
         const float g = f * f;
-        k[0] = uniform(c * f);
-        k[1] = uniform(k[0] * g * (-1.0f / 3));
-        k[2] = uniform(k[0] * g * g * (2.0f / 15));
-        k[3] = uniform(k[0] * g * g * g * (-17.0f / 315));
-        k[4] = uniform(k[0] * g * g * g * g * (62.0f / 2835));
+        k[0] = uniform(factor);
+        k[1] = uniform(factor * g * (-1.0f / 3));
+        k[2] = uniform(factor * g * g * (2.0f / 15));
+        k[3] = uniform(factor * g * g * g * (-17.0f / 315));
+        k[4] = uniform(factor * g * g * g * g * (62.0f / 2835));
     }
+    __device__ __forceinline__ float series(float s) const {
+        const float q = s * s;
+        return s * __builtin_fmaf(q, __builtin_fmaf(q, __builtin_fmaf(q, __builtin_fmaf(q, k[4], k[3]), k[2]), k[1]), k[0]);
+    }
+    __device__ __forceinline__ float small(float s) const { return c * tanh_fast(s * f); }
+    __device__ __forceinline__ float any(float s) const { return fabsf(s) <= near ? series(s) : small(s); }
 };
-__device__ __forceinline__ float cap_series(float s, const CapSeries &c) {
-    const float q = s * s;
-    return s * __builtin_fmaf(q, __builtin_fmaf(q, __builtin_fmaf(q, __builtin_fmaf(q, c.k[4], c.k[3]), c.k[2]), c.k[1]), c.k[0]);
-}
 
 // four keys (consecutive rows of the staged V) of one dim: 16 lanes hand in the addresses of 4 dims of 4 rows each
 __device__ __forceinline__ halfx4 lds_read_transposed(const half_t *p) {
@@ -169,12 +183,13 @@ struct ValueScale {
 
 // The waves walk all blocks of 64 keys, which they stage together in one of two LDS buffers, one barrier per block: the
 // block after the current one is in flight in registers meanwhile. KG = 2: twice the waves for the same rows, in two groups that take
-// every other block each and are joined at the end through LDS. WP: the width, padded to 64 or 128 with zeros. SHAPED: with
-// cap or distance bias. I8: keys and values are staged as the whole numbers they are, exact in f16; the scale of a key is
+// every other block each and are joined at the end through LDS. WP: the width, padded to 64 or 128 with zeros. SHAPE:
+// whether there is a cap or a distance bias. I8: keys and values are staged as the whole numbers they are, exact in f16; the scale of a key is
 // applied to its scores, that of a value to its weights, both in f32 and ahead of the exponential (ValueScale). The reference of a
 // query's softmax follows score + log2(value scale), so that what the second product holds in f16 goes by what a key contributes:
 // a large value of little weight takes no bits from the others.
-template <int WP, int STRETCH, bool I8, bool SHAPED, int TW, int KG>
+enum Shape { PLAIN, SHAPED_SCORES, LARGE_CAP };
+template <int WP, int STRETCH, bool I8, int SHAPE, int TW, int KG>
 __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_attention_kernel(ServingAttentionParams p) {
     constexpr int BKEYS = 64, RW = TW / KG, THREADS = 64 * RW;  // waves for the rows, threads that stage a block
     constexpr int PIECE = I8 ? 16 : 8;        // elements per 128 bit load
@@ -184,7 +199,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     constexpr int STAGE = BKEYS * (KS + VS);
     constexpr int OS = WP + 8, WAVE_ROWS = 32 * OS;
     constexpr int DT = WP / 32, QC = WP / 8;
-    constexpr bool PAGED = STRETCH != PROMPT;
+    constexpr bool PAGED = STRETCH != PROMPT, SHAPED = SHAPE != PLAIN;
     constexpr int JOIN = KG > 1 ? RW * 64 * (DT * 16 + 2) * 2 : 0;  // the other group's accumulators, in halves
     constexpr int LDS_HALVES = std::max({2 * KG * STAGE, TW * WAVE_ROWS, JOIN + RW * WAVE_ROWS});
     static_assert(WP != 128 || VECS >= 1, "unsupported shape");
@@ -319,11 +334,9 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const float sign = uniform(p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f);
     const float scale2 = uniform(p.scale == 0.0f ? 1.0f : fabsf(p.scale) * LOG2E);
     const bool capped = SHAPED && p.cap > 0.0f;
-    const float to_cap = uniform(capped ? scale2 / (LOG2E * p.cap) : 0.0f), cap2 = uniform(p.cap * LOG2E);
-    // the series takes scores (I8: scores over the cap) up to 0.35 of the cap; with caps so small that its coefficients would
-    // leave f32 nothing does
-    const CapSeries series(cap2, I8 ? 1.0f : to_cap);
-    const float near_cap = I8 ? 0.35f : uniform(to_cap < 4096.0f ? 0.35f / to_cap : -1.0f);
+    // (the scores of whole numbers have their factor already)
+    const float cap2 = uniform(capped ? p.cap * LOG2E : 1.0f);
+    const Cap cap(cap2, (I8 ? 1.0f : scale2) / cap2, I8 ? 1.0f : scale2);
     auto stage = [&](int buffer, bool masked) {
         half_t *ks = lds + (KG * buffer + group) * STAGE, *vs = ks + BKEYS * KS;
 #pragma unroll
@@ -335,7 +348,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
                 *(halfx8 *) &vs[r * VS + 16 * part] = widen(vreg[i].x, vreg[i].y);
                 *(halfx8 *) &vs[r * VS + 16 * part + 8] = widen(vreg[i].z, vreg[i].w);
                 if (part == 0) {
-                    kscale_s[buffer][r] = kscale[i] * (capped ? to_cap : scale2);
+                    kscale_s[buffer][r] = kscale[i] * scale2;
                     const ValueScale v(vscale[i]);
                     vlog_s[buffer][r] = v.log;
                     vinv_s[buffer][r] = v.inv;
@@ -491,12 +504,12 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
                 float far = fabsf(st[u][0]);
 #pragma unroll
                 for (int v = 1; v < 16; v++) far = fmaxf(far, fabsf(st[u][v]));
-                if (__all(far <= near_cap)) {
+                if (__all(far <= cap.near)) {
 #pragma unroll
-                    for (int v = 0; v < 16; v++) st[u][v] = cap_series(st[u][v], series);
+                    for (int v = 0; v < 16; v++) st[u][v] = cap.series(st[u][v]);
                 } else {
 #pragma unroll
-                    for (int v = 0; v < 16; v++) st[u][v] = cap2 * tanh_fast(I8 ? st[u][v] : st[u][v] * to_cap);
+                    for (int v = 0; v < 16; v++) st[u][v] = SHAPE == LARGE_CAP ? cap.any(st[u][v]) : cap.small(st[u][v]);
                 }
             } else if (SHAPED && !I8) {
 #pragma unroll
@@ -787,7 +800,8 @@ __global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))
     }
     const float scale2 = p.scale * LOG2E;
     const bool capped = SHAPED && p.cap > 0.0f;
-    const float to_cap = capped ? p.scale / p.cap : 0.0f, cap2 = p.cap * LOG2E;
+    const float cap2 = capped ? p.cap * LOG2E : 1.0f;
+    const Cap cap(cap2, scale2 / cap2, scale2);
     const char *kb = (const char *) p.k + kv_head * p.k_head * ELEM, *vb = (const char *) p.v + kv_head * p.v_head * ELEM;
     const bool v_live = i * DPL < p.width, k_whole = p.width == WP;
 
@@ -984,16 +998,28 @@ __global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))
             for (int n = 0; n < NT; n++) {
                 float top = -INFINITY, s2[8];
 #pragma unroll
+                for (int e = 0; e < 8; e++) s2[e] = st[n][e / 4][e % 4] * (I8 ? kscale[e / 4][e % 4] : 1.0f);
+                if (SHAPED && capped) {
+                    float far = fabsf(s2[0]);
+#pragma unroll
+                    for (int e = 1; e < 8; e++) far = fmaxf(far, fabsf(s2[e]));
+                    if (__all(far <= cap.near)) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) s2[e] = cap.series(s2[e]);
+                    } else if (!Cap::large(p.cap)) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) s2[e] = cap.small(s2[e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) s2[e] = cap.any(s2[e]);
+                    }
+                }
+#pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int key = key0 + 16 * (e / 4) + 4 * g + e % 4;
-                    float x = st[n][e / 4][e % 4];
-                    if (I8) x *= kscale[e / 4][e % 4];
-                    if (SHAPED) {
-                        x = capped ? cap2 * tanh_fast(x * to_cap) : x * scale2;
-                        x = __builtin_fmaf(-slope2[n], fabsf((float) (at[n] - key)), x);
-                    } else {
-                        x *= scale2;
-                    }
+                    float x = s2[e];
+                    if (!(SHAPED && capped)) x *= scale2;
+                    if (SHAPED) x = __builtin_fmaf(-slope2[n], fabsf((float) (at[n] - key)), x);
                     if (I8) x += value_log[e];
                     if (masked && ((unsigned) (key - lo[n]) >= (unsigned) (hi[n] - lo[n]) || key >= end || ((gone >> e) & 1))) x = -INFINITY;
                     s2[e] = x;
@@ -1303,8 +1329,9 @@ template <int WP, int STRETCH, bool I8, int RW, int KG>
 int launch_tiles(const ServingAttentionParams &p, unsigned workgroups, int splits, hipStream_t stream) {
     constexpr int TW = RW * KG;
     const dim3 grid(workgroups, (unsigned) splits), block(64 * TW);
-    if (p.cap > 0.0f || p.slopes) hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, true, TW, KG>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, false, TW, KG>), grid, block, 0, stream, p);
+    if (Cap::large(p.cap)) hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, LARGE_CAP, TW, KG>), grid, block, 0, stream, p);
+    else if (p.cap > 0.0f || p.slopes) hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, SHAPED_SCORES, TW, KG>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((tile_attention_kernel<WP, STRETCH, I8, PLAIN, TW, KG>), grid, block, 0, stream, p);
     return (int) hipGetLastError();
 }
 

@@ -13,8 +13,8 @@ def attend(q, k, v, at, places, visible, scale, cap, slope, value_scales=None):
     """One head in 64 bits: q [rows, width], k, v [keys, width], visible [rows, keys]. (result, bound on its error).
 
     A score is a sum of `width` products and the few operations behind it, in f32: off by (width + 16) 2^-24 of the sum of
-    its products' sizes. The cap does not enlarge that, and its own formula is off by 16 x 2^-24 of its result (a quotient
-    of 1 - 2 / (1 + e) is known to 2^-22, its result is at least a third of the cap). Factors and the bias in units of log2, the
+    its products' sizes. The cap does not enlarge that; its own formula is off by 16 x 2^-24 of its result (a quotient
+    of 1 - 2 / (1 + e) is known to 2^-22, its result is at least a third of the cap), or by 2^-22 of a cap of up to 45. Factors and the bias in units of log2, the
     difference to the reference, the power of two and, for 8 bit values, the logarithm of their scale (below 2^5 in size) add
     roundings of 2^-24 each of what they round: 8 x 2^-24 of score and bias, 64 x 2^-24 of one. An error d of a score moves
     its term of the result by d times its share. Weights are rounded to f16: half a step of 2^-11, and half of 2^-24 where
@@ -28,7 +28,7 @@ def attend(q, k, v, at, places, visible, scale, cap, slope, value_scales=None):
         off = (np.abs(q) @ np.abs(k).T) * abs(scale) * (q.shape[1] + 16) * 2.0 ** -24
     z = cap * np.tanh(s / cap) if cap else s
     bias = slope * np.abs(at[:, None] - places[None, :])
-    off = off + (24 * np.abs(z) + 8 * np.abs(bias) + 64) * 2.0 ** -24
+    off = off + (24 * np.abs(z) + 8 * np.abs(bias) + 64) * 2.0 ** -24 + (cap * 2.0 ** -22 if cap <= 45 else 0.0)
     z = np.where(visible, z - bias, -np.inf)
     top = z.max(-1, keepdims=True)
     e = np.exp(z - np.where(np.isfinite(top), top, 0.0))
@@ -204,3 +204,49 @@ def test_values_of_different_magnitudes(form, spread, dtype, hip_device):
                 case.q[..., 0] = 20
                 case.k[place, :, 0] = 4
     case.check(case.run(hip_device), f"{form} {spread}")
+
+
+# ---- caps ----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [0.5, 30.0, 1e4, 1e6, 1e30, 1e38])
+@pytest.mark.parametrize("dtype", [DType.I8, DType.F16], ids=lambda d: d.name)
+@pytest.mark.parametrize("form", FORMS)
+def test_caps_of_any_size(form, dtype, cap, hip_device):
+    """the cap's error goes by the score, not by the cap"""
+    case = Case(dtype, cap=cap, seed=1, **FORMS[form])
+    case.check(case.run(hip_device), form)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [DType.I8, DType.F16], ids=lambda d: d.name)
+@pytest.mark.parametrize("form", FORMS)
+def test_scores_on_both_sides_of_a_cap(form, dtype, hip_device):
+    """one key of a few has a score beyond a large cap (negative: without weight), the others lie far below it"""
+    case = Case(dtype, cap=2e5, seed=2, **FORMS[form])
+    case.q[..., 0] = 300
+    case.k[..., 0] = 0
+    case.k[::5, :, 0] = -60000
+    case.check(case.run(hip_device), form)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [30.0, 1e6, 1e30, 2e5])
+@pytest.mark.parametrize("queries,keys,width", [(40, 40, 64), (150, 150, 128), (70, 1500, 64)])
+def test_caps_of_prompts(queries, keys, width, cap, hip_device):
+    rng = np.random.default_rng(queries)
+    q, k, v = (rng.standard_normal((n, 2, width)).astype(np.float16) for n in (queries, keys, keys))
+    if cap == 2e5:
+        q[..., 0], k[..., 0], k[::5, :, 0] = 300, 0, -60000
+    dev = [upload(hip_device, x) for x in (q, k, v)]
+    out = kn.DeviceBuffer(hip_device, q.nbytes)
+    s = (0, 2 * width, width)
+    args = kn.attention_args(1, queries, keys, 2, 2, width, dev[0].ptr, s, dev[1].ptr, s, dev[2].ptr, s, out.ptr, s, causal=True, cap=cap)
+    stream = kn.HipStream(hip_device)
+    kn.attention(hip_device, stream, args, kn.DeviceBuffer(hip_device, max(kn.attention_workspace_bytes(args), 1)))
+    stream.synchronize()
+    got, at, places = out.to_array(np.float16, q.shape), np.arange(queries) + keys - queries, np.arange(keys)
+    for h in range(2):
+        e, bound = attend(*(x[:, h].astype(np.float64) for x in (q, k, v)), at, places, places <= at[:, None], float(np.float32(width ** -0.5)), float(np.float32(cap)), 0.0)
+        off = np.abs(got[:, h].astype(np.float64) - e)
+        assert (off <= bound).all(), f"{np.max(off / bound):.2f} of the bound, {np.max(off):.3e} off"
