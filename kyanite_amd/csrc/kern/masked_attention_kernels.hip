@@ -15,7 +15,9 @@
 //                           a prefix has its own part and the prefix's
 // Scores are computed transposed, S^T = K Q^T, so that a lane owns a query and the accumulators of S^T are the operands of
 // O^T += V^T P^T. The softmax runs in f32 in units of log2, with a running reference that follows the maximum lazily:
-// it moves when a score exceeds it by more than 2^8, weights are at most 256 until then.
+// it moves when a score exceeds it by more than SLACK. Weights enter the second product as f16 and are 2^LIFT at the reference, so that
+// they use the type's range: at most 2^15, and normal numbers (rounded by half of 2^-10, the type's step) down to 2^-21 of the
+// reference's. Their sum is that of the f32 numbers before the rounding, times 2^LIFT like them.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -41,7 +43,7 @@ typedef float floatx4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 constexpr float LOG2E = 1.44269504088896340736f;
-constexpr float SLACK = 8.0f;
+constexpr float SLACK = 8.0f, LIFT = 7.0f;
 constexpr int WAVES = 4;
 
 // ---- which keys a query sees ---------------------------------------------------------------------------------------
@@ -550,7 +552,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
                 for (int v = 0; v < 16; v++) oacc[t][v] *= alpha;
         }
-        const float minus = ref == -INFINITY ? 0.0f : ref;
+        const float minus = ref == -INFINITY ? 0.0f : ref - LIFT;
         halfx8 pv[4];
 #pragma unroll
         for (int u = 0; u < 2; u++)
@@ -1035,7 +1037,7 @@ __global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
                     for (int d = 0; d < DPL; d++) oacc[n][d] *= alpha;
                 }
-                const float minus = ref[n] == -INFINITY ? 0.0f : ref[n];
+                const float minus = ref[n] == -INFINITY ? 0.0f : ref[n] - LIFT;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const float x = __builtin_amdgcn_exp2f(s2[e] - minus);

@@ -206,6 +206,26 @@ def test_values_of_different_magnitudes(form, spread, dtype, hip_device):
     case.check(case.run(hip_device), f"{form} {spread}")
 
 
+# ---- weights far below the largest ---------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [DType.I8, DType.F16], ids=lambda d: d.name)
+@pytest.mark.parametrize("first", [True, False], ids=["sink_first", "sink_last"])
+@pytest.mark.parametrize("form", FORMS)
+def test_weights_far_below_the_largest(form, first, dtype, hip_device):
+    """one key of no value takes most of the weight, all others get the same 2^-17 or so of it: a number in the middle between two
+    multiples of 2^-24"""
+    case = Case(dtype, scale=1.0, **FORMS[form])
+    case.q[:], case.k[:], case.v[:] = 0, 0, 1.0
+    case.q[..., 0] = 1
+    scores = np.arange(-12, -11.5, 2.0 ** -7)  # numbers of f16
+    case.k[..., 0] = scores[np.argmin(np.abs(np.exp(scores) * 2.0 ** 24 % 1 - 0.5))]
+    for b in range(len(case.lengths)):
+        sink = case.place(b, 0) if first else case.place(b, case.prefix + case.lengths[b] - case.queries)
+        case.k[sink], case.v[sink] = 0, 0
+    case.check(case.run(hip_device), form)
+
+
 # ---- caps ----------------------------------------------------------------------------------------------------------
 
 @pytest.mark.gpu
