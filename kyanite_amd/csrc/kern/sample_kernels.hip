@@ -327,7 +327,8 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         return;
     }
     const float t = p.temperature ? p.temperature[r] : 1.0f;
-    if (!(t > 0.0f)) {  // the first of the largest
+    const float min_p = p.min_p ? p.min_p[r] : 0.0f;
+    if (!(t > 0.0f) || min_p > 1.0f) {  // the first of the largest (no weight but the most probable token's stays above 1)
         int first = p.vocab;
         auto look = [&](int i, const Group &g) {
 #pragma unroll
@@ -351,7 +352,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     const Weigher weigh{top, 369.32993046757462751 / (double) t, p.bits, sh.roots};
     const int k = p.top_k ? p.top_k[r] : 0;
     const float top_p = p.top_p ? p.top_p[r] : 1.0f;
-    const double min_w = p.min_p ? __builtin_ldexp((double) p.min_p[r], p.bits) : 0.0;
+    const double min_w = min_p > 0.0f ? __builtin_ldexp((double) min_p, p.bits) : 0.0;  // (at most the weight of the maximum, which is exact)
     // distances at which w may be more than zero: exp(-range / T) 2^bits = 1 / 4
     const float range = t * (0.6931472f * (p.bits + 2)), per_bucket = fminf(BUCKETS / range, 3e38f);
     const bool spread = range < 1e37f && top < INFINITY;
@@ -562,7 +563,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
             const mass_t sums = sums_in_order(kept ? w : 0, rank), wanted = wanted_of(lane_of(sums, 63));
             // (in the order of the logits: those before which less than `wanted` lies)
             const int stay = top_p < 1.0f ? 1 + (int) __popcll(__ballot(sums < wanted)) : 64;
-            kept = kept && rank < stay && (x == top || weigh.real(x) >= min_w);
+            kept = kept && rank < stay && weigh.real(x) >= min_w;
             const mass_t parts = sums_in_order(kept ? w : 0, place), total = lane_of(parts, 63);
             const int chosen = (int) __popcll(__ballot(parts <= target_of(p.uniform[r], total)));
             if (listed && place == chosen) {
@@ -595,7 +596,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const float x = logit_of((unsigned) (entry[e] >> 32));
-                        kept[e] = kept[e] && (x == top || weigh.real(x) >= min_w);
+                        kept[e] = kept[e] && weigh.real(x) >= min_w;
                         if (kept[e]) mine += w[e];
                     }
                     (void) block_scan(mine, sh.wave_mass, &total);
@@ -693,7 +694,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
             mass_t *queue = sh.hist + 128 * wave;
             auto kept = [&](float x) -> mass_t {
                 const double w = weigh.near_real(x);
-                return w >= min_w || x == top ? Weigher::whole(w) : 0;
+                return w >= min_w ? Weigher::whole(w) : 0;
             };
             auto settle = [&](mass_t item) {
                 const float x = __builtin_bit_cast(float, (unsigned) (item >> 32));
@@ -794,7 +795,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     auto weight_of = [&](float x, int i) -> mass_t {
         if (x == -INFINITY || !stays(key_of(x), i)) return 0;
         const double w = weigh.real(x);
-        return w >= min_w || x == top ? Weigher::whole(w) : 0;
+        return w >= min_w ? Weigher::whole(w) : 0;
     };
     if (!masses_known) {
         mass_t mass = 0;

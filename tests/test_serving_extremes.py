@@ -4,7 +4,7 @@ import pytest
 
 import kyanite_amd as kn
 from kyanite_amd import DType
-from serving_oracle import upload
+from serving_oracle import sample, upload
 
 PAGE = 16
 
@@ -270,3 +270,41 @@ def test_caps_of_prompts(queries, keys, width, cap, hip_device):
         e, bound = attend(*(x[:, h].astype(np.float64) for x in (q, k, v)), at, places, places <= at[:, None], float(np.float32(width ** -0.5)), float(np.float32(cap)), 0.0)
         off = np.abs(got[:, h].astype(np.float64) - e)
         assert (off <= bound).all(), f"{np.max(off / bound):.2f} of the bound, {np.max(off):.3e} off"
+
+
+# ---- sampling ------------------------------------------------------------------------------------------------------
+
+def _draw(device, logits, uniform, **filters):
+    """(tokens, probabilities) of f32 rows"""
+    types = dict(temperature=np.float32, top_k=np.int32, top_p=np.float32, min_p=np.float32)
+    rows, vocab = logits.shape
+    dev = {n: upload(device, np.full(rows, v, types[n])) for n, v in filters.items()}
+    x, u = upload(device, logits.astype(np.float32)), upload(device, uniform.astype(np.float32))
+    tokens, chance = upload(device, np.full(rows, -7, np.int32)), upload(device, np.full(rows, -7, np.float32))
+    args = kn.sample_args(DType.F32, rows, vocab, x.ptr, vocab, u.ptr, tokens.ptr, probabilities=chance.ptr, **{n: d.ptr for n, d in dev.items()})
+    stream = kn.HipStream(device)
+    kn.sample(device, stream, args)
+    stream.synchronize()
+    return tokens.to_array(np.int32, rows), chance.to_array(np.float32, rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("min_p", [1.0000001, 2.0, np.inf])
+@pytest.mark.parametrize("filters", [{}, dict(top_k=7), dict(top_k=100), dict(top_k=3000), dict(top_p=0.9), dict(top_k=2000, top_p=0.9, temperature=0.5)], ids=str)
+def test_min_p_beyond_one_keeps_the_first_of_equal_maxima(filters, min_p, hip_device):
+    rng = np.random.default_rng(1)
+    x = np.round(rng.standard_normal((40, 5000)) * 2).clip(-3, 3)  # tens of equal maxima per row
+    x[1] = 0
+    x[2, 4000:] = np.inf
+    tokens, chance = _draw(hip_device, x, rng.random(40), min_p=min_p, **filters)
+    assert np.array_equal(tokens, x.argmax(-1)) and (chance == 1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("min_p", [np.nan, -1.0, 0.0])
+@pytest.mark.parametrize("filters", [{}, dict(top_k=40), dict(top_p=0.9)], ids=str)
+def test_min_p_that_is_no_positive_number_is_off(filters, min_p, hip_device):
+    rng = np.random.default_rng(2)
+    x, u = rng.standard_normal((30, 3000)), rng.random(30)
+    for a, b in zip(_draw(hip_device, x, u, min_p=min_p, **filters), _draw(hip_device, x, u, **filters)):
+        assert np.array_equal(a, b)
