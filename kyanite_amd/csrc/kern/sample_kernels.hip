@@ -354,8 +354,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     const float top_p = p.top_p ? p.top_p[r] : 1.0f;
     const double min_w = min_p > 0.0f ? __builtin_ldexp((double) min_p, p.bits) : 0.0;  // (at most the weight of the maximum, which is exact)
     // distances at which w may be more than zero: exp(-range / T) 2^bits = 1 / 4
-    const float range = t * (0.6931472f * (p.bits + 2)), per_bucket = fminf(BUCKETS / range, 3e38f);
-    const bool spread = range < 1e37f && top < INFINITY;
+    const float range = t * (0.6931472f * (p.bits + 2)), per_bucket = BUCKETS / range;
+    // (not for temperatures so low or high that f32 cannot hold buckets which end at the range, on which near() relies)
+    const bool spread = range < 1e37f && per_bucket < 3e38f && top < INFINITY;
     auto bucket_of = [&](float x) { return (unsigned) ((top - x) * per_bucket); };  // (saturates: -inf falls behind the last)
     unsigned last_key = 0;  // what stays: larger keys, and this key up to last_index
     int last_index = p.vocab;

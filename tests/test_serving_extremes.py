@@ -308,3 +308,22 @@ def test_min_p_that_is_no_positive_number_is_off(filters, min_p, hip_device):
     x, u = rng.standard_normal((30, 3000)), rng.random(30)
     for a, b in zip(_draw(hip_device, x, u, min_p=min_p, **filters), _draw(hip_device, x, u, **filters)):
         assert np.array_equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temperature", [1e-45, 1e-41, 1e-39, 1e-38, 3e-38, 1e-37, 3e-37, 1e-36, 1e-30, 1e30, 1e35, 3e35, 1e36])
+@pytest.mark.parametrize("filters", [dict(top_p=0.9), dict(top_k=40), dict(top_k=3000, top_p=0.95), dict(min_p=0.05), {}], ids=str)
+def test_temperatures_at_both_ends_of_the_range(filters, temperature, hip_device):
+    """logits a few temperatures apart, so that several tokens have weight"""
+    rng = np.random.default_rng(3)
+    temperature = np.float32(temperature)
+    x = (rng.standard_normal((12, 5000)) * 2.5 * float(temperature)).astype(np.float32)
+    x[0, 7], x[1, 8] = np.inf, -np.inf
+    x[2] = np.round(x[2] / temperature) * temperature  # few values
+    u = rng.random(12).astype(np.float32)
+    each = {n: np.full(12, v, np.int32 if n == "top_k" else np.float32) for n, v in dict(filters, temperature=temperature).items()}
+    expected, probability = sample(x, u, **each)
+    tokens, chance = _draw(hip_device, x, u, temperature=temperature, **filters)
+    assert np.array_equal(tokens, expected)
+    # (weights are off by half of 2^-49 each, f32 rounds by 2^-24 of the value)
+    assert (np.abs(chance - probability) <= probability * 2.0 ** -23 + 5000 * 2.0 ** -49).all()
