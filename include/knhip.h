@@ -192,7 +192,7 @@ void knhip_kernel_free(knhip_kernel *kernel);
  * Addresses are device addresses with the alignment of their element; strides are in elements, may be zero or negative
  * in operands that are only read, and the axis along a row's `width` is contiguous. Sizes, codes and addresses are checked
  * on the host before anything is launched; rows that are written are refused where their strides let two of them share
- * memory, and so are calls beyond one launch (2^27 rows of a cache, 2^22 pairs of a sequence and a head of keys). Lengths,
+ * memory, and so are calls beyond one launch (2^27 - 7 rows of a cache, 2^22 pairs of a sequence and a head of keys). Lengths,
  * slots and page numbers are device data and cannot be checked: entries out of range are skipped, as the operators say,
  * and never reach outside the buffers. */
 

@@ -104,7 +104,8 @@ bool check_rows(const char *what, const knhip_kv_cache *cache, const knhip_cache
     check_cache_sizes(what, *cache);
     if (rows->dtype != KNHIP_F16 && rows->dtype != KNHIP_F32) fail(what, ": rows are f16 or f32, got dtype code ", rows->dtype);
     if (rows->tokens < 0) fail(what, ": negative size");
-    if ((long long) rows->tokens * cache->heads > INT_MAX / 16) fail(what, ": tokens * heads must stay below 2^27");
+    // (a launch has less than 2^32 threads, in workgroups of 8 rows or more with up to 32 lanes each)
+    if ((long long) rows->tokens * cache->heads > (1 << 27) - 8) fail(what, ": tokens * heads must stay below 2^27 - 7");
     if (rows->tokens == 0 || cache->heads == 0) return true;
     if (cache->pages > 0) check_cache_addresses(what, *cache);
     const size_t elem = rows->dtype == KNHIP_F16 ? 2 : 4;

@@ -327,3 +327,15 @@ def test_temperatures_at_both_ends_of_the_range(filters, temperature, hip_device
     assert np.array_equal(tokens, expected)
     # (weights are off by half of 2^-49 each, f32 rounds by 2^-24 of the value)
     assert (np.abs(chance - probability) <= probability * 2.0 ** -23 + 5000 * 2.0 ** -49).all()
+
+
+# ---- sizes ---------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("call", [kn.cache_write, kn.cache_read])
+@pytest.mark.parametrize("tokens,heads", [((1 << 27) - 7, 1), (1 << 27, 1), ((1 << 24) - 1, 8 + 1), ((1 << 31) - 1, 1)])
+def test_more_rows_than_a_launch_holds_are_refused(call, tokens, heads):
+    """(made up addresses: refused by size before anything else is looked at)"""
+    cache = kn.kv_cache(DType.F16, 1 << 20, heads, 128, 256, 256, 512)
+    rows = kn.cache_rows(DType.F16, tokens, 256, (heads * 256, 256), 512, (heads * 256, 256), 256)
+    with pytest.raises(kn.KnError, match="tokens \\* heads must stay below 2\\^27 - 7"):
+        call(0, 0, cache, rows)
