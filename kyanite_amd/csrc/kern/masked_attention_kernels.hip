@@ -670,28 +670,56 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 // every sequence's own keys) are cut into items of about the same size, ROW_ITEMS of them over all heads, and workgroup x
 // takes item x / kv_heads. The grid covers the largest number of items that any lengths can give. Parts of less than
 // ROW_MIN_KEYS keys are not made: four steps per wave take less time than the launch that joins two parts.
+// Every wave looks its item up in the lengths of all sequences, 64 at a time. That takes each round of workgroups the longer the more
+// sequences there are, so that for many of them a launch of one workgroup makes a list of the items first (LIST_FROM: sequences
+// times pairs of a sequence and a head of keys). Looked up / listed, us, sequences x heads of keys x keys: 256 x 1 x 16 8.9 / 10.2,
+// 96 x 8 x 200 25.2 / 25.7, 128 x 8 x 200 32.7 / 31.7, 256 x 8 x 200 68 / 55, 384 x 1 x 16 16.8 / 15.0, 1024 x 8 x 200 466 / 235,
+// 65536 x 1 x 16 120700 / 1500.
 constexpr int ROW_ITEMS = 512, ROW_MIN_KEYS = 1024, ROW_WAVES = 8, ROW_THREADS = 64 * ROW_WAVES;
+constexpr int LIST_FROM = 1 << 17, LIST_THREADS = 1024, NO_ITEM = -2;
 
 struct Item {
     int seg, length, from, end, nth, items;
 };
 
+// (length, first key that any row may see: a multiple of 32) of a sequence's own keys
+__device__ __forceinline__ int2 own_range(const ServingAttentionParams &p, int b) {
+    const int n = own_length(p, b);
+    return int2{n, p.window ? max(0, n - p.queries + 1 - p.window) & ~31 : 0};
+}
+__device__ __forceinline__ int steps_of(int2 range) { return (range.x - range.y + 31) / 32; }
+// steps per item, out of those of all stretches; no stretch has more than 2^26
+__device__ __forceinline__ int steps_per_item(const ServingAttentionParams &p, long long steps) {
+    return max(ROW_MIN_KEYS / 32, (int) min((steps * p.kv_heads + ROW_ITEMS - 1) / ROW_ITEMS, 1ll << 26));
+}
+__device__ __forceinline__ int items_of(int steps, int each) { return max(1, (steps + each - 1) / each); }
+
+// the n-th of a segment's items, all of which have the same number of steps, but for the last
+__device__ __forceinline__ void cut_item(int2 range, int steps, int nth, int items, Item &out) {
+    const int per = 32 * ((steps + items - 1) / items);
+    out.length = range.x;
+    out.items = items;
+    out.nth = nth;
+    out.from = min(range.y + nth * per, range.x);
+    out.end = min(range.y + nth * per + per, range.x);
+}
+
 // segments -1 (the prefix, when `with_prefix`) and 0 .. batch - 1; false when there is no such item. Every wave works it out
-// for itself, a lane per segment.
+// for itself, a lane per segment, or takes it from the list.
 __device__ __forceinline__ bool find_item(const ServingAttentionParams &p, int with_prefix, int item, Item &out) {
+    if (p.item_list) {
+        const int seg = __builtin_amdgcn_readfirstlane(p.item_list[item]);
+        if (seg == NO_ITEM) return false;
+        const int2 items = ((const int2 *) p.part_items)[seg + 1], range = own_range(p, seg);
+        out.seg = seg;
+        cut_item(range, steps_of(range), item - items.x, items.y, out);
+        return true;
+    }
     const int lane = threadIdx.x & 63, segs = p.batch + with_prefix;
-    auto range = [&](int s) {  // (length, first key that any row may see: a multiple of 32)
-        if (s >= segs) return int2{0, 0};
-        if (s < with_prefix) return int2{p.prefix_tokens, 0};
-        const int n = own_length(p, s - with_prefix);
-        return int2{n, p.window ? max(0, n - p.queries + 1 - p.window) & ~31 : 0};
-    };
+    auto range = [&](int s) { return s >= segs ? int2{0, 0} : s < with_prefix ? int2{p.prefix_tokens, 0} : own_range(p, s - with_prefix); };
     const int2 first = range(lane);
     long long steps = 0;  // of 32 keys, of all stretches (64 bits: many long tables may share pages)
-    for (int s0 = 0; s0 < segs; s0 += 64) {
-        const int2 r = s0 ? range(s0 + lane) : first;
-        steps += (r.x - r.y + 31) / 32;
-    }
+    for (int s0 = 0; s0 < segs; s0 += 64) steps += steps_of(s0 ? range(s0 + lane) : first);
     if (segs <= 64) {
         unsigned few = (unsigned) steps;  // (at most 64 stretches of 2^25 steps)
 #pragma unroll
@@ -701,12 +729,11 @@ __device__ __forceinline__ bool find_item(const ServingAttentionParams &p, int w
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) steps += __shfl_xor(steps, m);
     }
-    // steps per item; no stretch has more than 2^26
-    const int each = max(ROW_MIN_KEYS / 32, (int) min((steps * p.kv_heads + ROW_ITEMS - 1) / ROW_ITEMS, 1ll << 26));
+    const int each = steps_per_item(p, steps);
     int base = 0;
     for (int s0 = 0; s0 < segs; s0 += 64) {
         const int2 r = s0 ? range(s0 + lane) : first;
-        const int own_steps = (r.x - r.y + 31) / 32, n = s0 + lane < segs ? max(1, (own_steps + each - 1) / each) : 0;
+        const int own_steps = steps_of(r), n = s0 + lane < segs ? items_of(own_steps, each) : 0;
         int sums = n;
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) {
@@ -716,21 +743,54 @@ __device__ __forceinline__ bool find_item(const ServingAttentionParams &p, int w
         const int before = base + sums - n;
         const unsigned long long hit = __ballot(n > 0 && item >= before && item < before + n);
         if (hit) {
-            // the items of a stretch have the same number of steps, but for the last
-            const int l = __builtin_ctzll(hit), begin = __builtin_amdgcn_readlane(r.y, l), nth = item - __builtin_amdgcn_readlane(before, l);
-            out.items = __builtin_amdgcn_readlane(n, l);
+            const int l = __builtin_ctzll(hit);
             out.seg = s0 + l - with_prefix;
-            out.length = __builtin_amdgcn_readlane(r.x, l);
-            const int per = 32 * ((__builtin_amdgcn_readlane(own_steps, l) + out.items - 1) / out.items);
-            out.nth = nth;
-            out.from = min(begin + nth * per, out.length);
-            out.end = min(begin + nth * per + per, out.length);
-            if (nth == 0 && threadIdx.x == 0) ((int2 *) p.part_items)[out.seg + 1] = int2{item, out.items};
+            cut_item(int2{__builtin_amdgcn_readlane(r.x, l), __builtin_amdgcn_readlane(r.y, l)}, __builtin_amdgcn_readlane(own_steps, l),
+                     item - __builtin_amdgcn_readlane(before, l), __builtin_amdgcn_readlane(n, l), out);
+            if (out.nth == 0 && threadIdx.x == 0) ((int2 *) p.part_items)[out.seg + 1] = int2{item, out.items};
             return true;
         }
         base += __builtin_amdgcn_readlane(sums, 63);
     }
     return false;
+}
+
+// The items of all sequences' own keys: a thread per sequence, one workgroup. part_items as find_item() writes them, and the
+// sequence of each of the `items` that there may be.
+__global__ __launch_bounds__(LIST_THREADS) void list_items_kernel(ServingAttentionParams p, int items) {
+    constexpr int NWAVES = LIST_THREADS / 64;
+    __shared__ long long wave_steps[NWAVES];
+    __shared__ int wave_items[2][NWAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    long long steps = 0;
+    for (int b = threadIdx.x; b < p.batch; b += LIST_THREADS) steps += steps_of(own_range(p, b));
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) steps += __shfl_xor(steps, m);
+    if (lane == 0) wave_steps[wave] = steps;
+    __syncthreads();
+    steps = 0;
+    for (int w = 0; w < NWAVES; w++) steps += wave_steps[w];
+    const int each = steps_per_item(p, steps);
+    int base = 0;
+    for (int b0 = 0, turn = 0; b0 < p.batch; b0 += LIST_THREADS, turn ^= 1) {
+        const int b = b0 + (int) threadIdx.x, n = b < p.batch ? items_of(steps_of(own_range(p, b)), each) : 0;
+        int sums = n;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int other = __shfl_up(sums, m);
+            if (lane >= m) sums += other;
+        }
+        if (lane == 63) wave_items[turn][wave] = sums;
+        __syncthreads();  // (two buffers: one barrier per turn keeps writers away from readers)
+        int at = base + sums - n;
+        for (int w = 0; w < NWAVES; w++) {
+            if (w < wave) at += wave_items[turn][w];
+            base += wave_items[turn][w];
+        }
+        if (b < p.batch) ((int2 *) p.part_items)[b + 1] = int2{at, n};
+        for (int i = at; i < at + n && i < items; i++) p.item_list[i] = b;
+    }
+    for (int i = base + (int) threadIdx.x; i < items; i += LIST_THREADS) p.item_list[i] = NO_ITEM;
 }
 
 template <int WORDS>
@@ -1247,6 +1307,7 @@ struct Plan {
     int own_rows;             // per sequence and head of keys
     long long prefix_rows;
     bool own_in_rows, prefix_in_rows;  // which kernel
+    bool list;                         // of the row kernel's items
     bool prefix_inside;                // of every sequence's own rows, see row_attention_kernel
     long long own_tiles, prefix_tiles;
     int own_splits, prefix_splits;     // of the tile kernel
@@ -1317,6 +1378,7 @@ Plan plan_for(const ServingAttentionParams &p) {
         long long by_keys = p.batch * std::max(1ll, ((long long) p.table_tokens + ROW_MIN_KEYS - 1) / ROW_MIN_KEYS);
         if (l.prefix_in_rows) by_keys += std::max(1, (p.prefix_tokens + ROW_MIN_KEYS - 1) / ROW_MIN_KEYS);
         l.items = std::min(stretches + ROW_ITEMS / p.kv_heads, by_keys);
+        l.list = p.batch > 64 && p.batch * pairs >= LIST_FROM;  // (a prefix in this kernel has rows of 32 sequences at most)
         l.own_parts = l.items * p.kv_heads * l.own_rows;
         if (l.prefix_in_rows) l.prefix_parts = l.items * p.kv_heads * l.prefix_rows;
     }
@@ -1390,12 +1452,13 @@ int launch_join(const ServingAttentionParams &p, hipStream_t stream) {
 
 }  // namespace
 
-// partial values, then their references and sums, then the items of the row kernel
+// partial values, then their references and sums, then the items of the row kernel and their list
 size_t serving_attention_workspace(const ServingAttentionParams &p) {
     const Plan l = plan_for(p);
     const size_t parts = (size_t) (l.prefix_parts + l.own_parts);
     size_t bytes = round256(parts * l.wp * 4) + round256(parts * 8);
     if (l.own_in_rows) bytes += round256(((size_t) p.batch + 1) * 8);
+    if (l.list) bytes += round256((size_t) l.items * 4);
     return bytes;
 }
 
@@ -1407,6 +1470,7 @@ int launch_serving_attention(const ServingAttentionParams &given, void *workspac
     p.queries_div = FastDiv((uint32_t) p.queries);
     float *values = (float *) workspace, *stats = (float *) ((char *) workspace + round256(parts * l.wp * 4));
     p.part_items = l.own_in_rows ? (int32_t *) ((char *) stats + round256(parts * 8)) : nullptr;
+    p.item_list = l.list ? (int32_t *) ((char *) p.part_items + round256(((size_t) p.batch + 1) * 8)) : nullptr;
     p.row_prefix_part = 0;
     p.row_own_part = l.prefix_parts;
     p.prefix_inside = l.prefix_inside;
@@ -1431,6 +1495,11 @@ int launch_serving_attention(const ServingAttentionParams &given, void *workspac
         p.part_values = values;
         p.part_stats = stats;
         const unsigned workgroups = (unsigned) (l.items * p.kv_heads);
+        if (l.list) {
+            hipLaunchKernelGGL(list_items_kernel, dim3(1), dim3(LIST_THREADS), 0, stream, p, (int) l.items);
+            const int e = (int) hipGetLastError();
+            if (e != 0) return e;
+        }
         const bool two_tiles = (l.prefix_in_rows ? l.prefix_rows : l.own_rows) > 16;
         const int e = l.wp == 64 ? launch_rows_for<64>(p, workgroups, two_tiles, l.prefix_in_rows, stream) : launch_rows_for<128>(p, workgroups, two_tiles, l.prefix_in_rows, stream);
         if (e != 0) return e;

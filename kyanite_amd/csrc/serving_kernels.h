@@ -69,6 +69,7 @@ struct ServingAttentionParams {
     FastDiv group_div, queries_div;
     float *part_values, *part_stats;  // [row][width], [row][reference, sum]
     int32_t *part_items;  // [stretch][first item, items], the prefix first
+    int32_t *item_list;   // [item]: its sequence; null: looked up in the lengths (without a prefix among the stretches)
     long long row_prefix_part, row_own_part;
     int prefix_splits, own_splits;
     int prefix_inside;  // the workgroups of a sequence's own keys take the prefix as well

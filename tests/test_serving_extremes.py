@@ -134,6 +134,46 @@ FORMS = {
 }
 
 
+# ---- many sequences ------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    dict(lengths=[(37 * i) % 50 for i in range(400)]),                                                  # every item a sequence
+    dict(lengths=[(37 * i) % 50 for i in range(399)] + [2500], dtype=DType.I8, width=16),               # one of them in parts
+    dict(lengths=[2500] + [1] * 400 + [0, 1500], group=1, width=32),
+    dict(lengths=[(11 * i) % 90 for i in range(300)], kv=2, width=128, queries=3, window=20, page=5),
+    dict(lengths=[(11 * i) % 90 for i in range(500)], prefix=30, dtype=DType.I8),                        # a prefix beside the own keys
+    dict(lengths=[(11 * i) % 90 for i in range(400)], prefix=1900, group=1),                             # a prefix in tiles
+], ids=["one_item_each", "one_in_parts", "long_and_empty", "window", "prefix_inside", "prefix_apart"])
+def test_many_sequences(case, hip_device):
+    """so many that their items are listed"""
+    c = Case(**dict(dict(dtype=DType.F16), **case))
+    for call in range(2):
+        c.check(c.run(hip_device), f"call {call}")
+
+
+@pytest.mark.gpu
+def test_time_grows_with_the_number_of_sequences(hip_device):
+    """sixteen times the sequences take less than 64 times as long: their number, not its square"""
+    W, times = 64, []
+    stream = kn.HipStream(hip_device)
+    for B in (4096, 65536):
+        rows, out = upload(hip_device, np.zeros(B * W, np.float16)), kn.DeviceBuffer(hip_device, B * W * 2)
+        lengths, tables = upload(hip_device, np.ones(B, np.int32)), upload(hip_device, np.arange(B, dtype=np.int32))
+        cache = kn.kv_cache(DType.F16, B, 1, 1, W, rows.ptr, rows.ptr)
+        args = kn.cached_attention_args(B, 1, 1, cache, rows.ptr, (W, W, W), out.ptr, (W, W, W), lengths.ptr, tables.ptr, 1, 1)
+        workspace = kn.DeviceBuffer(hip_device, max(kn.cached_attention_workspace_bytes(args), 1))
+        seconds = []
+        for _ in range(4):
+            start = stream.record_event()
+            kn.cached_attention(hip_device, stream, args, workspace)
+            end = stream.record_event()
+            stream.synchronize()
+            seconds.append(end.time_elapsed_since(start))
+        times.append(min(seconds))
+    assert times[1] < 64 * times[0], times
+
+
 # ---- scales that nobody sees ---------------------------------------------------------------------------------------
 
 @pytest.mark.gpu
