@@ -4,6 +4,7 @@ Usage: python kyanite_amd/build.py [--force]  (run as a script: importing the pa
 """
 import hashlib
 import os
+import re
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -20,6 +21,10 @@ HOST_SOURCES = [
 ]
 DEVICE_SOURCES = ["kern/mfma_kernels.hip", "kern/mfma_f16_kernels.hip", "kern/attention_kernels.hip", "kern/attention_f16_kernels.hip",
                   "kern/static_scratch.hip", "kern/cache_kernels.hip", "kern/masked_attention_kernels.hip", "kern/sample_kernels.hip"]
+
+# kernels whose matrix instructions must leave their results in VGPRs: in AGPRs they have been read too early behind a branch
+RESULTS_IN_VGPRS = ["kern/masked_attention_kernels.hip"]
+RESOURCE_REPORT = "-Rpass-analysis=kernel-resource-usage"
 
 COMMON_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-D__HIP_PLATFORM_AMD__",
                 f"-I{ROCM}/include"]
@@ -44,6 +49,17 @@ def _headers_digest():
     return h.hexdigest()
 
 
+def check_no_agprs(src, report):
+    """`report`: what the compiler says about the registers of each kernel of `src`."""
+    kernels = re.findall(r"Function Name: (\S+)", report)
+    agprs = [int(n) for n in re.findall(r"\bAGPRs: (\d+)", report)]
+    if not kernels or len(kernels) != len(agprs):
+        raise RuntimeError(f"{src}: no report of the registers of {len(kernels) or 'any'} kernels")
+    using = [f"{name}: {n}" for name, n in zip(kernels, agprs) if n]
+    if using:
+        raise RuntimeError(f"{src}: kernels with AGPRs, whose matrix results may be read too early:\n" + "\n".join(using))
+
+
 def _compile(src, force, headers):
     path = os.path.join(CSRC, src)
     obj = os.path.join(BUILD_DIR, src.replace("/", "_") + ".o")
@@ -53,12 +69,18 @@ def _compile(src, force, headers):
     if not force and os.path.exists(obj) and os.path.exists(stamp) and open(stamp).read() == digest:
         return obj
     if src.endswith(".hip"):
-        cmd = [_hipcc(), "-c", path, "-o", obj] + COMMON_FLAGS + DEVICE_FLAGS
+        cmd = [_hipcc(), "-c", path, "-o", obj] + COMMON_FLAGS + DEVICE_FLAGS + ([RESOURCE_REPORT] if src in RESULTS_IN_VGPRS else [])
     else:
         cmd = ["g++", "-c", path, "-o", obj] + COMMON_FLAGS
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"compiling {src} failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    if src in RESULTS_IN_VGPRS:
+        try:
+            check_no_agprs(src, res.stderr)
+        except RuntimeError:
+            os.remove(obj)  # (nothing that failed is linked later)
+            raise
     with open(stamp, "w") as f:
         f.write(digest)
     return obj

@@ -814,7 +814,7 @@ __device__ __forceinline__ void load_words(const char *from, unsigned (&to)[WORD
 // number and address the whole wave shares, and lanes differ by 32 bit offsets
 template <int WP, int NT, bool I8, bool SHAPED, bool PAGE16, bool INSIDE>
 // (at least two waves per SIMD: with more registers than that leaves, the results of matrix instructions would lie in AGPRs, and
-// the compiler reads such a result too early behind a branch)
+// the compiler reads such a result too early behind a branch; the build refuses kernels of this file that have any)
 __global__ __launch_bounds__(ROW_THREADS) __attribute__((amdgpu_waves_per_eu(2))) void row_attention_kernel(ServingAttentionParams p, int with_prefix) {
     constexpr int ELEM = I8 ? 1 : 2;
     constexpr int KP = WP * ELEM / 64;    // 16 byte pieces of a key per lane
