@@ -34,6 +34,7 @@ int guarded(F f) {
 void select_device(int device) {
     HipDevice::check(device);
     hip_check(hipSetDevice(device), "hipSetDevice");
+    (void) hipGetLastError();  // (what an earlier call left, an allocation that failed for one, would be taken for the launch's)
 }
 
 void require_aligned(const char *what, const char *name, const void *ptr, size_t bytes) {

@@ -379,3 +379,27 @@ def test_more_rows_than_a_launch_holds_are_refused(call, tokens, heads):
     rows = kn.cache_rows(DType.F16, tokens, 256, (heads * 256, 256), 512, (heads * 256, 256), 256)
     with pytest.raises(kn.KnError, match="tokens \\* heads must stay below 2\\^27 - 7"):
         call(0, 0, cache, rows)
+
+
+# ---- errors of others ----------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+def test_an_error_that_an_earlier_call_left_is_not_reported_again(hip_device):
+    stream, W = kn.HipStream(hip_device), 64
+    mem = upload(hip_device, np.zeros(64 * W, np.float32))
+    slots = upload(hip_device, np.arange(4, dtype=np.int32))
+    zeros = upload(hip_device, np.zeros(64, np.int32))
+    out = kn.DeviceBuffer(hip_device, 64 * W * 4)
+    cache = kn.kv_cache(DType.F16, 4, 1, 16, W, mem.ptr, mem.ptr)
+    rows = kn.cache_rows(DType.F32, 4, out.ptr, (2 * W, W), out.ptr + 4 * W, (2 * W, W), slots.ptr)
+    cached = kn.cached_attention_args(1, 1, 1, cache, mem.ptr, (W, W, W), out.ptr, (W, W, W), zeros.ptr, zeros.ptr, 1, 1)
+    prompt = kn.attention_args(1, 4, 4, 1, 1, W, mem.ptr, (0, W, W), mem.ptr, (0, W, W), mem.ptr, (0, W, W), out.ptr, (0, W, W))
+    draw = kn.sample_args(DType.F32, 1, 64, mem.ptr, 64, mem.ptr, zeros.ptr)
+    workspace = kn.DeviceBuffer(hip_device, max(kn.cached_attention_workspace_bytes(cached), kn.attention_workspace_bytes(prompt), 1))
+    for call in (lambda: kn.cache_write(hip_device, stream, cache, rows), lambda: kn.cache_read(hip_device, stream, cache, rows),
+                 lambda: kn.cached_attention(hip_device, stream, cached, workspace), lambda: kn.attention(hip_device, stream, prompt, workspace),
+                 lambda: kn.sample(hip_device, stream, draw)):
+        with pytest.raises(kn.KnError, match="hipMalloc"):
+            kn.DeviceBuffer(hip_device, 1 << 50)
+        call()
+        stream.synchronize()
