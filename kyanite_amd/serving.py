@@ -9,10 +9,10 @@ from .graph import DType
 from .runtime import HipStream, _index
 
 
-def _three(name, strides):
+def _three(name, strides, axes="batch, token, head"):
     strides = tuple(int(s) for s in strides)
     if len(strides) != 3:
-        raise KnError(f"{name} takes three strides (batch, token, head), got {strides}")
+        raise KnError(f"{name} takes three strides ({axes}), got {strides}")
     return strides
 
 
@@ -31,7 +31,7 @@ def kv_cache(dtype, pages, heads, page_tokens, width, k, v, k_scales=0, v_scales
     c.k, c.v, c.k_scales, c.v_scales = k, v, k_scales or None, v_scales or None
     if strides is None:
         strides = (heads * page_tokens * width, page_tokens * width, width)
-    c.page_stride, c.head_stride, c.token_stride = _three("a cache", strides)
+    c.page_stride, c.head_stride, c.token_stride = _three("a cache", strides, "page, head, token")
     return c
 
 

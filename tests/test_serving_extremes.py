@@ -403,3 +403,7 @@ def test_an_error_that_an_earlier_call_left_is_not_reported_again(hip_device):
             kn.DeviceBuffer(hip_device, 1 << 50)
         call()
         stream.synchronize()
+
+def test_strides_of_a_cache_are_named():
+    with pytest.raises(kn.KnError, match=r"three strides \(page, head, token\)"):
+        kn.kv_cache(DType.F16, 1, 1, 16, 64, 0, 0, strides=(64, 64))
