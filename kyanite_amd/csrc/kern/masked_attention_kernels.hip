@@ -1299,9 +1299,12 @@ __global__ __launch_bounds__(64 * WAVES) void join_attention_kernel(ServingAtten
 // Waves for the rows of a tile, 32 rows each. Whole numbers are widened as they are staged, work that eight waves share better
 // than four (16384 shared keys of width 128 for 256 rows of 8 heads, and what goes with them: 76 us against 99). f16 only
 // passes through; eight waves still stage once for twice the rows, which pays where that leaves tiles enough to even out
-// their lengths (32 heads: 8192 tokens 627 us against 663, 4096 tokens 175 against 190, but 2048 tokens 96 against 74). `rows`:
-// of a sequence and head of keys, `pairs` of which there are.
-int tile_waves(int wp, bool i8, long long rows, long long pairs) { return wp == 128 && (i8 || (rows >= 1024 && rows * pairs >= 1024 * 128)) ? 8 : 4; }
+// their lengths. Four / eight waves, us, causal prompts of 32 heads: 1024 tokens 32 / 46, 2048 67 / 84, 2816 93 / 99, 3328 119 / 118,
+// 3584 138 / 127, 4096 177 / 159, 5000 250 / 255, 8192 633 / 595; four prompts of 1024 tokens 59 / 54, of 2048 184 / 174; 4096
+// tokens in 4 documents 97 / 93, in 9 78 / 76, in 20 65 / 70; 8192 with a window of 256 79 / 83, of 1024 182 / 178. With 8 heads
+// the longer tiles win earlier (8192 tokens 241 / 213, but 12000 381 / 397). `rows`: of a sequence and head of keys,
+// `pairs` of which there are.
+int tile_waves(int wp, bool i8, long long rows, long long pairs) { return wp == 128 && (i8 || (rows >= 1024 && rows * pairs >= 7 << 14)) ? 8 : 4; }
 
 struct Plan {
     int own_rows;             // per sequence and head of keys
