@@ -201,7 +201,7 @@ void knhip_kernel_free(knhip_kernel *kernel);
  * (innermost first, an unpadded cache is [pages, heads, page_tokens, width]; a cache without pages is one of a single
  * page per sequence). KNHIP_F16 keeps the rows as they are. KNHIP_I8 keeps a row x as whole numbers q and one f32 scale:
  * scale = max |x| / 127, q = x / scale rounded to the nearest, ties to even (all zeros where the scale is zero), standing
- * for q * scale; the scales are dense arrays [pages, heads, page_tokens]. `width` is a multiple of 16 up to 256, `k` and `v`
+ * for q * scale, a scale is never negative; the scales are dense arrays [pages, heads, page_tokens]. `width` is a multiple of 16 up to 256, `k` and `v`
  * are 16 byte aligned and so are the strides in bytes; no two rows share memory. pages * page_tokens stays below 2^31. */
 typedef struct {
     int dtype; /* KNHIP_I8 or KNHIP_F16 */
@@ -241,7 +241,8 @@ int knhip_cache_read(int device, void *stream, const knhip_kv_cache *cache, cons
  *     out = sum_j softmax(z)_j v_j, or zeros where nothing is seen
  * A query that would stand before the sequence's own first token (lengths[b] < queries: a padded batch) gives zeros.
  * Lengths beyond table_pages * page_tokens count as that, negative ones as 0; the keys of a page number outside the cache
- * are not seen. q and out are f16; many shared tokens are read once for all sequences. Sums and statistics are f32, the
+ * are not seen. What no query sees may hold anything (slots behind a sequence's last key, keys in front of every window; scales of
+ * theirs that are not finite too). q and out are f16; many shared tokens are read once for all sequences. Sums and statistics are f32, the
  * weights enter the second product as f16. width: a multiple of 16 up to 128. */
 typedef struct {
     int batch, queries, heads;
@@ -314,7 +315,7 @@ typedef struct {
     const float *temperature; /* [rows], NULL: 1 */
     const int32_t *top_k;     /* [rows], NULL or <= 0: off */
     const float *top_p;       /* [rows], NULL or >= 1: off */
-    const float *min_p;       /* [rows], NULL or <= 0: off */
+    const float *min_p;       /* [rows], NULL or <= 0: off; above 1: the most probable token alone */
     const float *uniform;     /* [rows] */
     int32_t *tokens;          /* [rows] */
     float *probabilities;     /* [rows], may be NULL */

@@ -5,7 +5,7 @@
 // argument are f64: the nearest of 10^5 borders between tokens is then missed once in 10^10 rows or so.
 //
 // A row belongs to one workgroup of 16 waves, each of which owns a contiguous part of it. What bounds a row is the arithmetic
-// per logit of one compute unit, and the fetch rate of one (about 40 GB/s) for rows that do not fit LDS. So a row is read
+// per logit of one compute unit, and the fetch rate of one (60 GB/s where 64 of them read) for rows that do not fit LDS. So a row is read
 // once where it fits (f16: 53000 logits), and the maxima of its groups of 8 logits are kept beside it, so that later passes
 // touch only groups that can matter. The filters end in one threshold, the last token that stays in the order of falling
 // logits (ties: rising index):
