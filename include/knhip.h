@@ -242,7 +242,8 @@ int knhip_cache_read(int device, void *stream, const knhip_kv_cache *cache, cons
  * A query that would stand before the sequence's own first token (lengths[b] < queries: a padded batch) gives zeros.
  * Lengths beyond table_pages * page_tokens count as that, negative ones as 0; the keys of a page number outside the cache
  * are not seen. What no query sees may hold anything (slots behind a sequence's last key, keys in front of every window; scales of
- * theirs that are not finite too). q and out are f16; many shared tokens are read once for all sequences. Sums and statistics are f32, the
+ * theirs that are not finite too); an infinity among the values that a query sees makes that element infinite, or NaN where its
+ * weight is below 2^-32 of the largest. q and out are f16; many shared tokens are read once for all sequences. Sums and statistics are f32, the
  * weights enter the second product as f16. width: a multiple of 16 up to 128. */
 typedef struct {
     int batch, queries, heads;

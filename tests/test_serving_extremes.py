@@ -4,7 +4,7 @@ import pytest
 
 import kyanite_amd as kn
 from kyanite_amd import DType
-from serving_oracle import sample, upload
+from serving_oracle import Graph, sample, upload
 
 PAGE = 16
 
@@ -150,6 +150,41 @@ def test_many_sequences(case, hip_device):
     c = Case(**dict(dict(dtype=DType.F16), **case))
     for call in range(2):
         c.check(c.run(hip_device), f"call {call}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [DType.I8, DType.F16], ids=lambda d: d.name)
+def test_many_sequences_captured_and_replayed(dtype, hip_device):
+    """lengths that change from replay to replay move the items of the list: results are those of the call outside the graph"""
+    rng = np.random.default_rng(4)
+    B, W, table_pages = 400, 32, 100
+    pages = 150  # (sequences share them)
+    k, v = (rng.standard_normal((pages, 1, PAGE, W)) for _ in range(2))
+    held = [np.rint(x * 30).clip(-127, 127).astype(np.int8) if dtype == DType.I8 else x.astype(np.float16) for x in (k, v)]
+    mem = [upload(hip_device, x) for x in held]
+    scales = upload(hip_device, np.full(pages * PAGE, 1 / 30, np.float32))
+    q, tables = upload(hip_device, rng.standard_normal((B, 2, W)).astype(np.float16)), upload(hip_device, rng.integers(0, pages, (B, table_pages)).astype(np.int32))
+    lengths, out = kn.DeviceBuffer(hip_device, B * 4), kn.DeviceBuffer(hip_device, B * 2 * W * 2)
+    cache = kn.kv_cache(dtype, pages, 1, PAGE, W, mem[0].ptr, mem[1].ptr, *([scales.ptr] * 2 if dtype == DType.I8 else []))
+    args = kn.cached_attention_args(B, 1, 2, cache, q.ptr, (2 * W, 2 * W, W), out.ptr, (2 * W, 2 * W, W), lengths.ptr, tables.ptr, table_pages, table_pages)
+    workspace, other = (kn.DeviceBuffer(hip_device, kn.cached_attention_workspace_bytes(args)) for _ in range(2))
+    stream, graph, seen = kn.HipStream(hip_device), None, []
+    for replay in range(4):
+        n = rng.integers(0, 40, B).astype(np.int32)
+        n[rng.integers(0, B, replay)] = 1600  # some in parts
+        kn._lib.check(kn._lib.lib.knhip_memcpy_h2d(hip_device.index, lengths.ptr, n.ctypes.data, n.nbytes))
+        if graph is None:
+            with Graph(stream) as graph:
+                kn.cached_attention(hip_device, stream, args, workspace)
+        graph.launch()
+        stream.synchronize()
+        replayed = out.to_array(np.uint16, B * 2 * W)
+        kn.cached_attention(hip_device, stream, args, other)
+        stream.synchronize()
+        assert np.array_equal(replayed, out.to_array(np.uint16, B * 2 * W)), replay
+        assert (replayed.reshape(B, -1)[n == 0] == 0).all() and (replayed.reshape(B, -1)[n > 0] != 0).any(-1).all()
+        seen.append(replayed)
+    assert not np.array_equal(seen[0], seen[1])
 
 
 @pytest.mark.gpu
